@@ -362,6 +362,87 @@ int gpsr_active_sample(const double* data, int N, int D, int K, int n_pick, doub
                        void* stream);
 
 /*
+ * Example bank: predictions from ALL example windows instead of the few hundred an exact GP can hold.  No counterpart in
+ * the reference, which throws nine tenths of its candidates away (agpr.py:120-137); gpsr_predict is the unnormalised
+ * sibling over one patch's own training points.  The answer to a query q is the kernel-weighted mean of the examples'
+ * values, with weights proportional to exp(-|q - k_r|^2 * scale / 2) (GPSR_KERNEL_RBF, scale = 1 / lengthscale^2) or
+ * exp(scale * q.k_r) (GPSR_KERNEL_LINEAR); the RBF weights are evaluated as exp(scale * (q.k_r + offset_r)),
+ * offset_r = -|k_r|^2 / 2, which differs by a factor that the normalisation removes.
+ *
+ * A bank holds rows (key k_r, value v_r, `dim` columns each, for each of `heads` heads) in 4 or 8 bits:
+ *   codes    [pages][heads][page_rows][dim * bits / 8]  E2M1 pairs, low nibble first (4 bits), or E4M3 bytes (8 bits)
+ *   scales   [pages][heads][page_rows][dim / 32]        one byte for 32 columns: 2^(byte - 127); 255: all 32 are NaN
+ *   offset   [pages][heads][page_rows] f32              -|k_r|^2 / 2 of the held key (RBF), 0 (LINEAR)
+ *   centroid [pages][heads][dim] f32                    mean of the page's held keys
+ * (code and scale arrays 16-byte aligned).  A scale is the smallest power of two at which no value of its 32 is clipped,
+ * kept within 2^-110 .. 2^125 (4 bits) / 2^119 (8 bits); values are rounded to nearest, ties to the even code.  Column
+ * counts that are no multiple of 32 are padded with zeros by the caller.
+ * Rows of one batch entry (a bank of its own length) lie in the pages that its table row names: position r is row
+ * r % page_rows of page table[b][r / page_rows].  Table entries outside [0, pages) are allowed: their rows do not exist
+ * for a reader and are dropped by a writer.  One page may serve several entries for reading; a page that a call writes
+ * must appear once among the pages that the call writes.
+ *
+ * Queries and outputs: [B][T][q_heads][dim] of `dtype`, q_heads a multiple of heads (query head h reads bank head
+ * h / (q_heads / heads)).  skip (or NULL): [B][T][2] int32, query t of entry b does not see positions skip[0] <= r <
+ * skip[1] (leave-one-image-out).  A query that sees no row gets zeros (lse -inf).  Rows that a query does not see have no
+ * influence, whatever they hold.  Sums, maxima and exponentials are kept in 32 bits; queries and weights enter the matrix
+ * units as one (bf16), two (f16) or three (f32) bf16 terms, so that each type keeps its own precision.
+ */
+enum { GPSR_BF16 = 0, GPSR_F16 = 1, GPSR_F32 = 2 };
+typedef struct {
+  uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
+  float *offset, *centroid;
+  int64_t pages;
+  int32_t heads;      /* 1 .. 65535 */
+  int32_t page_rows;  /* 16, 32, 64, 128 or 256 */
+  int32_t dim;        /* 32, 64, 96, 128, 192 or 256 */
+  int32_t bits;       /* 4 or 8 */
+  int32_t kernel_id;  /* GPSR_KERNEL_RBF or GPSR_KERNEL_LINEAR */
+} gpsr_bank;
+
+/*
+ * Rounds and stores rows: k, v [B][T][heads][dim] with element strides kst / vst = {batch, row, head} (columns
+ * contiguous); row t < count[b] goes to position start[b] + t (start[b] < 0 or count[b] <= 0: nothing of entry b).
+ * Also refreshes offset, and the centroid of every page written to, over the page's rows up to the last one written (the
+ * bank ends there).  table: [B][table_pages] int32.
+ */
+int gpsr_bank_write(const gpsr_bank* bank, const int32_t* table, int B, int table_pages, const int32_t* start,
+                    const int32_t* count, const void* k, const void* v, int dtype, int T, const int64_t* kst,
+                    const int64_t* vst, void* stream);
+/* The values that positions start[b] .. start[b] + count[b] - 1 hold, rounded once to dtype: k, v [B][T][heads][dim]
+ * contiguous; rows that do not exist and rows t >= count[b] are zero. */
+int gpsr_bank_read(const gpsr_bank* bank, const int32_t* table, int B, int table_pages, const int32_t* start,
+                   const int32_t* count, void* k, void* v, int dtype, int T, void* stream);
+/*
+ * Attention over the whole bank.  q strides qst = {batch, row, head} in elements; out contiguous; lse [B][q_heads][T] f32
+ * or NULL: log sum_r exp(scale * (q.k_r + offset_r)).  length[b]: rows of entry b.  scale > 0.
+ * Two banks' answers are joined by their lse.
+ */
+size_t gpsr_bank_attend_workspace_bytes(const gpsr_bank* bank, int B, int table_pages, int T, int q_heads, int dtype);
+int gpsr_bank_attend(const gpsr_bank* bank, const int32_t* table, int B, int table_pages, const int32_t* length,
+                     const void* q, int dtype, int T, int q_heads, const int64_t* qst, float scale, const int32_t* skip,
+                     void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+/*
+ * The n_sel (1..64) best pages for each query and bank head: sel [B][T][heads][n_sel], logical page numbers (table
+ * columns) in ascending order, -1 behind the last one.  Score of a page with centroid c: the sum over the query heads of
+ * the bank head of q.c (- |c|^2 / 2 for RBF), in 64 bits; equal scores: the lower page first.  A page can be chosen if
+ * its table entry exists and it has a row below length[b] that the query does not skip.
+ */
+size_t gpsr_bank_select_workspace_bytes(const gpsr_bank* bank, int B, int table_pages, int T, int q_heads, int n_sel, int dtype);
+int gpsr_bank_select(const gpsr_bank* bank, const int32_t* table, int B, int table_pages, const int32_t* length,
+                     const void* q, int dtype, int T, int q_heads, const int64_t* qst, int n_sel, const int32_t* skip,
+                     int32_t* sel, void* workspace, size_t workspace_bytes, void* stream);
+/*
+ * Attention over chosen pages: sel [B][T][heads][n_sel] as gpsr_bank_select gives it.  Entries outside [0, table_pages)
+ * and repeats of an earlier entry are passed over; the order is free.
+ */
+size_t gpsr_bank_attend_pages_workspace_bytes(const gpsr_bank* bank, int B, int table_pages, int T, int q_heads, int n_sel, int dtype);
+int gpsr_bank_attend_pages(const gpsr_bank* bank, const int32_t* table, int B, int table_pages, const int32_t* length,
+                           const void* q, int dtype, int T, int q_heads, const int64_t* qst, const int32_t* sel, int n_sel,
+                           float scale, const int32_t* skip, void* out, float* lse, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/*
  * Kernel timing for bench.py's roofline line: HIP-event brackets around the
  * tagged launches, on the stream they are launched on.  No counterpart in the
  * reference (its only instrumentation is time.time() per image, gprsr.py:49-72).

@@ -4,18 +4,29 @@ The HIP library is the product path: there is NO CPU fallback.  If the shared
 object is missing or cannot be loaded, every compute entry point raises.
 """
 import ctypes
+import glob
 import os
 import subprocess
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("GPSR_LIB", os.path.join(_HERE, "libgpsr.so"))   # override: instrumented debug builds (tools/upd_trace.py)
-SRC = os.path.join(_HERE, "csrc", "gpsr_api.hip")
+_CSRC = os.path.join(_HERE, "csrc")
+SRC = os.path.join(_CSRC, "gpsr_api.hip")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-HIPCC_FLAGS = ["-O3", "--offload-arch=gfx950", "-shared", "-fPIC", "-ffp-contract=off"]
+# no packed float32 arithmetic: some of its forms have given wrong results on this hardware
+HIPCC_FLAGS = ["-O3", "--offload-arch=gfx950", "-shared", "-fPIC", "-ffp-contract=off",
+               "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 _lib = None
 
 c_void_p, c_int, c_float, c_size_t = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t
+
+
+class Bank(ctypes.Structure):
+    """gpsr_bank of include/gpsr.h."""
+    _fields_ = [(n, c_void_p) for n in ("k_codes", "k_scales", "v_codes", "v_scales", "offset", "centroid")] + [
+        ("pages", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in ("heads", "page_rows", "dim", "bits", "kernel_id")]
+
 
 # name -> (restype, argtypes); must list every symbol include/gpsr.h declares
 SIGNATURES = {
@@ -73,6 +84,17 @@ SIGNATURES = {
     "gpsr_active_sample_workspace_bytes": (c_size_t, [c_int]),
     "gpsr_active_sample": (c_int, [c_void_p, c_int, c_int, c_int, c_int, ctypes.c_double, ctypes.c_double,
                                    ctypes.c_double, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "gpsr_bank_write": (c_int, [c_void_p, c_void_p, c_int, c_int] + [c_void_p] * 4 + [c_int, c_int] + [c_void_p] * 3),
+    "gpsr_bank_read": (c_int, [c_void_p, c_void_p, c_int, c_int] + [c_void_p] * 4 + [c_int, c_int, c_void_p]),
+    "gpsr_bank_attend_workspace_bytes": (c_size_t, [c_void_p] + [c_int] * 5),
+    "gpsr_bank_attend": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p,
+                                 c_float] + [c_void_p] * 4 + [c_size_t, c_void_p]),
+    "gpsr_bank_select_workspace_bytes": (c_size_t, [c_void_p] + [c_int] * 6),
+    "gpsr_bank_select": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p,
+                                 c_int] + [c_void_p] * 3 + [c_size_t, c_void_p]),
+    "gpsr_bank_attend_pages_workspace_bytes": (c_size_t, [c_void_p] + [c_int] * 6),
+    "gpsr_bank_attend_pages": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int,
+                                       c_void_p, c_void_p, c_int, c_float] + [c_void_p] * 4 + [c_size_t, c_void_p]),
     "gpsr_sepfilter_u8": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p]),
     "gpsr_metrics_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
     "gpsr_metrics": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
@@ -80,14 +102,26 @@ SIGNATURES = {
 
 
 def build(force=False):
-    """Compile csrc/gpsr_api.hip for gfx950 into libgpsr.so (in-tree)."""
-    srcs = [SRC, os.path.join(_HERE, "csrc", "gpsr_kernels.hpp"),
-            os.path.join(os.path.dirname(_HERE), "include", "gpsr.h")]
-    if not force and os.path.exists(LIB_PATH) and all(
-            os.path.getmtime(LIB_PATH) >= os.path.getmtime(s) for s in srcs):
+    """Compile csrc/*.hip for gfx950 (one object per file, side by side) into libgpsr.so (in-tree)."""
+    from concurrent.futures import ThreadPoolExecutor
+    heads = glob.glob(os.path.join(_CSRC, "*.hpp")) + [os.path.join(os.path.dirname(_HERE), "include", "gpsr.h")]
+    srcs = sorted(glob.glob(os.path.join(_CSRC, "*.hip")))
+    newer = lambda path, than: os.path.exists(path) and all(os.path.getmtime(path) >= os.path.getmtime(t) for t in than)
+    if not force and newer(LIB_PATH, srcs + heads):
         return LIB_PATH
-    cmd = [HIPCC] + HIPCC_FLAGS + ["-o", LIB_PATH, SRC]
-    subprocess.run(cmd, check=True, cwd=_HERE)
+    objdir = os.path.join(_HERE, "build")
+    os.makedirs(objdir, exist_ok=True)
+    flags = [f for f in HIPCC_FLAGS if f != "-shared"]
+
+    def compile_one(src):
+        obj = os.path.join(objdir, os.path.basename(src) + ".o")
+        if force or not newer(obj, [src] + heads):
+            subprocess.run([HIPCC] + flags + ["-c", "-o", obj, src], check=True, cwd=_HERE)
+        return obj
+
+    with ThreadPoolExecutor(max_workers=min(8, len(srcs))) as pool:
+        objs = list(pool.map(compile_one, srcs))
+    subprocess.run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB_PATH] + objs, check=True, cwd=_HERE)
     return LIB_PATH
 
 

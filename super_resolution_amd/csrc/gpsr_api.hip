@@ -1,6 +1,7 @@
 // gpsr_api.hip -- C ABI (include/gpsr.h) over the gfx950 kernels.  No torch types; the only allocation is
 // the workspace of an optional gpsr_ctx (gpsr_create): every other buffer belongs to the caller.
 #include "gpsr_kernels.hpp"
+#include "gpsr_host.hpp"
 #include "../../include/gpsr.h"
 
 #include <math.h>
@@ -10,21 +11,14 @@
 
 static thread_local char g_err[256] = "";
 
-static int hip_fail(hipError_t e, const char* where) {
+int hip_fail(hipError_t e, const char* where) {
   snprintf(g_err, sizeof(g_err), "%s: %s", where, hipGetErrorString(e));
   return -2;
 }
-static int arg_fail(const char* what) {
+int arg_fail(const char* what) {
   snprintf(g_err, sizeof(g_err), "bad argument: %s", what);
   return -1;
 }
-#define CHECK_LAUNCH(where)                                 \
-  do {                                                      \
-    hipError_t e_ = hipGetLastError();                      \
-    if (e_ != hipSuccess) return hip_fail(e_, where);       \
-  } while (0)
-
-static inline size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 // ---------------------------------------------------------------- kernel timing (bench.py roofline)
 // Optional HIP-event brackets around tagged launches, on the stream the kernel is

@@ -4,6 +4,8 @@ PyTorch is plumbing here: it owns device memory and the HIP stream; all
 arithmetic on the path happens in libgpsr.so.  Every function requires CUDA
 (ROCm) tensors and raises otherwise -- there is no CPU path.
 """
+from typing import NamedTuple
+
 import numpy as np
 import torch
 
@@ -395,6 +397,172 @@ def active_sample(data, K, n_pick, bandwidth, w_rep, w_div):
     _lib.check(lib.gpsr_active_sample(_p(data, torch.float64), N, D, int(K), int(n_pick), float(bandwidth), float(w_rep), float(w_div),
                                       _p(idx, torch.int32), _p(rep), _p(ws), nbytes, _stream()), "gpsr_active_sample")
     return idx, rep
+
+
+# ------------------------------------------------------------ example bank
+BANK_GROUP = 32                              # columns that share a scale byte
+BANK_DIMS = (32, 64, 96, 128, 192, 256)
+BANK_PAGE_ROWS = (16, 32, 64, 128, 256)
+_BANK_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+class Bank(NamedTuple):
+    """Example windows in 4 or 8 bits (gpsr_bank of include/gpsr.h): the arrays of a bank, which bank_write fills and the
+    other bank_* functions read.  codes [pages,H,P,D*bits/8] uint8, scales [pages,H,P,D/32] uint8, offset [pages,H,P]
+    and centroid [pages,H,D] float32; kernel_id RBF or LINEAR.  bank_alloc makes an empty one."""
+    k_codes: torch.Tensor
+    k_scales: torch.Tensor
+    v_codes: torch.Tensor
+    v_scales: torch.Tensor
+    offset: torch.Tensor
+    centroid: torch.Tensor
+    bits: int = 4
+    kernel_id: int = RBF
+
+
+def bank_alloc(pages, heads, dim, page_rows=64, bits=4, kernel_id=RBF, device=None):
+    """An empty Bank: `pages` pages of `page_rows` rows for each of `heads` heads, `dim` columns for keys and for values."""
+    if bits not in (4, 8) or dim not in BANK_DIMS or page_rows not in BANK_PAGE_ROWS or pages < 1 or heads < 1:
+        raise _lib.GpsrError(f"bank_alloc: pages={pages}, heads={heads}, dim={dim} (one of {BANK_DIMS}), page_rows={page_rows} "
+                             f"(one of {BANK_PAGE_ROWS}), bits={bits} (4 or 8)")
+    if kernel_id not in (RBF, LINEAR):
+        raise _lib.GpsrError("bank_alloc: kernel_id must be RBF or LINEAR")
+    if device is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    u8 = lambda n: torch.zeros((pages, heads, page_rows, n), dtype=torch.uint8, device=device)
+    f32 = lambda n: torch.zeros((pages, heads, n), dtype=torch.float32, device=device)
+    width, groups = dim * bits // 8, dim // BANK_GROUP
+    return Bank(u8(width), u8(groups), u8(width), u8(groups), f32(page_rows), f32(dim), bits, kernel_id)
+
+
+def _bank(bank):
+    """The checked gpsr_bank of a Bank, and (pages, heads, page_rows, dim)."""
+    import ctypes
+    pages, H, P, width = bank.k_codes.shape
+    if bank.bits not in (4, 8):
+        raise _lib.GpsrError(f"bank: bits must be 4 or 8, got {bank.bits}")
+    D = width * 8 // bank.bits
+    want = ((pages, H, P, width), (pages, H, P, D // BANK_GROUP)) * 2 + ((pages, H, P), (pages, H, D))
+    got = tuple(tuple(t.shape) for t in bank[:6])
+    if got != want:
+        raise _lib.GpsrError(f"bank: array shapes {got}, expected {want}")
+    ptrs = [_p(t, torch.uint8) for t in bank[:4]] + [_p(t, torch.float32) for t in bank[4:6]]
+    s = _lib.Bank(*ptrs, pages, H, P, D, bank.bits, bank.kernel_id)
+    return ctypes.byref(s), (pages, H, P, D)
+
+
+def _strided(t, shape, what):
+    """Pointer, dtype code and (first three) element strides of a [B,T,H,D] tensor whose columns are contiguous."""
+    import ctypes
+    if t.dim() != 4 or any(w is not None and w != g for w, g in zip(shape, t.shape)):
+        raise _lib.GpsrError(f"{what}: expected [B,T,heads,dim] = {shape}, got {tuple(t.shape)}")
+    if t.dtype not in _BANK_TYPES:
+        raise _lib.GpsrError(f"{what}: expected bfloat16, float16 or float32, got {t.dtype}")
+    if t.shape[3] > 1 and t.stride(3) != 1:
+        raise _lib.GpsrError(f"{what}: the columns must be contiguous")
+    _p(t.as_strided((0,), (1,)))     # device checks
+    return t.data_ptr(), _BANK_TYPES[t.dtype], (ctypes.c_int64 * 3)(*t.stride()[:3])
+
+
+def _bank_index(table, per_entry, what):
+    """Pointers of table [B,J] and of one int32 per entry."""
+    if table.dim() != 2 or any(t.shape != (table.shape[0],) for t in per_entry):
+        raise _lib.GpsrError(f"{what}: expected a [B,J] table and [B] integers, got {tuple(table.shape)}, "
+                             f"{[tuple(t.shape) for t in per_entry]}")
+    return _p(table, torch.int32), [_p(t, torch.int32) for t in per_entry]
+
+
+def bank_write(bank, table, start, count, k, v):
+    """Rounds rows k, v [B,T,H,D] (bfloat16 / float16 / float32, any strides with contiguous columns) into the bank, in place:
+    row t < count[b] goes to position start[b] + t of entry b, whose pages table [B,J] (int32) names; refreshes offsets and
+    centroids (gpsr_bank_write).  A page may be written by one entry of a call only."""
+    lib = _lib.load()
+    ref, (_, H, P, D) = _bank(bank)
+    tp, (sp, cp) = _bank_index(table, (start, count), "bank_write")
+    B = table.shape[0]
+    kp, dt, kst = _strided(k, (B, None, H, D), "bank_write: k")
+    if v.shape != k.shape or v.dtype != k.dtype:
+        raise _lib.GpsrError(f"bank_write: v {tuple(v.shape)} {v.dtype} does not fit k {tuple(k.shape)} {k.dtype}")
+    vp, _, vst = _strided(v, (B, None, H, D), "bank_write: v")
+    _lib.check(lib.gpsr_bank_write(ref, tp, B, table.shape[1], sp, cp, kp, vp, dt, k.shape[1], kst, vst, _stream()), "gpsr_bank_write")
+
+
+def bank_read(bank, table, start, count, rows, dtype=torch.float32):
+    """-> k, v [B,rows,H,D]: the values that positions start[b] .. start[b] + count[b] - 1 hold, zeros behind them (gpsr_bank_read)."""
+    lib = _lib.load()
+    ref, (_, H, P, D) = _bank(bank)
+    tp, (sp, cp) = _bank_index(table, (start, count), "bank_read")
+    if dtype not in _BANK_TYPES:
+        raise _lib.GpsrError(f"bank_read: expected bfloat16, float16 or float32, got {dtype}")
+    B = table.shape[0]
+    k, v = (torch.empty((B, rows, H, D), dtype=dtype, device=table.device) for _ in range(2))
+    _lib.check(lib.gpsr_bank_read(ref, tp, B, table.shape[1], sp, cp, k.data_ptr(), v.data_ptr(), _BANK_TYPES[dtype], rows,
+                                  _stream()), "gpsr_bank_read")
+    return k, v
+
+
+def _bank_query(bank, table, length, q, skip, what):
+    ref, (_, H, P, D) = _bank(bank)
+    tp, (lp,) = _bank_index(table, (length,), what)
+    B = table.shape[0]
+    qp, dt, qst = _strided(q, (B, None, None, D), what + ": q")
+    T, Hq = q.shape[1], q.shape[2]
+    if Hq < 1 or Hq % H:
+        raise _lib.GpsrError(f"{what}: {Hq} query heads are no multiple of the bank's {H}")
+    if skip is not None and skip.shape != (B, T, 2):
+        raise _lib.GpsrError(f"{what}: skip must be [{B},{T},2], got {tuple(skip.shape)}")
+    return ref, (tp, B, table.shape[1], lp, qp, dt, T, Hq, qst), _p(skip, torch.int32), (B, T, H, Hq, D)
+
+
+def _bank_out(q, want_lse, B, T, Hq):
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device) if want_lse else None
+    return out, lse
+
+
+def bank_attend(bank, table, length, q, scale, skip=None, want_lse=False):
+    """q [B,T,Hq,D] -> out [B,T,Hq,D]: the mean of the values of entry b's first length[b] rows, weighted by
+    exp(-scale |q - k|^2 / 2) (RBF) or exp(scale q.k) (LINEAR); with want_lse also the log of the sum of the weights
+    [B,Hq,T] (RBF: without its factor exp(-scale |q|^2 / 2)).  skip [B,T,2] int32: positions lo <= r < hi that a query does
+    not see; one that sees none gets zeros and -inf (gpsr_bank_attend)."""
+    lib = _lib.load()
+    ref, args, sk, (B, T, H, Hq, D) = _bank_query(bank, table, length, q, skip, "bank_attend")
+    out, lse = _bank_out(q, want_lse, B, T, Hq)
+    nbytes = lib.gpsr_bank_attend_workspace_bytes(ref, B, table.shape[1], T, Hq, args[5])
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _lib.check(lib.gpsr_bank_attend(ref, *args, float(scale), sk, out.data_ptr(), _p(lse), _p(ws), nbytes, _stream()), "gpsr_bank_attend")
+    return (out, lse) if want_lse else out
+
+
+def bank_select(bank, table, length, q, n_sel, skip=None):
+    """-> int32 [B,T,H,n_sel]: the n_sel (1..64) pages of entry b (columns of its table row) whose centroids suit the query
+    best, ascending, -1 behind the last; the heads that share a bank head choose together (gpsr_bank_select)."""
+    lib = _lib.load()
+    ref, args, sk, (B, T, H, Hq, D) = _bank_query(bank, table, length, q, skip, "bank_select")
+    n_sel = int(n_sel)
+    if not 1 <= n_sel <= 64:
+        raise _lib.GpsrError(f"bank_select: n_sel must be in 1..64, got {n_sel}")
+    sel = torch.empty((B, T, H, n_sel), dtype=torch.int32, device=q.device)
+    nbytes = lib.gpsr_bank_select_workspace_bytes(ref, B, table.shape[1], T, Hq, n_sel, args[5])
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _lib.check(lib.gpsr_bank_select(ref, *args, n_sel, sk, sel.data_ptr(), _p(ws), nbytes, _stream()), "gpsr_bank_select")
+    return sel
+
+
+def bank_attend_pages(bank, table, length, q, pages, scale, skip=None, want_lse=False):
+    """bank_attend over the rows of each query's own pages [B,T,H,S] (S in 1..64; bank_select gives them) only.  Numbers outside the
+    table and repeats are passed over (gpsr_bank_attend_pages)."""
+    lib = _lib.load()
+    ref, args, sk, (B, T, H, Hq, D) = _bank_query(bank, table, length, q, skip, "bank_attend_pages")
+    if pages.dim() != 4 or pages.shape[:3] != (B, T, H) or not 1 <= pages.shape[3] <= 64:
+        raise _lib.GpsrError(f"bank_attend_pages: pages must be [{B},{T},{H},1..64], got {tuple(pages.shape)}")
+    out, lse = _bank_out(q, want_lse, B, T, Hq)
+    n_sel = pages.shape[3]
+    nbytes = lib.gpsr_bank_attend_pages_workspace_bytes(ref, B, table.shape[1], T, Hq, n_sel, args[5])
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _lib.check(lib.gpsr_bank_attend_pages(ref, *args, _p(pages, torch.int32), n_sel, float(scale), sk, out.data_ptr(), _p(lse),
+                                          _p(ws), nbytes, _stream()), "gpsr_bank_attend_pages")
+    return (out, lse) if want_lse else out
 
 
 # ------------------------------------------------------------ kernel timing
