@@ -1,135 +1,207 @@
-// gpsr_bank_attend.hip -- example bank: attention over all rows, and over chosen pages (include/gpsr.h).
-#include "gpsr_bank.hpp"
+// gpsr_bank_attend.hip -- example bank: attention over all rows (include/gpsr.h).
+#include "gpsr_bank_tile.hpp"
 
-// One workgroup per query and head: 32 rows at a time are decoded to LDS, each row's logit is one thread-octet's dot product,
-// the running maximum and sum rescale the output of the columns' own threads.
-#define AT_ROWS 32
-template <int DT, int BITS>
-__global__ void __launch_bounds__(256)
+// ---------------------------------------------------------------- attention over the whole bank
+// Columns are the (query, head) pairs that share a bank head.  A workgroup of 4 waves walks the rows of its split of the
+// bank, KT at a time: all threads decode the tile to LDS once, then each wave multiplies it with its own columns.
+//   WK = 1: the waves have 32 NQ columns each (many queries; bound by the matrix units and the exponentials)
+//   WK = 4: all have the same 32 columns and a quarter of the tile's rows each (few queries; bound by reading the bank)
+template <int DT, int BITS, int D, int NQ, int WK, int KT>
+__global__ void __launch_bounds__(256, tile_waves(D, Terms<DT>::N, NQ))
 k_bank_attend(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, int pshift, const int32_t* __restrict__ length,
-              const typename Row<DT>::T* __restrict__ q, int T, int G, Strides qs, const int32_t* __restrict__ sel, int n_sel,
-              float scale, const int32_t* __restrict__ skip, typename Row<DT>::T* __restrict__ out, float* __restrict__ lse) {
-  extern __shared__ float sm[];
-  const int D = bk.dim, ld = D + 1, tid = threadIdx.x, P = 1 << pshift;
-  float* tile = sm;                   // [AT_ROWS][D + 1]
-  float* qv = tile + AT_ROWS * ld;    // [D]
-  float* x = qv + D;                  // [AT_ROWS]
-  const int t = blockIdx.x, hq = blockIdx.y, b = blockIdx.z, h = hq / G, H = bk.heads;
-  for (int i = tid; i < D; i += 256) qv[i] = to_f32<DT>(q[b * qs.b + t * qs.t + hq * qs.h + i]);
-  int64_t len = length[b];
-  if (len > (int64_t)table_pages * P) len = (int64_t)table_pages * P;
-  const int lo = skip ? skip[((size_t)b * T + t) * 2] : 0, hi = skip ? skip[((size_t)b * T + t) * 2 + 1] : 0;
-  const int32_t* mine = sel ? sel + (((size_t)b * T + t) * H + h) * n_sel : nullptr;
-  const int pages = sel ? n_sel : (int)((len + P - 1) >> pshift);
-  float m = -__builtin_inff(), l = 0.f, acc = 0.f;
-  const float c2 = scale * 1.4426950408889634f;
-  for (int i = 0; i < pages; ++i) {
-    const int lp = sel ? mine[i] : i;
-    if (lp < 0 || lp >= table_pages) continue;
-    bool again = false;
-    if (sel) for (int j = 0; j < i; ++j) again |= mine[j] == lp;
-    if (again) continue;
-    const int64_t page = table[(size_t)b * table_pages + lp];
-    if (page < 0 || page >= bk.pages) continue;
-    const size_t row0 = ((size_t)page * H + h) << pshift;
-    const int64_t pos0 = (int64_t)lp << pshift;
-    for (int r0 = 0; r0 < P && pos0 + r0 < len; r0 += AT_ROWS) {
-      for (int pass = 0; pass < 2; ++pass) {
-        __syncthreads();
-        for (int e = tid; e < AT_ROWS * (D / 8); e += 256) {
-          const int r = e / (D / 8), c = e % (D / 8);
-          float y[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-          const int64_t pos = pos0 + r0 + r;
-          if (r0 + r < P && pos < len && !(pos >= lo && pos < hi)) {
-            const size_t row = row0 + r0 + r;
-            const unsigned* w = (const unsigned*)((pass ? bk.v_codes : bk.k_codes) + row * (size_t)(D * BITS / 8)) + c * (BITS / 4);
-            decode8<BITS>(w[0], BITS == 8 ? w[1] : 0u, scale_of((pass ? bk.v_scales : bk.k_scales)[row * (size_t)(D / BK_GROUP) + c / 4]), y);
-          }
-          for (int j = 0; j < 8; ++j) tile[r * ld + c * 8 + j] = y[j];
-        }
-        __syncthreads();
-        if (pass == 0) {
-          const int r = tid / 8, o = tid % 8;
-          float s = 0.f;
-          for (int i2 = o; i2 < D; i2 += 8) s = fmaf(qv[i2], tile[r * ld + i2], s);
-          s += __shfl_xor(s, 1); s += __shfl_xor(s, 2); s += __shfl_xor(s, 4);
-          const int64_t pos = pos0 + r0 + r;
-          const bool ok = r0 + r < P && pos < len && !(pos >= lo && pos < hi);
-          if (o == 0) x[r] = ok ? (s + bk.offset[row0 + r0 + r]) * c2 : -__builtin_inff();
-        }
-      }
-      float mn = m;
-      for (int r = 0; r < AT_ROWS; ++r) mn = fmaxf(mn, x[r]);
-      const float safe = mn == -__builtin_inff() ? 0.f : mn;
-      const float a = exp2f(m - safe);
-      l *= a; acc *= a; m = mn;
-      for (int r = 0; r < AT_ROWS; ++r) {
-        const float p = exp2f(x[r] - safe);
-        l += p;
-        if (tid < D) acc = fmaf(p, tile[r * ld + tid], acc);
-      }
+              const typename Row<DT>::T* __restrict__ q, int T, int G, Strides qs, bool qwide, float scale,
+              const int32_t* __restrict__ skip, typename Row<DT>::T* __restrict__ out, float* __restrict__ lse, int splits,
+              float* __restrict__ part) {
+  constexpr int NT = Terms<DT>::N, KW = KT / WK, NB = KW / 32;   // row blocks of 32 of one wave
+  constexpr int CW = (4 / WK) * 32 * NQ;                         // columns of the workgroup
+  __shared__ __attribute__((aligned(16))) char sm[tile_lds(D, KT)];
+  Tile<D, KT> tile(sm);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+  const int h = blockIdx.y, b = blockIdx.z, H = bk.heads;
+  const int split = blockIdx.x % splits;
+  const int64_t C = (int64_t)T * G, c0 = (int64_t)(blockIdx.x / splits) * CW + (WK == 1 ? wave * 32 * NQ : 0);
+  const int wrow = WK == 1 ? 0 : wave * KW;                      // first row of this wave within a tile
+
+  unsigned len = (unsigned)max(length[b], 0);
+  const int64_t most = (int64_t)table_pages << pshift;
+  if ((int64_t)len > most) len = (unsigned)most;
+  const unsigned tiles = (len + KT - 1) / KT;
+  const unsigned per = (tiles + splits - 1) / splits;
+  const unsigned i0 = min(per * split, tiles), i1 = min(i0 + per, tiles);
+
+  // this lane's columns: query rows as operand fragments, and what they skip
+  bf8 qf[NQ][NT][D / 16];
+  unsigned lo[NQ], hi[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int64_t c = c0 + n * 32 + col;
+    const bool there = c < C;
+    const int64_t t = there ? c / G : 0;
+    load_query<DT, D>(q + b * qs.b + t * qs.t + (int64_t)(h * G + (there ? c - t * G : 0)) * qs.h, qwide, there, half, qf[n]);
+    lo[n] = hi[n] = 0;
+    if (skip && there) {
+      const int32_t* s = skip + ((size_t)b * T + t) * 2;
+      lo[n] = (unsigned)max(s[0], 0); hi[n] = (unsigned)max(s[1], 0);
     }
   }
-  const size_t at = (((size_t)b * T + t) * (size_t)(H * G) + hq) * D;
-  if (tid < D) {
-    const float y = l == 0.f ? 0.f : acc / l;
-    if constexpr (DT == GPSR_BF16) out[at + tid] = bf16_rne(y); else out[at + tid] = (typename Row<DT>::T)y;
+  Soft<D, NQ> st;
+  st.clear();
+  const float c2 = scale * 1.4426950408889634f;
+
+  tile.clear_marks(tid);
+  Fetch<BITS, D, KT> f;
+  const int32_t* tab = table + (size_t)b * table_pages;
+  f.pages(bk, tab, table_pages, pshift, i0 * KT, len, tid);
+  f.codes(bk, h, pshift, i0 * KT, tid);
+  f.pages(bk, tab, table_pages, pshift, (i0 + 1) * KT, len, tid);
+  for (unsigned i = i0; i < i1; ++i) {
+    __syncthreads();
+    f.store(tile, tid, i + 1);
+    __syncthreads();
+    f.codes(bk, h, pshift, (i + 1) * KT, tid);
+    f.pages(bk, tab, table_pages, pshift, (i + 2) * KT, len, tid);
+    f16v s[NB][NQ];
+    tile_logits<D, KT, NT, NQ, NB>(tile, wrow, col, half, qf, s);
+    const unsigned p0 = i * KT;
+    bool any = false;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) any |= lo[n] < p0 + KT && hi[n] > p0 && lo[n] < hi[n];
+    if (__ballot(any)) {
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const unsigned pos = p0 + wrow + kb * 32 + 8 * (e >> 2) + 4 * half + (e & 3);
+            if (pos >= lo[n] && pos < hi[n]) s[kb][n][e] = -__builtin_inff();
+          }
+    }
+    tile_marks<D, KT, NQ, NB>(tile, wrow, half, i + 1, s, st);
+    tile_accumulate<D, KT, NT, NQ, NB>(tile, wrow, col, half, c2, s, st);
   }
-  if (lse && tid == 0) lse[((size_t)b * (H * G) + hq) * T + t] = l == 0.f ? -__builtin_inff() : (log2f(l) + m) * 0.6931471805599453f;
+  st.spoil();
+
+  if constexpr (WK > 1) {   // the four waves' results, joined through LDS by wave 0
+    __syncthreads();
+    st.template join<WK>((float*)sm, wave, lane, c2);
+    if (wave) return;
+  }
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int64_t c = c0 + n * 32 + col;
+    if (c >= C) continue;
+    const int64_t t = c / G;
+    const int hq = h * G + (int)(c - t * G);
+    if (splits == 1) {
+      st.finish(n, c2);
+      store_column<DT, D>(out + (((size_t)b * T + t) * (size_t)(H * G) + hq) * D, half, st.o, n);
+      if (lse && half == 0) lse[((size_t)b * (H * G) + hq) * T + t] = st.lse(n, c2);
+    } else {
+      float* p = part + (((size_t)(b * H + h) * splits + split) * C + c) * (D + 2);
+      store_partial<D>(p, half, st, n);
+    }
+  }
 }
 
-static const char* attend_wrong(const gpsr_bank* bank, const int32_t* table, int B, int table_pages, const int32_t* length,
-                                const void* q, int dtype, int q_heads, const int64_t* qst, float scale, const void* out) {
-  if (const char* w = bank_wrong(bank)) return w;
-  if ((!table && table_pages) || !length || !q || !qst || !out) return "bank_attend: null pointer";
-  if (!type_ok(dtype)) return "bank_attend: dtype";
-  if (B > 65535) return "bank_attend: more than 65535 entries";
-  if (table_pages < 0) return "bank_attend: table_pages";
-  if (q_heads < 1 || q_heads > 65535 || q_heads % bank->heads) return "bank_attend: query heads must be a multiple of the bank's heads, up to 65535";
-  if (!(scale > 0.f) || scale > 3.0e38f) return "bank_attend: scale must be positive and finite";
-  if ((uintptr_t)out & 15) return "bank_attend: out must be 16-byte aligned";
-  return nullptr;
+// joins the splits of one column: one wave per column, lanes over the dim
+template <int DT, int D>
+__global__ void __launch_bounds__(256)
+k_bank_join(const float* __restrict__ part, int T, int G, int H, int64_t C, int splits, float c2,
+            typename Row<DT>::T* __restrict__ out, float* __restrict__ lse) {
+  const int lane = threadIdx.x & 63;
+  const int64_t c = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (c >= C) return;
+  const int h = blockIdx.y, b = blockIdx.z;
+  const float* p = part + ((size_t)(b * H + h) * splits * C + c) * (D + 2);
+  const size_t step = (size_t)C * (D + 2);
+  float m = -__builtin_inff();
+  for (int i = lane; i < splits; i += 64) m = fmaxf(m, p[i * step + D]);
+  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  const float safe = m == -__builtin_inff() ? 0.f : m;
+  constexpr int E = (D + 63) / 64;
+  float acc[E] = {}, l = 0.f;
+  for (int i = 0; i < splits; ++i) {
+    const float w = exp2f((p[i * step + D] - safe) * c2);
+    l = fmaf(w, p[i * step + D + 1], l);
+#pragma unroll
+    for (int e = 0; e < E; ++e) if (e * 64 + lane < D) acc[e] = fmaf(w, p[i * step + e * 64 + lane], acc[e]);
+  }
+  const int64_t t = c / G;
+  const int hq = h * G + (int)(c - t * G);
+  typename Row<DT>::T* o = out + (((size_t)b * T + t) * (size_t)(H * G) + hq) * D;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (e * 64 + lane < D) o[e * 64 + lane] = from_f32<DT>(l == 0.f ? 0.f : acc[e] / l);
+  if (lse && lane == 0) lse[((size_t)b * (H * G) + hq) * T + t] = l == 0.f ? -__builtin_inff() : (log2f(l) + m * c2) * 0.6931471805599453f;
 }
 
-static int attend(const gpsr_bank* bank, const int32_t* table, int B, int table_pages, const int32_t* length, const void* q,
-                  int dtype, int T, int q_heads, const int64_t* qst, const int32_t* sel, int n_sel, float scale,
-                  const int32_t* skip, void* out, float* lse, hipStream_t st) {
-  const int pshift = __builtin_ctz((unsigned)bank->page_rows), G = q_heads / bank->heads;
-  const Strides qs = {qst[0], qst[1], qst[2]};
-  const dim3 grid((unsigned)T, (unsigned)q_heads, (unsigned)B);
-  const size_t lds = (AT_ROWS * (bank->dim + 1) + bank->dim + AT_ROWS) * sizeof(float);
-#define ATTEND(DT, BITS) hipLaunchKernelGGL((k_bank_attend<DT, BITS>), grid, dim3(256), lds, st, *bank, table, table_pages, pshift, \
-                                            length, (const Row<DT>::T*)q, T, G, qs, sel, n_sel, scale, skip, (Row<DT>::T*)out, lse)
-  if (bank->bits == 4) {
-    if (dtype == GPSR_BF16) ATTEND(GPSR_BF16, 4); else if (dtype == GPSR_F16) ATTEND(GPSR_F16, 4); else ATTEND(GPSR_F32, 4);
-  } else {
-    if (dtype == GPSR_BF16) ATTEND(GPSR_BF16, 8); else if (dtype == GPSR_F16) ATTEND(GPSR_F16, 8); else ATTEND(GPSR_F32, 8);
+// How one call is cut: a plan of sizes alone, so that the workspace can be asked for beforehand.
+struct Plan { bool few; int cw, kt, splits; int64_t groups; };
+static Plan plan_of(const gpsr_bank* bk, int B, int table_pages, int T, int q_heads, int dtype) {
+  Plan p;
+  const int64_t C = (int64_t)T * (q_heads / bk->heads);
+  const int nt = dtype == GPSR_BF16 ? 1 : dtype == GPSR_F16 ? 2 : 3;
+  p.few = C <= 32;
+  const int nq = p.few ? 1 : tile_nq(bk->dim, nt);
+  p.cw = p.few ? 32 : 128 * nq;
+  p.kt = p.few ? 128 : 64;
+  p.groups = (C + p.cw - 1) / p.cw;
+  const int64_t tiles = (((int64_t)table_pages * bk->page_rows) + p.kt - 1) / p.kt;
+  // the splits that end soonest when `slots` workgroups run at a time, each paying for 2 tiles besides its own
+  const int64_t slots = 512, wgs = p.groups * bk->heads * B;
+  int64_t best = -1;
+  p.splits = 1;
+  for (int s = 1; s <= 64 && s <= (tiles > 1 ? tiles : 1); ++s) {
+    const int64_t cost = ((wgs * s + slots - 1) / slots) * ((tiles + s - 1) / s + 2) + (s > 1 ? 2 + s / 4 : 0);
+    if (best < 0 || cost < best) { best = cost; p.splits = s; }
   }
-#undef ATTEND
-  CHECK_LAUNCH("k_bank_attend");
-  return 0;
+  return p;
 }
 
 extern "C" size_t gpsr_bank_attend_workspace_bytes(const gpsr_bank* bank, int B, int table_pages, int T, int q_heads, int dtype) {
-  return 0;
+  if (bank_wrong(bank) || B <= 0 || T <= 0 || table_pages < 0 || q_heads < 1 || q_heads % bank->heads || !type_ok(dtype)) return 0;
+  const Plan p = plan_of(bank, B, table_pages, T, q_heads, dtype);
+  return p.splits == 1 ? 0 : (size_t)p.splits * B * T * q_heads * (bank->dim + 2) * sizeof(float);
 }
+
+template <int DT, int BITS, int D>
+static void launch_attend(const Plan& p, const gpsr_bank& bk, const int32_t* table, int B, int table_pages, const int32_t* length,
+                          const void* q, int T, int G, Strides qs, bool qwide, float scale, const int32_t* skip, void* out,
+                          float* lse, float* part, hipStream_t st) {
+  typedef typename Row<DT>::T E;
+  constexpr int NQ = tile_nq(D, Terms<DT>::N);
+  const int pshift = __builtin_ctz((unsigned)bk.page_rows);
+  const dim3 grid((unsigned)(p.groups * p.splits), (unsigned)bk.heads, (unsigned)B);
+#define ATTEND(NQ_, WK, KT) hipLaunchKernelGGL((k_bank_attend<DT, BITS, D, NQ_, WK, KT>), grid, dim3(256), 0, st, bk, table, \
+    table_pages, pshift, length, (const E*)q, T, G, qs, qwide, scale, skip, (E*)out, lse, p.splits, part)
+  if (p.few) ATTEND(1, 4, 128); else ATTEND(NQ, 1, 64);
+#undef ATTEND
+  if (p.splits > 1) {
+    const int64_t C = (int64_t)T * G;
+    hipLaunchKernelGGL((k_bank_join<DT, D>), dim3((unsigned)((C + 3) / 4), (unsigned)bk.heads, (unsigned)B), dim3(256), 0, st, part,
+                       T, G, bk.heads, C, p.splits, scale * 1.4426950408889634f, (E*)out, lse);
+  }
+}
+
 extern "C" int gpsr_bank_attend(const gpsr_bank* bank, const int32_t* table, int B, int table_pages, const int32_t* length,
                                 const void* q, int dtype, int T, int q_heads, const int64_t* qst, float scale,
                                 const int32_t* skip, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
   if (B <= 0 || T <= 0) return 0;
   if (const char* w = attend_wrong(bank, table, B, table_pages, length, q, dtype, q_heads, qst, scale, out)) return arg_fail(w);
-  return attend(bank, table, B, table_pages, length, q, dtype, T, q_heads, qst, nullptr, 0, scale, skip, out, lse, (hipStream_t)stream);
-}
-extern "C" size_t gpsr_bank_attend_pages_workspace_bytes(const gpsr_bank* bank, int B, int table_pages, int T, int q_heads, int n_sel, int dtype) {
+  const Plan p = plan_of(bank, B, table_pages, T, q_heads, dtype);
+  if (p.groups * p.splits > 0x7fffffff) return arg_fail("bank_attend: too many queries for one call");
+  const size_t need = gpsr_bank_attend_workspace_bytes(bank, B, table_pages, T, q_heads, dtype);
+  if (workspace_bytes < need || (need && !workspace)) return arg_fail("workspace too small");
+  if (need && ((uintptr_t)workspace & 15)) return arg_fail("bank_attend: workspace must be 16-byte aligned");
+  const Strides qs = {qst[0], qst[1], qst[2]};
+  const bool wide = rows_wide(q, qst, dtype);
+  const int G = q_heads / bank->heads;
+  hipStream_t st = (hipStream_t)stream;
+#define ATTEND(DT, BITS, D) launch_attend<DT, BITS, D>(p, *bank, table, B, table_pages, length, q, T, G, qs, wide, scale, skip, \
+                                                       out, lse, (float*)workspace, st)
+  BANK_DISPATCH(ATTEND, dtype, bank->bits, bank->dim);
+#undef ATTEND
+  CHECK_LAUNCH("k_bank_attend");
   return 0;
-}
-extern "C" int gpsr_bank_attend_pages(const gpsr_bank* bank, const int32_t* table, int B, int table_pages, const int32_t* length,
-                                      const void* q, int dtype, int T, int q_heads, const int64_t* qst, const int32_t* sel, int n_sel,
-                                      float scale, const int32_t* skip, void* out, float* lse, void* workspace,
-                                      size_t workspace_bytes, void* stream) {
-  if (B <= 0 || T <= 0) return 0;
-  if (const char* w = attend_wrong(bank, table, B, table_pages, length, q, dtype, q_heads, qst, scale, out)) return arg_fail(w);
-  if (!sel) return arg_fail("bank_attend_pages: null pointer");
-  if (n_sel < 1 || n_sel > 64) return arg_fail("bank_attend_pages: n_sel must be in 1..64");
-  return attend(bank, table, B, table_pages, length, q, dtype, T, q_heads, qst, sel, n_sel, scale, skip, out, lse, (hipStream_t)stream);
 }
