@@ -51,15 +51,16 @@ k_bank_attend(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, 
   tile.clear_marks(tid);
   Fetch<BITS, D, KT> f;
   const int32_t* tab = table + (size_t)b * table_pages;
-  f.pages(bk, tab, table_pages, pshift, i0 * KT, len, tid);
+  const WholeBank rows = {tab, bk.pages, pshift, len};
+  f.pages(rows, i0 * KT, tid);
   f.codes(bk, h, pshift, i0 * KT, tid);
-  f.pages(bk, tab, table_pages, pshift, (i0 + 1) * KT, len, tid);
+  f.pages(rows, (i0 + 1) * KT, tid);
   for (unsigned i = i0; i < i1; ++i) {
     __syncthreads();
     f.store(tile, tid, i + 1);
     __syncthreads();
     f.codes(bk, h, pshift, (i + 1) * KT, tid);
-    f.pages(bk, tab, table_pages, pshift, (i + 2) * KT, len, tid);
+    f.pages(rows, (i + 2) * KT, tid);
     f16v s[NB][NQ];
     tile_logits<D, KT, NT, NQ, NB>(tile, wrow, col, half, qf, s);
     const unsigned p0 = i * KT;
@@ -102,38 +103,6 @@ k_bank_attend(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, 
       store_partial<D>(p, half, st, n);
     }
   }
-}
-
-// joins the splits of one column: one wave per column, lanes over the dim
-template <int DT, int D>
-__global__ void __launch_bounds__(256)
-k_bank_join(const float* __restrict__ part, int T, int G, int H, int64_t C, int splits, float c2,
-            typename Row<DT>::T* __restrict__ out, float* __restrict__ lse) {
-  const int lane = threadIdx.x & 63;
-  const int64_t c = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (c >= C) return;
-  const int h = blockIdx.y, b = blockIdx.z;
-  const float* p = part + ((size_t)(b * H + h) * splits * C + c) * (D + 2);
-  const size_t step = (size_t)C * (D + 2);
-  float m = -__builtin_inff();
-  for (int i = lane; i < splits; i += 64) m = fmaxf(m, p[i * step + D]);
-  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-  const float safe = m == -__builtin_inff() ? 0.f : m;
-  constexpr int E = (D + 63) / 64;
-  float acc[E] = {}, l = 0.f;
-  for (int i = 0; i < splits; ++i) {
-    const float w = exp2f((p[i * step + D] - safe) * c2);
-    l = fmaf(w, p[i * step + D + 1], l);
-#pragma unroll
-    for (int e = 0; e < E; ++e) if (e * 64 + lane < D) acc[e] = fmaf(w, p[i * step + e * 64 + lane], acc[e]);
-  }
-  const int64_t t = c / G;
-  const int hq = h * G + (int)(c - t * G);
-  typename Row<DT>::T* o = out + (((size_t)b * T + t) * (size_t)(H * G) + hq) * D;
-#pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (e * 64 + lane < D) o[e * 64 + lane] = from_f32<DT>(l == 0.f ? 0.f : acc[e] / l);
-  if (lse && lane == 0) lse[((size_t)b * (H * G) + hq) * T + t] = l == 0.f ? -__builtin_inff() : (log2f(l) + m * c2) * 0.6931471805599453f;
 }
 
 // How one call is cut: a plan of sizes alone, so that the workspace can be asked for beforehand.
@@ -180,7 +149,8 @@ static void launch_attend(const Plan& p, const gpsr_bank& bk, const int32_t* tab
   if (p.splits > 1) {
     const int64_t C = (int64_t)T * G;
     hipLaunchKernelGGL((k_bank_join<DT, D>), dim3((unsigned)((C + 3) / 4), (unsigned)bk.heads, (unsigned)B), dim3(256), 0, st, part,
-                       T, G, bk.heads, C, p.splits, scale * 1.4426950408889634f, (E*)out, lse);
+                       T, G, bk.heads, C, p.splits, (size_t)p.splits * C, (size_t)1, (size_t)G, (size_t)C,
+                       scale * 1.4426950408889634f, (E*)out, lse);
   }
 }
 

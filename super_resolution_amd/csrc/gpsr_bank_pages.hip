@@ -1,105 +1,294 @@
 // gpsr_bank_pages.hip -- example bank: attention over chosen pages (include/gpsr.h).
+//
+// Two ways through the same mathematics:
+//   by query: a workgroup per query walks that query's pages, its four waves 32 rows each against the query's heads.  Nothing
+//     is shared, 31 of 32 columns of the matrix instructions idle (one head), but it takes one or two launches.
+//   by page: the choices are turned over (for each page the list of queries that chose it), a workgroup takes one page and
+//     128 of its queries, writes each query's partial result for that page, and a last kernel joins each query's partials.
+//     Pages are decoded once per 128 queries and all columns work, at the price of writing and reading the partials.
+// The lists come from atomic counters, so their order may differ from run to run; a partial does not depend on its place in a
+// list, and the join runs in the order of the caller's numbers: results do not change.
 #include "gpsr_bank_tile.hpp"
 
-// One workgroup per query and head: 32 rows at a time are decoded to LDS, each row's logit is one thread-octet's dot product,
-// the running maximum and sum rescale the output of the columns' own threads.
-#define AT_ROWS 32
-template <int DT, int BITS>
-__global__ void __launch_bounds__(256)
-k_bank_attend_pages(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, int pshift, const int32_t* __restrict__ length,
-              const typename Row<DT>::T* __restrict__ q, int T, int G, Strides qs, const int32_t* __restrict__ sel, int n_sel,
-              float scale, const int32_t* __restrict__ skip, typename Row<DT>::T* __restrict__ out, float* __restrict__ lse) {
-  extern __shared__ float sm[];
-  const int D = bk.dim, ld = D + 1, tid = threadIdx.x, P = 1 << pshift;
-  float* tile = sm;                   // [AT_ROWS][D + 1]
-  float* qv = tile + AT_ROWS * ld;    // [D]
-  float* x = qv + D;                  // [AT_ROWS]
-  const int t = blockIdx.x, hq = blockIdx.y, b = blockIdx.z, h = hq / G, H = bk.heads;
-  for (int i = tid; i < D; i += 256) qv[i] = to_f32<DT>(q[b * qs.b + t * qs.t + hq * qs.h + i]);
-  int64_t len = length[b];
-  if (len > (int64_t)table_pages * P) len = (int64_t)table_pages * P;
-  const int lo = skip ? skip[((size_t)b * T + t) * 2] : 0, hi = skip ? skip[((size_t)b * T + t) * 2 + 1] : 0;
-  const int32_t* mine = sel ? sel + (((size_t)b * T + t) * H + h) * n_sel : nullptr;
-  const int pages = sel ? n_sel : (int)((len + P - 1) >> pshift);
-  float m = -__builtin_inff(), l = 0.f, acc = 0.f;
+// ---------------------------------------------------------------- by query
+template <int DT, int BITS, int D>
+__global__ void __launch_bounds__(256, tile_waves(D, Terms<DT>::N, 1))
+k_bank_pages_query(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, int pshift, const int32_t* __restrict__ length,
+                   const typename Row<DT>::T* __restrict__ q, int T, int G, Strides qs, bool qwide, const int32_t* __restrict__ sel,
+                   int n_sel, float scale, const int32_t* __restrict__ skip, typename Row<DT>::T* __restrict__ out,
+                   float* __restrict__ lse, int groups, int splits, float* __restrict__ part) {
+  constexpr int NT = Terms<DT>::N, KT = 128;
+  __shared__ __attribute__((aligned(16))) char sm[tile_lds(D, KT)];
+  __shared__ int phys[64], rown[64], first[64], total;
+  Tile<D, KT> tile(sm);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+  const int h = blockIdx.y, b = blockIdx.z, H = bk.heads, P = 1 << pshift;
+  const int split = blockIdx.x % splits, group = blockIdx.x / splits % groups;
+  const int64_t t = blockIdx.x / splits / groups;
+  const int wrow = wave * 32;
+
+  // the pages that exist, have rows, and were not named before, in the caller's order
+  if (tid < 64) {
+    const int64_t len = length[b];
+    const int32_t* mine = sel + (((size_t)b * T + t) * H + h) * n_sel;
+    const int lp = tid < n_sel ? mine[tid] : -1;
+    bool ok = (unsigned)lp < (unsigned)table_pages && (int64_t)lp * P < len;
+    int p = -1;
+    if (ok) { p = table[(size_t)b * table_pages + lp]; ok = (unsigned)p < (unsigned)bk.pages; }
+    for (int i = 0; i + 1 < n_sel; ++i) { const int o = __shfl(lp, i); ok = ok && !(i < tid && o == lp); }
+    const unsigned long long all = __ballot(ok);
+    if (ok) {
+      const int at = __popcll(all & ((1ull << tid) - 1));
+      phys[at] = p; first[at] = lp; rown[at] = (int)min((int64_t)P, len - (int64_t)lp * P);
+    }
+    if (tid == 0) total = __popcll(all);
+  }
+  tile.clear_marks(tid);
+  const int g = group * 32 + col;
+  const bool there = g < G;
+  bf8 qf[1][NT][D / 16];
+  load_query<DT, D>(q + b * qs.b + t * qs.t + (int64_t)(h * G + (there ? g : 0)) * qs.h, qwide, there, half, qf[0]);
+  const int64_t lo = skip ? skip[((size_t)b * T + t) * 2] : 0, hi = skip ? skip[((size_t)b * T + t) * 2 + 1] : 0;
+  Soft<D, 1> st;
+  st.clear();
   const float c2 = scale * 1.4426950408889634f;
-  for (int i = 0; i < pages; ++i) {
-    const int lp = sel ? mine[i] : i;
-    if (lp < 0 || lp >= table_pages) continue;
-    bool again = false;
-    if (sel) for (int j = 0; j < i; ++j) again |= mine[j] == lp;
-    if (again) continue;
-    const int64_t page = table[(size_t)b * table_pages + lp];
-    if (page < 0 || page >= bk.pages) continue;
-    const size_t row0 = ((size_t)page * H + h) << pshift;
-    const int64_t pos0 = (int64_t)lp << pshift;
-    for (int r0 = 0; r0 < P && pos0 + r0 < len; r0 += AT_ROWS) {
-      for (int pass = 0; pass < 2; ++pass) {
-        __syncthreads();
-        for (int e = tid; e < AT_ROWS * (D / 8); e += 256) {
-          const int r = e / (D / 8), c = e % (D / 8);
-          float y[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-          const int64_t pos = pos0 + r0 + r;
-          if (r0 + r < P && pos < len && !(pos >= lo && pos < hi)) {
-            const size_t row = row0 + r0 + r;
-            const unsigned* w = (const unsigned*)((pass ? bk.v_codes : bk.k_codes) + row * (size_t)(D * BITS / 8)) + c * (BITS / 4);
-            decode8<BITS>(w[0], BITS == 8 ? w[1] : 0u, scale_of((pass ? bk.v_scales : bk.k_scales)[row * (size_t)(D / BK_GROUP) + c / 4]), y);
-          }
-          for (int j = 0; j < 8; ++j) tile[r * ld + c * 8 + j] = y[j];
-        }
-        __syncthreads();
-        if (pass == 0) {
-          const int r = tid / 8, o = tid % 8;
-          float s = 0.f;
-          for (int i2 = o; i2 < D; i2 += 8) s = fmaf(qv[i2], tile[r * ld + i2], s);
-          s += __shfl_xor(s, 1); s += __shfl_xor(s, 2); s += __shfl_xor(s, 4);
-          const int64_t pos = pos0 + r0 + r;
-          const bool ok = r0 + r < P && pos < len && !(pos >= lo && pos < hi);
-          if (o == 0) x[r] = ok ? (s + bk.offset[row0 + r0 + r]) * c2 : -__builtin_inff();
-        }
-      }
-      float mn = m;
-      for (int r = 0; r < AT_ROWS; ++r) mn = fmaxf(mn, x[r]);
-      const float safe = mn == -__builtin_inff() ? 0.f : mn;
-      const float a = exp2f(m - safe);
-      l *= a; acc *= a; m = mn;
-      for (int r = 0; r < AT_ROWS; ++r) {
-        const float p = exp2f(x[r] - safe);
-        l += p;
-        if (tid < D) acc = fmaf(p, tile[r * ld + tid], acc);
+  __syncthreads();
+  const PageList rows = {phys, rown, pshift, (unsigned)total};
+  const unsigned tiles = (((unsigned)total << pshift) + KT - 1) / KT, per = (tiles + splits - 1) / splits;
+  const unsigned i0 = min(per * split, tiles), i1 = min(i0 + per, tiles);
+  Fetch<BITS, D, KT> f;
+  f.pages(rows, i0 * KT, tid);
+  f.codes(bk, h, pshift, i0 * KT, tid);
+  f.pages(rows, (i0 + 1) * KT, tid);
+  for (unsigned i = i0; i < i1; ++i) {
+    __syncthreads();
+    f.store(tile, tid, i + 1);
+    __syncthreads();
+    f.codes(bk, h, pshift, (i + 1) * KT, tid);
+    f.pages(rows, (i + 2) * KT, tid);
+    f16v s[1][1];
+    tile_logits<D, KT, NT, 1, 1>(tile, wrow, col, half, qf, s);
+    if (lo < hi) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const unsigned v = i * KT + wrow + 8 * (e >> 2) + 4 * half + (e & 3), slot = v >> pshift;
+        const int64_t pos = slot < (unsigned)total ? (int64_t)first[slot] * P + (v & (P - 1)) : -1;
+        if (pos >= lo && pos < hi) s[0][0][e] = -__builtin_inff();
       }
     }
+    tile_marks<D, KT, 1, 1>(tile, wrow, half, i + 1, s, st);
+    tile_accumulate<D, KT, NT, 1, 1>(tile, wrow, col, half, c2, s, st);
   }
-  const size_t at = (((size_t)b * T + t) * (size_t)(H * G) + hq) * D;
-  if (tid < D) {
-    const float y = l == 0.f ? 0.f : acc / l;
-    if constexpr (DT == GPSR_BF16) out[at + tid] = bf16_rne(y); else out[at + tid] = (typename Row<DT>::T)y;
+  st.spoil();
+  __syncthreads();
+  st.template join<4>((float*)sm, wave, lane, c2);
+  if (wave || !there) return;
+  const int hq = h * G + g;
+  if (splits == 1) {
+    st.finish(0, c2);
+    store_column<DT, D>(out + (((size_t)b * T + t) * (size_t)(H * G) + hq) * D, half, st.o, 0);
+    if (lse && half == 0) lse[((size_t)b * (H * G) + hq) * T + t] = st.lse(0, c2);
+  } else {
+    store_partial<D>(part + ((((size_t)(b * H + h) * T + t) * splits + split) * G + g) * (D + 2), half, st, 0);
   }
-  if (lse && tid == 0) lse[((size_t)b * (H * G) + hq) * T + t] = l == 0.f ? -__builtin_inff() : (log2f(l) + m) * 0.6931471805599453f;
 }
 
-static int attend(const gpsr_bank* bank, const int32_t* table, int B, int table_pages, const int32_t* length, const void* q,
-                  int dtype, int T, int q_heads, const int64_t* qst, const int32_t* sel, int n_sel, float scale,
-                  const int32_t* skip, void* out, float* lse, hipStream_t st) {
-  const int pshift = __builtin_ctz((unsigned)bank->page_rows), G = q_heads / bank->heads;
-  const Strides qs = {qst[0], qst[1], qst[2]};
-  const dim3 grid((unsigned)T, (unsigned)q_heads, (unsigned)B);
-  const size_t lds = (AT_ROWS * (bank->dim + 1) + bank->dim + AT_ROWS) * sizeof(float);
-#define ATTEND(DT, BITS) hipLaunchKernelGGL((k_bank_attend_pages<DT, BITS>), grid, dim3(256), lds, st, *bank, table, table_pages, pshift, \
-                                            length, (const Row<DT>::T*)q, T, G, qs, sel, n_sel, scale, skip, (Row<DT>::T*)out, lse)
-  if (bank->bits == 4) {
-    if (dtype == GPSR_BF16) ATTEND(GPSR_BF16, 4); else if (dtype == GPSR_F16) ATTEND(GPSR_F16, 4); else ATTEND(GPSR_F32, 4);
-  } else {
-    if (dtype == GPSR_BF16) ATTEND(GPSR_BF16, 8); else if (dtype == GPSR_F16) ATTEND(GPSR_F16, 8); else ATTEND(GPSR_F32, 8);
+// ---------------------------------------------------------------- by page
+// bucket (b, h, logical page) -> how many queries chose it; each choice's place in that list, -1 if it is passed over
+__global__ void __launch_bounds__(256)
+k_bank_pages_clear(int* __restrict__ count, int buckets) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < buckets) count[i] = 0;
+}
+
+__global__ void __launch_bounds__(256)
+k_bank_pages_count(const int32_t* __restrict__ sel, int n_sel, const int32_t* __restrict__ table, int table_pages, int64_t pages,
+                   int pshift, const int32_t* __restrict__ length, int B, int T, int H, int G, int D2, int* __restrict__ count,
+                   int* __restrict__ rank, float* __restrict__ part) {
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x, entries = (int64_t)B * T * H * n_sel;
+  if (e >= entries) return;
+  const int s = (int)(e % n_sel);
+  const int64_t bth = e / n_sel;
+  const int h = (int)(bth % H);
+  const int64_t bt = bth / H;
+  const int b = (int)(bt / T);
+  const int lp = sel[e];
+  bool ok = (unsigned)lp < (unsigned)table_pages && ((int64_t)lp << pshift) < length[b];
+  if (ok) ok = (uint64_t)(int64_t)table[(size_t)b * table_pages + lp] < (uint64_t)pages;
+  for (int i = 0; ok && i < s; ++i) ok = sel[e - s + i] != lp;
+  rank[e] = ok ? atomicAdd(&count[((int64_t)b * H + h) * table_pages + lp], 1) : -1;
+  if (!ok) {
+    const int64_t t = bt % T;
+    for (int g = 0; g < G; ++g) part[(((((size_t)b * H + h) * T + t) * n_sel + s) * G + g) * D2 + D2 - 1] = 0.f;   // saw nothing
   }
-#undef ATTEND
-  CHECK_LAUNCH("k_bank_attend_pages");
-  return 0;
+}
+
+// exclusive sums of the counts and of the workgroups that each bucket needs; one workgroup
+__global__ void __launch_bounds__(1024)
+k_bank_pages_scan(const int* __restrict__ count, int buckets, int G, int cw, int* __restrict__ start, int* __restrict__ wgs) {
+  __shared__ int sc[16], sw[16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int per = (buckets + 1023) / 1024;
+  const int i0 = min(tid * per, buckets), i1 = min(i0 + per, buckets);
+  int c = 0, w = 0;
+  for (int i = i0; i < i1; ++i) { const int n = count[i]; c += n; w += (int)(((int64_t)n * G + cw - 1) / cw); }
+  int pc = c, pw = w;
+  for (int o = 1; o < 64; o <<= 1) {
+    const int a = __shfl_up(pc, o), d = __shfl_up(pw, o);
+    if (lane >= o) { pc += a; pw += d; }
+  }
+  if (lane == 63) { sc[wave] = pc; sw[wave] = pw; }
+  __syncthreads();
+  for (int i = 0; i < wave; ++i) { pc += sc[i]; pw += sw[i]; }
+  int oc = pc - c, ow = pw - w;
+  for (int i = i0; i < i1; ++i) {
+    start[i] = oc; wgs[i] = ow;
+    const int n = count[i];
+    oc += n; ow += (int)(((int64_t)n * G + cw - 1) / cw);
+  }
+  if (tid == 1023) { start[buckets] = pc; wgs[buckets] = pw; }
+}
+
+__global__ void __launch_bounds__(256)
+k_bank_pages_fill(const int32_t* __restrict__ sel, int n_sel, int table_pages, int T, int H, int64_t entries,
+                  const int* __restrict__ rank, const int* __restrict__ start, int* __restrict__ list) {
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (e >= entries) return;
+  const int r = rank[e];
+  if (r < 0) return;
+  const int64_t bth = e / n_sel, bt = bth / H;
+  const int h = (int)(bth % H);
+  const int64_t b = bt / T, t = bt % T;
+  list[start[(b * H + h) * table_pages + sel[e]] + r] = (int)(t * n_sel + e % n_sel);
+}
+
+template <int DT, int BITS, int D, int KT>
+__global__ void __launch_bounds__(256, tile_waves(D, Terms<DT>::N, 1))
+k_bank_pages_page(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, int pshift, const int32_t* __restrict__ length,
+                  const typename Row<DT>::T* __restrict__ q, int T, int G, Strides qs, bool qwide, int n_sel, float scale,
+                  const int32_t* __restrict__ skip, const int* __restrict__ start, const int* __restrict__ wgs, int buckets,
+                  const int* __restrict__ list, float* __restrict__ part) {
+  constexpr int NT = Terms<DT>::N, NB = KT / 32, CW = 128;
+  __shared__ __attribute__((aligned(16))) char sm[tile_lds(D, KT)];
+  Tile<D, KT> tile(sm);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+  const int w = blockIdx.x;
+  if (w >= wgs[buckets]) return;
+  int a = 0, z = buckets;                 // the last bucket whose first workgroup is not behind this one
+  while (z - a > 1) { const int mid = (a + z) >> 1; if (wgs[mid] <= w) a = mid; else z = mid; }
+  const int lp = a % table_pages, H = bk.heads, P = 1 << pshift;
+  const int bh = a / table_pages, h = bh % H, b = bh / H;
+  const int n = start[a + 1] - start[a];
+  const int64_t c = (int64_t)(w - wgs[a]) * CW + wave * 32 + col;
+  const bool there = c < (int64_t)n * G;
+  const int id = there ? list[start[a] + (int)(c / G)] : 0, g = (int)(c % G);
+  const int t = id / n_sel;
+  bf8 qf[1][NT][D / 16];
+  load_query<DT, D>(q + b * qs.b + t * qs.t + (int64_t)(h * G + (there ? g : 0)) * qs.h, qwide, there, half, qf[0]);
+  int64_t lo = 0, hi = 0;
+  if (skip && there) { lo = skip[((size_t)b * T + t) * 2]; hi = skip[((size_t)b * T + t) * 2 + 1]; }
+  const int64_t pos0 = (int64_t)lp << pshift;
+  const OnePage rows = {table[(size_t)b * table_pages + lp], (int)min((int64_t)P, length[b] - pos0)};
+  Soft<D, 1> st;
+  st.clear();
+  const float c2 = scale * 1.4426950408889634f;
+  tile.clear_marks(tid);
+  Fetch<BITS, D, KT> f;
+  f.pages(rows, 0, tid);
+  f.codes(bk, h, pshift, 0, tid);
+  for (int v = 0; v < rows.rows; v += KT) {
+    __syncthreads();
+    f.store(tile, tid, v / KT + 1);
+    __syncthreads();
+    f.pages(rows, v + KT, tid);
+    f.codes(bk, h, pshift, v + KT, tid);
+    f16v s[NB][1];
+    tile_logits<D, KT, NT, 1, NB>(tile, 0, col, half, qf, s);
+    if (__ballot(lo < pos0 + v + KT && hi > pos0 + v && lo < hi)) {
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int64_t pos = pos0 + v + kb * 32 + 8 * (e >> 2) + 4 * half + (e & 3);
+          if (pos >= lo && pos < hi) s[kb][0][e] = -__builtin_inff();
+        }
+    }
+    tile_marks<D, KT, 1, NB>(tile, 0, half, v / KT + 1, s, st);
+    tile_accumulate<D, KT, NT, 1, NB>(tile, 0, col, half, c2, s, st);
+  }
+  st.spoil();
+  if (there) store_partial<D>(part + (((size_t)bh * T * n_sel + id) * G + g) * (D + 2), half, st, 0);
+}
+
+// ---------------------------------------------------------------- host
+struct PagesPlan { bool by_page; int groups, splits; int64_t entries, buckets, most_wgs; size_t rank, start, wgs, list, part, bytes; };
+static PagesPlan plan_of(const gpsr_bank* bk, int B, int table_pages, int T, int q_heads, int n_sel) {
+  PagesPlan p = {};
+  const int H = bk->heads, G = q_heads / H;
+  p.entries = (int64_t)B * T * H * n_sel;
+  p.buckets = (int64_t)B * H * table_pages;
+  // by page where a page serves 8 choices or more on average
+  p.by_page = p.buckets > 0 && p.entries * G >= 8 * p.buckets && p.entries * G >= 4096 && p.entries <= 0x7fffffff && p.buckets <= (1 << 24);
+  if (p.by_page) {
+    p.most_wgs = p.entries * G / 128 + (p.buckets < p.entries ? p.buckets : p.entries);
+    size_t at = align256((size_t)p.buckets * 4);
+    p.rank = at; at += align256((size_t)p.entries * 4);
+    p.start = at; at += align256((size_t)(p.buckets + 1) * 4);
+    p.wgs = at; at += align256((size_t)(p.buckets + 1) * 4);
+    p.list = at; at += align256((size_t)p.entries * 4);
+    p.part = at; at += (size_t)p.entries * G * (bk->dim + 2) * sizeof(float);
+    p.bytes = at;
+  } else {
+    p.groups = (G + 31) / 32;
+    const int64_t wgs = (int64_t)B * T * H * p.groups, tiles = ((int64_t)n_sel * bk->page_rows + 127) / 128;
+    int64_t s = 512 / wgs;
+    if (s < 1) s = 1;
+    p.splits = (int)(s > tiles ? tiles : s);
+    if (p.splits > 1) p.bytes = (size_t)p.splits * B * T * q_heads * (bk->dim + 2) * sizeof(float);
+  }
+  return p;
 }
 
 extern "C" size_t gpsr_bank_attend_pages_workspace_bytes(const gpsr_bank* bank, int B, int table_pages, int T, int q_heads, int n_sel, int dtype) {
-  return 0;
+  if (bank_wrong(bank) || B <= 0 || T <= 0 || table_pages < 0 || q_heads < 1 || q_heads % bank->heads || n_sel < 1 || n_sel > 64 || !type_ok(dtype)) return 0;
+  return plan_of(bank, B, table_pages, T, q_heads, n_sel).bytes;
 }
+
+template <int DT, int BITS, int D>
+static void launch_pages(const PagesPlan& p, const gpsr_bank& bk, const int32_t* table, int B, int table_pages, const int32_t* length,
+                         const void* q, int T, int q_heads, Strides qs, bool qwide, const int32_t* sel, int n_sel, float scale,
+                         const int32_t* skip, void* out, float* lse, char* ws, hipStream_t st) {
+  typedef typename Row<DT>::T E;
+  const int pshift = __builtin_ctz((unsigned)bk.page_rows), H = bk.heads, G = q_heads / H;
+  const int64_t C = (int64_t)T * G;
+  const dim3 join((unsigned)((C + 3) / 4), (unsigned)H, (unsigned)B);
+  const float c2 = scale * 1.4426950408889634f;
+  if (!p.by_page) {
+    float* part = (float*)ws;
+    hipLaunchKernelGGL((k_bank_pages_query<DT, BITS, D>), dim3((unsigned)((int64_t)T * p.groups * p.splits), (unsigned)H, (unsigned)B),
+                       dim3(256), 0, st, bk, table, table_pages, pshift, length, (const E*)q, T, G, qs, qwide, sel, n_sel, scale, skip,
+                       (E*)out, lse, p.groups, p.splits, part);
+    if (p.splits > 1)
+      hipLaunchKernelGGL((k_bank_join<DT, D>), join, dim3(256), 0, st, part, T, G, H, C, p.splits, (size_t)p.splits * C, (size_t)1,
+                         (size_t)p.splits * G, (size_t)G, c2, (E*)out, lse);
+    return;
+  }
+  int *count = (int*)ws, *rank = (int*)(ws + p.rank), *start = (int*)(ws + p.start), *wgs = (int*)(ws + p.wgs), *list = (int*)(ws + p.list);
+  float* part = (float*)(ws + p.part);
+  const unsigned per_entry = (unsigned)((p.entries + 255) / 256);
+  hipLaunchKernelGGL(k_bank_pages_clear, dim3((unsigned)((p.buckets + 255) / 256)), dim3(256), 0, st, count, (int)p.buckets);
+  hipLaunchKernelGGL(k_bank_pages_count, dim3(per_entry), dim3(256), 0, st, sel, n_sel, table, table_pages, bk.pages, pshift, length, B,
+                     T, H, G, D + 2, count, rank, part);
+  hipLaunchKernelGGL(k_bank_pages_scan, dim3(1), dim3(1024), 0, st, count, (int)p.buckets, G, 128, start, wgs);
+  hipLaunchKernelGGL(k_bank_pages_fill, dim3(per_entry), dim3(256), 0, st, sel, n_sel, table_pages, T, H, p.entries, rank, start, list);
+#define PAGE(KT) hipLaunchKernelGGL((k_bank_pages_page<DT, BITS, D, KT>), dim3((unsigned)p.most_wgs), dim3(256), 0, st, bk, table, \
+    table_pages, pshift, length, (const E*)q, T, G, qs, qwide, n_sel, scale, skip, start, wgs, (int)p.buckets, list, part)
+  if (bk.page_rows <= 32) PAGE(32); else PAGE(64);
+#undef PAGE
+  hipLaunchKernelGGL((k_bank_join<DT, D>), join, dim3(256), 0, st, part, T, G, H, C, n_sel, (size_t)n_sel * C, (size_t)1,
+                     (size_t)n_sel * G, (size_t)G, c2, (E*)out, lse);
+}
+
 extern "C" int gpsr_bank_attend_pages(const gpsr_bank* bank, const int32_t* table, int B, int table_pages, const int32_t* length,
                                       const void* q, int dtype, int T, int q_heads, const int64_t* qst, const int32_t* sel, int n_sel,
                                       float scale, const int32_t* skip, void* out, float* lse, void* workspace,
@@ -108,5 +297,18 @@ extern "C" int gpsr_bank_attend_pages(const gpsr_bank* bank, const int32_t* tabl
   if (const char* w = attend_wrong(bank, table, B, table_pages, length, q, dtype, q_heads, qst, scale, out)) return arg_fail(w);
   if (!sel) return arg_fail("bank_attend_pages: null pointer");
   if (n_sel < 1 || n_sel > 64) return arg_fail("bank_attend_pages: n_sel must be in 1..64");
-  return attend(bank, table, B, table_pages, length, q, dtype, T, q_heads, qst, sel, n_sel, scale, skip, out, lse, (hipStream_t)stream);
+  const PagesPlan p = plan_of(bank, B, table_pages, T, q_heads, n_sel);
+  if (p.by_page ? p.most_wgs > 0x7fffffff : (int64_t)T * p.groups * p.splits > 0x7fffffff)
+    return arg_fail("bank_attend_pages: too many queries for one call");
+  if (workspace_bytes < p.bytes || (p.bytes && !workspace)) return arg_fail("workspace too small");
+  if (p.bytes && ((uintptr_t)workspace & 15)) return arg_fail("bank_attend_pages: workspace must be 16-byte aligned");
+  const Strides qs = {qst[0], qst[1], qst[2]};
+  const bool wide = rows_wide(q, qst, dtype);
+  hipStream_t st = (hipStream_t)stream;
+#define PAGES(DT, BITS, D) launch_pages<DT, BITS, D>(p, *bank, table, B, table_pages, length, q, T, q_heads, qs, wide, sel, n_sel, \
+                                                     scale, skip, out, lse, (char*)workspace, st)
+  BANK_DISPATCH(PAGES, dtype, bank->bits, bank->dim);
+#undef PAGES
+  CHECK_LAUNCH("k_bank_attend_pages");
+  return 0;
 }

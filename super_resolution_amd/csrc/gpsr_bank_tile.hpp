@@ -87,6 +87,35 @@ __device__ __forceinline__ unsigned pair(unsigned w0, unsigned w1, float s) {
   return __builtin_bit_cast(unsigned, r);
 }
 
+// ---- where the rows of a walk come from: page(v) is the physical page of row v of the walk (-1: no such row), left(v) how many
+// of the rows v .. v + 3 (one page's) exist.  Row v lies at v % page_rows of its page.
+struct WholeBank {
+  const int32_t* tab;
+  int64_t pages;
+  int pshift;
+  unsigned len;
+  __device__ __forceinline__ int page(unsigned v) const {
+    const int p = v < len ? tab[v >> pshift] : -1;
+    return (unsigned)p < (unsigned)pages ? p : -1;
+  }
+  __device__ __forceinline__ int left(unsigned v) const { return v < len ? (int)min(len - v, 4u) : 0; }
+};
+struct PageList {   // in LDS: physical pages and how many rows each has
+  const int *phys, *rows;
+  int pshift;
+  unsigned n;
+  __device__ __forceinline__ int page(unsigned v) const { return left(v) > 0 ? phys[v >> pshift] : -1; }
+  __device__ __forceinline__ int left(unsigned v) const {
+    const unsigned i = v >> pshift;
+    return i < n ? min(rows[i] - (int)(v & ((1u << pshift) - 1)), 4) : 0;
+  }
+};
+struct OnePage {
+  int phys, rows;
+  __device__ __forceinline__ int page(unsigned v) const { return (int)v < rows ? phys : -1; }
+  __device__ __forceinline__ int left(unsigned v) const { return min(rows - (int)v, 4); }
+};
+
 // ---- a tile on its way: codes are loaded a tile ahead of their use, page numbers two
 template <int BITS, int D, int KT>
 struct Fetch {
@@ -98,28 +127,25 @@ struct Fetch {
   unsigned kw[NU][4 * W], vw[NU][4][W];
   unsigned ks[NU];
   unsigned vs[NU][4];
-  float off;
+  int vleft[NU], fleft[NU];
+  float offs[NU];
 
   // page numbers of the rows from p0 on
-  __device__ __forceinline__ void pages(const gpsr_bank& bk, const int32_t* __restrict__ tab, int table_pages, int pshift,
-                                        unsigned p0, unsigned len, int tid) {
+  template <class Rows>
+  __device__ __forceinline__ void pages(const Rows& rows, unsigned p0, int tid) {
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
       const int u = tid + 256 * i, x = 255 - tid + 256 * i;
       const unsigned kr = p0 + u / (D / 32), vr = p0 + x / (D / 8) * 4;
-      kpage[i] = u < U && kr < len ? tab[kr >> pshift] : -1;
-      vpage[i] = x < U && vr < len ? tab[vr >> pshift] : -1;
-      if ((unsigned)kpage[i] >= (unsigned)bk.pages) kpage[i] = -1;
-      if ((unsigned)vpage[i] >= (unsigned)bk.pages) vpage[i] = -1;
+      kpage[i] = u < U ? rows.page(kr) : -1;
+      vpage[i] = x < U ? rows.page(vr) : -1;
+      vleft[i] = rows.left(vr);
     }
-    left = (int)(len > p0 ? min(len - p0, (unsigned)KT) : 0u);
   }
-  int left, fleft;
 
   // codes, scales and offsets of the rows whose pages were fetched last
   __device__ __forceinline__ void codes(const gpsr_bank& bk, int h, int pshift, unsigned p0, int tid) {
     const unsigned mask = (1u << pshift) - 1;
-    fleft = left;
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
       const int u = tid + 256 * i, x = 255 - tid + 256 * i;
@@ -134,9 +160,9 @@ struct Fetch {
           kw[i][4 * j] = a.x; kw[i][4 * j + 1] = a.y; kw[i][4 * j + 2] = a.z; kw[i][4 * j + 3] = a.w;
         }
         ks[i] = bk.k_scales[row * (size_t)(D / 32) + g];
-        if (g == 0) off = bk.offset[row];
-        offs[i] = off;
+        if (g == 0) offs[i] = bk.offset[row];
       }
+      fleft[i] = vpage[i] >= 0 ? vleft[i] : 0;
       if (vpage[i] >= 0) {
         const int r = x / (D / 8) * 4, c = x % (D / 8);
         const size_t row = (((size_t)vpage[i] * bk.heads + h) << pshift) + ((p0 + r) & mask);
@@ -148,13 +174,9 @@ struct Fetch {
           else { const u2v a = *(const u2v*)(src + j * (D * BITS / 8)); vw[i][j][0] = a.x; vw[i][j][1] = a.y; }
           vs[i][j] = sc[j * (D / 32)];
         }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) { vs[i][j] = 127; for (int w = 0; w < W; ++w) vw[i][j][w] = 0; }
       }
     }
   }
-  float offs[NU];
 
   // decodes them to LDS; rows that do not exist become zeros with an offset of -inf
   __device__ __forceinline__ void store(const Tile<D, KT>& tile, int tid, unsigned number) {
@@ -178,7 +200,7 @@ struct Fetch {
         unsigned y[4][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const bool nan = r + j < fleft && vs[i][j] == 255u, there = r + j < fleft && !nan;
+          const bool here = j < fleft[i], nan = here && vs[i][j] == 255u, there = here && !nan;
           if (nan) { tile.mark[(r + j) * (D / 32) + c / 4] = number; tile.mark[KT * (D / 32)] = number; }
           const float s = scale_of(there ? vs[i][j] : 127u);
           const unsigned w0 = there ? vw[i][j][0] : 0u, w1 = there ? vw[i][j][W - 1] : 0u;
@@ -410,6 +432,41 @@ __device__ __forceinline__ void store_partial(float* __restrict__ p, int half, S
 #pragma unroll
       for (int j = 0; j < 4; ++j) p[d * 32 + 8 * i + 4 * half + j] = st.o[d][n][4 * i + j];
   if (half == 0) { p[D] = st.m[n]; p[D + 1] = l; }
+}
+
+// Joins the partial results of one column: one wave per column, lanes over the dim.  Column (t, g) of bank head bh has its n
+// partials [D + 2] at bh * per_bh + t * per_t + g * per_g + i * per_i.
+template <int DT, int D>
+__global__ void __launch_bounds__(256)
+k_bank_join(const float* __restrict__ part, int T, int G, int H, int64_t C, int n, size_t per_bh, size_t per_g, size_t per_t,
+            size_t per_i, float c2, typename Row<DT>::T* __restrict__ out, float* __restrict__ lse) {
+  const int lane = threadIdx.x & 63;
+  const int64_t c = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (c >= C) return;
+  const int h = blockIdx.y, b = blockIdx.z;
+  const int64_t t = c / G;
+  const int g = (int)(c - t * G), hq = h * G + g;
+  const float* p = part + ((size_t)(b * H + h) * per_bh + t * per_t + g * per_g) * (D + 2);
+  const size_t step = per_i * (D + 2);
+  float m = -__builtin_inff();
+  for (int i = lane; i < n; i += 64) if (p[i * step + D + 1] != 0.f) m = fmaxf(m, p[i * step + D]);
+  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  const float safe = m == -__builtin_inff() ? 0.f : m;
+  constexpr int E = (D + 63) / 64;
+  float acc[E] = {}, l = 0.f;
+  for (int i = 0; i < n; ++i) {
+    const float li = p[i * step + D + 1];
+    if (li == 0.f) continue;             // saw nothing: its sums were not written
+    const float w = exp2f((p[i * step + D] - safe) * c2);
+    l = fmaf(w, li, l);
+#pragma unroll
+    for (int e = 0; e < E; ++e) if (e * 64 + lane < D) acc[e] = fmaf(w, p[i * step + e * 64 + lane], acc[e]);
+  }
+  typename Row<DT>::T* o = out + (((size_t)b * T + t) * (size_t)(H * G) + hq) * D;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (e * 64 + lane < D) o[e * 64 + lane] = from_f32<DT>(l == 0.f ? 0.f : acc[e] / l);
+  if (lse && lane == 0) lse[((size_t)b * (H * G) + hq) * T + t] = l == 0.f ? -__builtin_inff() : (log2f(l) + m * c2) * 0.6931471805599453f;
 }
 
 // ---- host side

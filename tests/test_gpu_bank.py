@@ -439,6 +439,30 @@ def test_attend_pages(dtype, bits, D, P, H, G, T, S, lengths):
         c.check(q, out, lse, s, seen)
 
 
+@pytest.mark.parametrize("dtype,bits", [(BF16, 4), (F16, 8), (F32, 4)])
+@pytest.mark.parametrize("D,P,H,G,T,S,lengths", [
+    (64, 64, 1, 1, 600, 8, [900]), (32, 16, 2, 2, 150, 8, [200, 77]), (128, 128, 1, 1, 700, 6, [1500]), (96, 32, 1, 3, 100, 16, [333]),
+    (256, 256, 1, 1, 1100, 4, [700]), (192, 16, 3, 1, 100, 16, [160])])
+def test_attend_pages_of_many_queries(dtype, bits, D, P, H, G, T, S, lengths):
+    """Enough queries for each page to be taken page by page; repeats, numbers outside the table and skipped rows among them."""
+    ops = _ops()
+    c = Case(lengths, H, D, P, bits, "RBF", dtype, seed=D + S)
+    q, qd = c.queries(T, G, dtype)
+    s = float(np.float32(1.0 / math.sqrt(D)))
+    J = c.table.shape[1]
+    sel = c.rng.integers(-2, J + 1, (len(lengths), T, H, S)).astype(np.int32)
+    sd = torch.as_tensor(sel).to(c.dev)
+    skip, kd = _skips(len(lengths), T, lengths, c.rng, c.dev)
+    out, lse = ops.bank_attend_pages(c.bank, c.table, c.length, qd, sd, s, skip=kd, want_lse=True)
+
+    def seen(b, t, h):
+        r = np.arange(lengths[b])
+        return np.isin(r // P, sel[b, t, h]) & ~((r >= skip[b, t, 0]) & (r < skip[b, t, 1]))
+    c.check(q, out, lse, s, seen)
+    again = [ops.bank_attend_pages(c.bank, c.table, c.length, qd, sd, s, skip=kd) for _ in range(3)]
+    assert all(torch.equal(out, a) for a in again)
+
+
 def test_all_pages_chosen_equals_the_whole_bank_and_banks_join_by_lse():
     """The set as a user runs it: append, read back, choose, attend; two halves of a bank joined by their lse."""
     ops = _ops()
