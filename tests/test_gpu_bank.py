@@ -414,6 +414,82 @@ def test_select_near_ties_are_decided_in_64_bits():
     assert np.array_equal(got[0, 3, 0], np.sort(np.argsort(-order)[:9]))
 
 
+def _select_exact_many(c, q, n_sel, skip=None, rbf=True):
+    """The same for many queries: a stable sort by falling score."""
+    B, T, Hq, D = q.shape
+    G = Hq // c.H
+    cent = c.bank.centroid.double().cpu().numpy()
+    qd = q.double().numpy().reshape(B, T, c.H, G, D).sum(3)
+    out = np.full((B, T, c.H, n_sel), -1, np.int32)
+    for b in range(B):
+        n = c.lengths[b]
+        first = np.arange(-(-n // c.P)) * c.P
+        ok = np.ones((T, len(first)), bool)
+        if skip is not None:
+            ok = ~((skip[b, :, :1] <= first) & (skip[b, :, 1:] >= np.minimum(first + c.P, n)))
+        for h in range(c.H):
+            ce = cent[c.table_np[b, :len(first)], h]
+            # one sum for each score, all in the same order: a matrix product gives equal pages scores that differ in the last bit
+            dot = np.stack([(x * ce).sum(-1) for x in qd[b, :, h]])
+            score = np.where(ok, dot - (G * (ce * ce).sum(1) / 2 if rbf else 0.0), -np.inf)
+            at = np.argsort(-score, axis=1, kind="stable")[:, :n_sel]
+            at = np.sort(np.where(np.take_along_axis(score, at, 1) == -np.inf, 2 ** 30, at), 1)
+            out[b, :, h, :at.shape[1]] = np.where(at == 2 ** 30, -1, at)
+    return out
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("D,P,H,G,T,n_sel,lengths", [
+    (64, 16, 1, 1, 700, 16, [16 * 400 - 3]), (32, 16, 2, 1, 301, 4, [1100, 16 * 70]), (128, 32, 1, 3, 513, 64, [32 * 300]),
+    (96, 16, 1, 2, 600, 33, [16 * 3000]), (192, 64, 1, 1, 520, 1, [64 * 80]), (256, 16, 1, 1, 550, 9, [16 * 99 + 1])])
+def test_select_for_many_queries(dtype, D, P, H, G, T, n_sel, lengths):
+    """Enough queries and pages for the screen in fewer bits: the choice has to stay the one in 64."""
+    ops = _ops()
+    for kernel in ("RBF", "LINEAR"):
+        c = Case(lengths, H, D, P, 4, kernel, dtype, seed=D + T + 1)
+        q, qd = c.queries(T, G, dtype)
+        got = ops.bank_select(c.bank, c.table, c.length, qd, n_sel)
+        assert np.array_equal(got.cpu().numpy(), _select_exact_many(c, q, n_sel, rbf=kernel == "RBF"))
+        skip, sd = _skips(len(lengths), T, lengths, c.rng, c.dev)
+        got = ops.bank_select(c.bank, c.table, c.length, qd, n_sel, skip=sd)
+        assert np.array_equal(got.cpu().numpy(), _select_exact_many(c, q, n_sel, skip, kernel == "RBF"))
+
+
+def test_select_for_many_queries_where_few_bits_do_not_tell():
+    """Runs of equal pages (more candidates than the screen holds), scores one 32-bit step apart, pages of huge and of tiny norm,
+    pages that are not numbers (never chosen), queries of zeros and of huge values."""
+    ops = _ops()
+    P, n, T = 16, 700, 600
+    for kernel in ("RBF", "LINEAR"):
+        for dtype in (BF16, F32):
+            c = Case([P * n], 1, 64, P, 4, kernel, dtype, seed=77)
+            q, _ = c.queries(T, 1, dtype)
+            rng = c.rng
+            cent = rng.normal(size=(n, 64)).astype(np.float32) * 0.2
+            cent[100:400] = cent[99]                                            # equal
+            cent[400:500] = cent[99]
+            cent[400:500, 0] += np.arange(100, dtype=np.float32) * 2.0 ** -24   # next to equal
+            cent[500:510] *= np.float32(1e25)
+            cent[510:520] *= np.float32(1e-30)
+            order = torch.as_tensor(c.table_np[0, :n].astype(np.int64)).to(c.dev)
+            q[0, :4] = 0
+            q[0, 4:200] = torch.as_tensor(cent[99]).to(dtype) * 2
+            q[0, 200] *= 1e25
+            q[0, 201] *= 1e-30
+            qd = q.to(c.dev)
+            c.bank.centroid[order, 0] = torch.as_tensor(cent).to(c.dev)
+            for n_sel in (5, 64):
+                got = ops.bank_select(c.bank, c.table, c.length, qd, n_sel).cpu().numpy()
+                assert np.array_equal(got, _select_exact_many(c, q, n_sel, rbf=kernel == "RBF"))
+            bad = rng.choice(n, 60, replace=False)
+            c.bank.centroid[order[torch.as_tensor(bad).to(c.dev)], 0, 7] = math.nan
+            got = ops.bank_select(c.bank, c.table, c.length, qd, 20).cpu().numpy()
+            assert not np.isin(got, bad).any() and (got >= 0).all()
+            c.bank.centroid[order[torch.as_tensor(bad).to(c.dev)], 0] = -1e30 if kernel == "RBF" else 0.0
+            if kernel == "RBF":     # the same choice as with those pages as far away as can be
+                assert np.array_equal(got, _select_exact_many(c, q, 20))
+
+
 # ------------------------------------------------------------ attention over chosen pages
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("bits", [4, 8])
