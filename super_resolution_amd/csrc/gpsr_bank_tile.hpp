@@ -18,7 +18,7 @@ template <> struct Terms<GPSR_F32> { static constexpr int N = 3; };
 // blocks of 32 columns that a wave holds: two halve the LDS reads for a product, where the registers allow it
 static constexpr int tile_nq(int d, int nt) { return nt == 1 && d <= 64 ? 2 : 1; }
 // waves per SIMD that the registers are budgeted for
-static constexpr int tile_waves(int d, int nt, int nq) { return (d * nq * (nt + 2)) / 4 + 64 * nq > 220 ? 1 : 2; }
+static constexpr int tile_waves(int d, int nt, int nq) { return (d * nq * (nt + 1)) / 4 + 32 * nq > 160 ? 1 : 2; }
 
 template <int DT>
 __device__ __forceinline__ typename Row<DT>::T from_f32(float y) {
