@@ -1,25 +1,28 @@
 // gpsr_bank_attend.hip -- example bank: attention over all rows (include/gpsr.h).
 #include "gpsr_bank_tile.hpp"
 
+#include <type_traits>
+
 // ---------------------------------------------------------------- attention over the whole bank
-// Columns are the (query, head) pairs that share a bank head.  A workgroup of 4 waves walks the rows of its split of the
-// bank, KT at a time: all threads decode the tile to LDS once, then each wave multiplies it with its own columns.
-//   WK = 1: the waves have 32 NQ columns each (many queries; bound by the matrix units and the exponentials)
-//   WK = 4: all have the same 32 columns and a quarter of the tile's rows each (few queries; bound by reading the bank)
-template <int DT, int BITS, int D, int NQ, int WK, int KT>
-__global__ void __launch_bounds__(256, tile_waves(D, Terms<DT>::N, NQ))
+// Columns are the (query, head) pairs that share a bank head.  A workgroup of NW waves walks the rows of its split of the
+// bank, KT at a time: all threads decode the tile to LDS once, then each wave multiplies it with its own 32 columns, NB x 32
+// rows at a time.
+//   WK = 1: each wave has columns of its own (many queries; bound by the exponentials and the matrix units)
+//   WK = NW: all have the same columns and a share of the tile's rows each (few queries; bound by reading the bank)
+template <int DT, int BITS, int D, int NW, int WK, int KT, int NB>
+__global__ void __launch_bounds__(64 * NW, tile_waves(D, Terms<DT>::N, 1, NB))
 k_bank_attend(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, int pshift, const int32_t* __restrict__ length,
               const typename Row<DT>::T* __restrict__ q, int T, int G, Strides qs, bool qwide, float scale,
               const int32_t* __restrict__ skip, typename Row<DT>::T* __restrict__ out, float* __restrict__ lse, int splits,
               float* __restrict__ part) {
-  constexpr int NT = Terms<DT>::N, KW = KT / WK, NB = KW / 32;   // row blocks of 32 of one wave
-  constexpr int CW = (4 / WK) * 32 * NQ;                         // columns of the workgroup
+  constexpr int NT = Terms<DT>::N, KW = KT / WK;                 // rows of one wave
+  constexpr int CW = (NW / WK) * 32, NQ = 1;                     // columns of the workgroup
   __shared__ __attribute__((aligned(16))) char sm[tile_lds(D, KT)];
   Tile<D, KT> tile(sm);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
   const int h = blockIdx.y, b = blockIdx.z, H = bk.heads;
   const int split = blockIdx.x % splits;
-  const int64_t C = (int64_t)T * G, c0 = (int64_t)(blockIdx.x / splits) * CW + (WK == 1 ? wave * 32 * NQ : 0);
+  const int64_t C = (int64_t)T * G, c0 = (int64_t)(blockIdx.x / splits) * CW + (WK == 1 ? wave * 32 : 0);
   const int wrow = WK == 1 ? 0 : wave * KW;                      // first row of this wave within a tile
 
   unsigned len = (unsigned)max(length[b], 0);
@@ -45,47 +48,62 @@ k_bank_attend(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, 
     }
   }
   Soft<D, NQ> st;
-  st.clear();
   const float c2 = scale * 1.4426950408889634f;
 
-  tile.clear_marks(tid);
-  Fetch<BITS, D, KT> f;
-  const int32_t* tab = table + (size_t)b * table_pages;
-  const WholeBank rows = {tab, bk.pages, pshift, len};
-  f.pages(rows, i0 * KT, tid);
-  f.codes(bk, h, pshift, i0 * KT, tid);
-  f.pages(rows, (i0 + 1) * KT, tid);
-  for (unsigned i = i0; i < i1; ++i) {
+  tile.clear_marks(tid, 64 * NW);
+  Fetch<BITS, D, KT, 64 * NW> f;
+  const WholeBank rows = {table + (size_t)b * table_pages, bk.pages, pshift, len};
+  const auto step = [&](unsigned i, auto move) {
     __syncthreads();
     f.store(tile, tid, i + 1);
     __syncthreads();
     f.codes(bk, h, pshift, (i + 1) * KT, tid);
     f.pages(rows, (i + 2) * KT, tid);
-    f16v s[NB][NQ];
-    tile_logits<D, KT, NT, NQ, NB>(tile, wrow, col, half, qf, s);
     const unsigned p0 = i * KT;
+    tile_marks<D, KT, NQ, KW>(tile, wrow, i + 1, st, [&](int n, int r) { return !(p0 + wrow + r >= lo[n] && p0 + wrow + r < hi[n]); });
     bool any = false;
 #pragma unroll
     for (int n = 0; n < NQ; ++n) any |= lo[n] < p0 + KT && hi[n] > p0 && lo[n] < hi[n];
-    if (__ballot(any)) {
+    const bool skips = skip && __ballot(any);
+#pragma unroll 1
+    for (int r = 0; r < KW; r += 32 * NB) {
+      f16v s[NB][NQ];
+      tile_logits<D, KT, NT, NQ, NB>(tile, wrow + r, col, half, qf, s);
+      if (skips) {
+        asm volatile("");        // not to be computed for the tiles that nobody skips
 #pragma unroll
-      for (int n = 0; n < NQ; ++n)
+        for (int n = 0; n < NQ; ++n)
 #pragma unroll
-        for (int kb = 0; kb < NB; ++kb)
+          for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const unsigned pos = p0 + wrow + kb * 32 + 8 * (e >> 2) + 4 * half + (e & 3);
-            if (pos >= lo[n] && pos < hi[n]) s[kb][n][e] = -__builtin_inff();
-          }
+            for (int e = 0; e < 16; ++e) {
+              const unsigned pos = p0 + wrow + r + kb * 32 + 8 * (e >> 2) + 4 * half + (e & 3);
+              if (pos >= lo[n] && pos < hi[n]) s[kb][n][e] = -__builtin_inff();
+            }
+      }
+      tile_accumulate<D, KT, NT, NQ, NB, decltype(move)::value>(tile, wrow + r, col, half, c2, s, st);
     }
-    tile_marks<D, KT, NQ, NB>(tile, wrow, half, i + 1, s, st);
-    tile_accumulate<D, KT, NT, NQ, NB>(tile, wrow, col, half, c2, s, st);
+  };
+  st.clear();
+  for (bool safe = WK > 1; i0 < i1; safe = true) {
+    f.pages(rows, i0 * KT, tid);
+    f.codes(bk, h, pshift, i0 * KT, tid);
+    f.pages(rows, (i0 + 1) * KT, tid);
+    // The steps without a move are a loop of their own, in which the sums never leave their registers.  The waves of a
+    // workgroup may be in different ones of the two; every step has the same barriers.
+    for (unsigned i = i0; i < i1;) {
+      step(i++, std::true_type());
+      if constexpr (WK == 1)
+        while (i < i1 && !safe && !st.wants_move()) step(i++, std::false_type());
+    }
+    if (WK > 1 || safe || !__syncthreads_or(st.lost())) break;
+    st.clear();
   }
   st.spoil();
 
   if constexpr (WK > 1) {   // the four waves' results, joined through LDS by wave 0
     __syncthreads();
-    st.template join<WK>((float*)sm, wave, lane, c2);
+    st.template join<WK>((float*)sm, wave, lane);
     if (wave) return;
   }
 #pragma unroll
@@ -95,9 +113,9 @@ k_bank_attend(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, 
     const int64_t t = c / G;
     const int hq = h * G + (int)(c - t * G);
     if (splits == 1) {
-      st.finish(n, c2);
+      st.finish(n);
       store_column<DT, D>(out + (((size_t)b * T + t) * (size_t)(H * G) + hq) * D, half, st.o, n);
-      if (lse && half == 0) lse[((size_t)b * (H * G) + hq) * T + t] = st.lse(n, c2);
+      if (lse && half == 0) lse[((size_t)b * (H * G) + hq) * T + t] = st.lse(n);
     } else {
       float* p = part + (((size_t)(b * H + h) * splits + split) * C + c) * (D + 2);
       store_partial<D>(p, half, st, n);
@@ -107,18 +125,20 @@ k_bank_attend(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, 
 
 // How one call is cut: a plan of sizes alone, so that the workspace can be asked for beforehand.
 struct Plan { bool few; int cw, kt, splits; int64_t groups; };
+static constexpr int many_nb(int d, int nt) { return tile_waves(d, nt, 1, 2) == tile_waves(d, nt, 1, 1) ? 2 : 1; }
+static constexpr int many_nw(int d, int nt) { return tile_waves(d, nt, 1, many_nb(d, nt)) >= 2 ? 8 : 4; }
+static constexpr int many_kt(int d, int nt) { return many_nw(d, nt) == 8 && tile_lds(d, 128) <= 80 * 1024 ? 128 : 64; }
 static Plan plan_of(const gpsr_bank* bk, int B, int table_pages, int T, int q_heads, int dtype) {
   Plan p;
   const int64_t C = (int64_t)T * (q_heads / bk->heads);
-  const int nt = dtype == GPSR_BF16 ? 1 : dtype == GPSR_F16 ? 2 : 3;
+  const int nt = dtype == GPSR_BF16 ? 1 : dtype == GPSR_F16 ? 2 : 3, nw = many_nw(bk->dim, nt);
   p.few = C <= 32;
-  const int nq = p.few ? 1 : tile_nq(bk->dim, nt);
-  p.cw = p.few ? 32 : 128 * nq;
-  p.kt = p.few ? 128 : 64;
+  p.cw = p.few ? 32 : 32 * nw;
+  p.kt = p.few ? 128 : many_kt(bk->dim, nt);
   p.groups = (C + p.cw - 1) / p.cw;
   const int64_t tiles = (((int64_t)table_pages * bk->page_rows) + p.kt - 1) / p.kt;
   // the splits that end soonest when `slots` workgroups run at a time, each paying for 2 tiles besides its own
-  const int64_t slots = 512, wgs = p.groups * bk->heads * B;
+  const int64_t slots = p.few ? 512 : 256 * 4 * tile_waves(bk->dim, nt, 1, many_nb(bk->dim, nt)) / nw, wgs = p.groups * bk->heads * B;
   int64_t best = -1;
   p.splits = 1;
   for (int s = 1; s <= 64 && s <= (tiles > 1 ? tiles : 1); ++s) {
@@ -139,18 +159,18 @@ static void launch_attend(const Plan& p, const gpsr_bank& bk, const int32_t* tab
                           const void* q, int T, int G, Strides qs, bool qwide, float scale, const int32_t* skip, void* out,
                           float* lse, float* part, hipStream_t st) {
   typedef typename Row<DT>::T E;
-  constexpr int NQ = tile_nq(D, Terms<DT>::N);
+  constexpr int NT = Terms<DT>::N, NW = many_nw(D, NT);
   const int pshift = __builtin_ctz((unsigned)bk.page_rows);
   const dim3 grid((unsigned)(p.groups * p.splits), (unsigned)bk.heads, (unsigned)B);
-#define ATTEND(NQ_, WK, KT) hipLaunchKernelGGL((k_bank_attend<DT, BITS, D, NQ_, WK, KT>), grid, dim3(256), 0, st, bk, table, \
+#define ATTEND(NW_, WK, KT, NB) hipLaunchKernelGGL((k_bank_attend<DT, BITS, D, NW_, WK, KT, NB>), grid, dim3(64 * NW_), 0, st, bk, table, \
     table_pages, pshift, length, (const E*)q, T, G, qs, qwide, scale, skip, (E*)out, lse, p.splits, part)
-  if (p.few) ATTEND(1, 4, 128); else ATTEND(NQ, 1, 64);
+  if (p.few) ATTEND(4, 4, 128, 1); else ATTEND(NW, 1, many_kt(D, NT), many_nb(D, NT));
 #undef ATTEND
   if (p.splits > 1) {
     const int64_t C = (int64_t)T * G;
     hipLaunchKernelGGL((k_bank_join<DT, D>), dim3((unsigned)((C + 3) / 4), (unsigned)bk.heads, (unsigned)B), dim3(256), 0, st, part,
                        T, G, bk.heads, C, p.splits, (size_t)p.splits * C, (size_t)1, (size_t)G, (size_t)C,
-                       scale * 1.4426950408889634f, (E*)out, lse);
+                       (E*)out, lse);
   }
 }
 

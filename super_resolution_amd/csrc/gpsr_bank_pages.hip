@@ -12,7 +12,7 @@
 
 // ---------------------------------------------------------------- by query
 template <int DT, int BITS, int D>
-__global__ void __launch_bounds__(256, tile_waves(D, Terms<DT>::N, 1))
+__global__ void __launch_bounds__(256, tile_waves(D, Terms<DT>::N, 1, 1))
 k_bank_pages_query(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, int pshift, const int32_t* __restrict__ length,
                    const typename Row<DT>::T* __restrict__ q, int T, int G, Strides qs, bool qwide, const int32_t* __restrict__ sel,
                    int n_sel, float scale, const int32_t* __restrict__ skip, typename Row<DT>::T* __restrict__ out,
@@ -43,7 +43,7 @@ k_bank_pages_query(gpsr_bank bk, const int32_t* __restrict__ table, int table_pa
     }
     if (tid == 0) total = __popcll(all);
   }
-  tile.clear_marks(tid);
+  tile.clear_marks(tid, 256);
   const int g = group * 32 + col;
   const bool there = g < G;
   bf8 qf[1][NT][D / 16];
@@ -56,38 +56,44 @@ k_bank_pages_query(gpsr_bank bk, const int32_t* __restrict__ table, int table_pa
   const PageList rows = {phys, rown, pshift, (unsigned)total};
   const unsigned tiles = (((unsigned)total << pshift) + KT - 1) / KT, per = (tiles + splits - 1) / splits;
   const unsigned i0 = min(per * split, tiles), i1 = min(i0 + per, tiles);
-  Fetch<BITS, D, KT> f;
-  f.pages(rows, i0 * KT, tid);
-  f.codes(bk, h, pshift, i0 * KT, tid);
-  f.pages(rows, (i0 + 1) * KT, tid);
+  Fetch<BITS, D, KT, 256> f;
+  if (i0 < i1) {
+    f.pages(rows, i0 * KT, tid);
+    f.codes(bk, h, pshift, i0 * KT, tid);
+    f.pages(rows, (i0 + 1) * KT, tid);
+  }
   for (unsigned i = i0; i < i1; ++i) {
     __syncthreads();
     f.store(tile, tid, i + 1);
     __syncthreads();
     f.codes(bk, h, pshift, (i + 1) * KT, tid);
     f.pages(rows, (i + 2) * KT, tid);
+    const auto skips = [&](unsigned v) {
+      const unsigned slot = v >> pshift;
+      const int64_t pos = slot < (unsigned)total ? (int64_t)first[slot] * P + (v & (P - 1)) : -1;
+      return pos >= lo && pos < hi;
+    };
+    tile_marks<D, KT, 1, 32>(tile, wrow, i + 1, st, [&](int, int r) { return !skips(i * KT + wrow + r); });
     f16v s[1][1];
     tile_logits<D, KT, NT, 1, 1>(tile, wrow, col, half, qf, s);
     if (lo < hi) {
+      asm volatile("");
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const unsigned v = i * KT + wrow + 8 * (e >> 2) + 4 * half + (e & 3), slot = v >> pshift;
-        const int64_t pos = slot < (unsigned)total ? (int64_t)first[slot] * P + (v & (P - 1)) : -1;
-        if (pos >= lo && pos < hi) s[0][0][e] = -__builtin_inff();
+        if (skips(i * KT + wrow + 8 * (e >> 2) + 4 * half + (e & 3))) s[0][0][e] = -__builtin_inff();
       }
     }
-    tile_marks<D, KT, 1, 1>(tile, wrow, half, i + 1, s, st);
-    tile_accumulate<D, KT, NT, 1, 1>(tile, wrow, col, half, c2, s, st);
+    tile_accumulate<D, KT, NT, 1, 1, true>(tile, wrow, col, half, c2, s, st);
   }
   st.spoil();
   __syncthreads();
-  st.template join<4>((float*)sm, wave, lane, c2);
+  st.template join<4>((float*)sm, wave, lane);
   if (wave || !there) return;
   const int hq = h * G + g;
   if (splits == 1) {
-    st.finish(0, c2);
+    st.finish(0);
     store_column<DT, D>(out + (((size_t)b * T + t) * (size_t)(H * G) + hq) * D, half, st.o, 0);
-    if (lse && half == 0) lse[((size_t)b * (H * G) + hq) * T + t] = st.lse(0, c2);
+    if (lse && half == 0) lse[((size_t)b * (H * G) + hq) * T + t] = st.lse(0);
   } else {
     store_partial<D>(part + ((((size_t)(b * H + h) * T + t) * splits + split) * G + g) * (D + 2), half, st, 0);
   }
@@ -163,7 +169,7 @@ k_bank_pages_fill(const int32_t* __restrict__ sel, int n_sel, int table_pages, i
 }
 
 template <int DT, int BITS, int D, int KT>
-__global__ void __launch_bounds__(256, tile_waves(D, Terms<DT>::N, 1))
+__global__ void __launch_bounds__(256, tile_waves(D, Terms<DT>::N, 1, KT / 32))
 k_bank_pages_page(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, int pshift, const int32_t* __restrict__ length,
                   const typename Row<DT>::T* __restrict__ q, int T, int G, Strides qs, bool qwide, int n_sel, float scale,
                   const int32_t* __restrict__ skip, const int* __restrict__ start, const int* __restrict__ wgs, int buckets,
@@ -192,8 +198,8 @@ k_bank_pages_page(gpsr_bank bk, const int32_t* __restrict__ table, int table_pag
   Soft<D, 1> st;
   st.clear();
   const float c2 = scale * 1.4426950408889634f;
-  tile.clear_marks(tid);
-  Fetch<BITS, D, KT> f;
+  tile.clear_marks(tid, 256);
+  Fetch<BITS, D, KT, 256> f;
   f.pages(rows, 0, tid);
   f.codes(bk, h, pshift, 0, tid);
   for (int v = 0; v < rows.rows; v += KT) {
@@ -202,9 +208,11 @@ k_bank_pages_page(gpsr_bank bk, const int32_t* __restrict__ table, int table_pag
     __syncthreads();
     f.pages(rows, v + KT, tid);
     f.codes(bk, h, pshift, v + KT, tid);
+    tile_marks<D, KT, 1, KT>(tile, 0, v / KT + 1, st, [&](int, int r) { return !(pos0 + v + r >= lo && pos0 + v + r < hi); });
     f16v s[NB][1];
     tile_logits<D, KT, NT, 1, NB>(tile, 0, col, half, qf, s);
-    if (__ballot(lo < pos0 + v + KT && hi > pos0 + v && lo < hi)) {
+    if (skip && __ballot(lo < pos0 + v + KT && hi > pos0 + v && lo < hi)) {
+      asm volatile("");
 #pragma unroll
       for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
@@ -213,8 +221,7 @@ k_bank_pages_page(gpsr_bank bk, const int32_t* __restrict__ table, int table_pag
           if (pos >= lo && pos < hi) s[kb][0][e] = -__builtin_inff();
         }
     }
-    tile_marks<D, KT, 1, NB>(tile, 0, half, v / KT + 1, s, st);
-    tile_accumulate<D, KT, NT, 1, NB>(tile, 0, col, half, c2, s, st);
+    tile_accumulate<D, KT, NT, 1, NB, true>(tile, 0, col, half, c2, s, st);
   }
   st.spoil();
   if (there) store_partial<D>(part + (((size_t)bh * T * n_sel + id) * G + g) * (D + 2), half, st, 0);
@@ -262,7 +269,6 @@ static void launch_pages(const PagesPlan& p, const gpsr_bank& bk, const int32_t*
   const int pshift = __builtin_ctz((unsigned)bk.page_rows), H = bk.heads, G = q_heads / H;
   const int64_t C = (int64_t)T * G;
   const dim3 join((unsigned)((C + 3) / 4), (unsigned)H, (unsigned)B);
-  const float c2 = scale * 1.4426950408889634f;
   if (!p.by_page) {
     float* part = (float*)ws;
     hipLaunchKernelGGL((k_bank_pages_query<DT, BITS, D>), dim3((unsigned)((int64_t)T * p.groups * p.splits), (unsigned)H, (unsigned)B),
@@ -270,7 +276,7 @@ static void launch_pages(const PagesPlan& p, const gpsr_bank& bk, const int32_t*
                        (E*)out, lse, p.groups, p.splits, part);
     if (p.splits > 1)
       hipLaunchKernelGGL((k_bank_join<DT, D>), join, dim3(256), 0, st, part, T, G, H, C, p.splits, (size_t)p.splits * C, (size_t)1,
-                         (size_t)p.splits * G, (size_t)G, c2, (E*)out, lse);
+                         (size_t)p.splits * G, (size_t)G, (E*)out, lse);
     return;
   }
   int *count = (int*)ws, *rank = (int*)(ws + p.rank), *start = (int*)(ws + p.start), *wgs = (int*)(ws + p.wgs), *list = (int*)(ws + p.list);
@@ -286,7 +292,7 @@ static void launch_pages(const PagesPlan& p, const gpsr_bank& bk, const int32_t*
   if (bk.page_rows <= 32) PAGE(32); else PAGE(64);
 #undef PAGE
   hipLaunchKernelGGL((k_bank_join<DT, D>), join, dim3(256), 0, st, part, T, G, H, C, n_sel, (size_t)n_sel * C, (size_t)1,
-                     (size_t)n_sel * G, (size_t)G, c2, (E*)out, lse);
+                     (size_t)n_sel * G, (size_t)G, (E*)out, lse);
 }
 
 extern "C" int gpsr_bank_attend_pages(const gpsr_bank* bank, const int32_t* table, int B, int table_pages, const int32_t* length,

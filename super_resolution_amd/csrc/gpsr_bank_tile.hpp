@@ -15,10 +15,12 @@ template <> struct Terms<GPSR_BF16> { static constexpr int N = 1; };
 template <> struct Terms<GPSR_F16> { static constexpr int N = 2; };
 template <> struct Terms<GPSR_F32> { static constexpr int N = 3; };
 
-// blocks of 32 columns that a wave holds: two halve the LDS reads for a product, where the registers allow it
-static constexpr int tile_nq(int d, int nt) { return nt == 1 && d <= 64 ? 2 : 1; }
-// waves per SIMD that the registers are budgeted for
-static constexpr int tile_waves(int d, int nt, int nq) { return (d * nq * (nt + 1)) / 4 + 32 * nq > 160 ? 1 : 2; }
+// registers that a wave of NQ x 32 columns and NB x 32 rows at a time needs, roughly: sums, logits, query terms, the rest
+static constexpr int tile_regs(int d, int nt, int nq, int nb) { return nq * (d / 2 + 16 * nb + nt * d / 4) + 64; }
+// waves per SIMD that they are budgeted for
+static constexpr int tile_waves(int d, int nt, int nq, int nb) {
+  return tile_regs(d, nt, nq, nb) <= 128 ? 4 : tile_regs(d, nt, nq, nb) <= 250 ? 2 : 1;
+}
 
 template <int DT>
 __device__ __forceinline__ typename Row<DT>::T from_f32(float y) {
@@ -55,12 +57,16 @@ __device__ __forceinline__ void load_query(const typename Row<DT>::T* __restrict
   }
 }
 
-// ---- the tile in LDS: keys [KT][D + 8], values [D][KT + 8] (rows permuted as above), offsets [KT], rows whose values are NaN
-static constexpr int tile_lds(int d, int kt) { return (kt * (d + 8) + d * (kt + 8)) * 2 + kt * 4 + (kt * (d / 32) + 4) * 4; }
+// ---- the tile in LDS: keys [KT][D + 8], values [D][KT] (rows of the bank permuted as above), offsets [KT], marks
+// The values' 16-byte granules are exchanged within each 8 by the column's number: a wave writes 8 rows x 8 columns at a time,
+// 8 columns apart, and reads 8 neighbouring columns, and neither falls on the same banks (with padded rows instead, 80 % of
+// the LDS cycles of 180 000 rows x 12 queries were conflicts: 153 against 87 us).
+static constexpr int tile_lds(int d, int kt) { return (kt * (d + 8) + d * kt) * 2 + kt * 4 + (kt * (d / 32) + 4) * 4; }
 
 template <int D, int KT>
 struct Tile {
-  static constexpr int KS = D + 8, VS = KT + 8;
+  static constexpr int KS = D + 8, VS = KT;
+  static constexpr int SWZ = (KT >= 64 ? 7 : KT / 8 - 1);   // granules of a row that may change places
   uint16_t *k, *v;
   float* off;
   // A value group that is NaN is held as zeros, so that it cannot reach queries that do not see its row (0 * NaN); who does
@@ -70,8 +76,10 @@ struct Tile {
   __device__ Tile(char* sm) {
     k = (uint16_t*)sm; v = k + KT * KS; off = (float*)(v + D * VS); mark = (unsigned*)(off + KT);
   }
-  __device__ void clear_marks(int tid) {
-    for (int i = tid; i < KT * (D / 32) + 1; i += 256) mark[i] = 0;
+  // where slot s of column c lies
+  __device__ __forceinline__ static int at(int c, int s) { return c * VS + (s ^ (((c ^ (c >> 3)) & SWZ) << 3)); }
+  __device__ void clear_marks(int tid, int threads) {
+    for (int i = tid; i < KT * (D / 32) + 1; i += threads) mark[i] = 0;
   }
 };
 
@@ -88,15 +96,16 @@ __device__ __forceinline__ unsigned pair(unsigned w0, unsigned w1, float s) {
 }
 
 // ---- where the rows of a walk come from: page(v) is the physical page of row v of the walk (-1: no such row), left(v) how many
-// of the rows v .. v + 3 (one page's) exist.  Row v lies at v % page_rows of its page.
+// of the rows v .. v + 3 (one page's) exist.  Row v lies at v % page_rows of its page.  A walk has at least one row (len, n > 0);
+// lookups behind its end read its last entry and are then discarded, which costs less than a branch.
 struct WholeBank {
   const int32_t* tab;
   int64_t pages;
   int pshift;
   unsigned len;
   __device__ __forceinline__ int page(unsigned v) const {
-    const int p = v < len ? tab[v >> pshift] : -1;
-    return (unsigned)p < (unsigned)pages ? p : -1;
+    const int p = tab[min(v, len - 1) >> pshift];
+    return v < len && (unsigned)p < (unsigned)pages ? p : -1;
   }
   __device__ __forceinline__ int left(unsigned v) const { return v < len ? (int)min(len - v, 4u) : 0; }
 };
@@ -104,10 +113,14 @@ struct PageList {   // in LDS: physical pages and how many rows each has
   const int *phys, *rows;
   int pshift;
   unsigned n;
-  __device__ __forceinline__ int page(unsigned v) const { return left(v) > 0 ? phys[v >> pshift] : -1; }
+  __device__ __forceinline__ int page(unsigned v) const {
+    const int p = phys[min(v >> pshift, n - 1)];
+    return left(v) > 0 ? p : -1;
+  }
   __device__ __forceinline__ int left(unsigned v) const {
     const unsigned i = v >> pshift;
-    return i < n ? min(rows[i] - (int)(v & ((1u << pshift) - 1)), 4) : 0;
+    const int r = rows[min(i, n - 1)] - (int)(v & ((1u << pshift) - 1));
+    return i < n ? min(r, 4) : 0;
   }
 };
 struct OnePage {
@@ -116,63 +129,66 @@ struct OnePage {
   __device__ __forceinline__ int left(unsigned v) const { return min(rows - (int)v, 4); }
 };
 
-// ---- a tile on its way: codes are loaded a tile ahead of their use, page numbers two
-template <int BITS, int D, int KT>
+// ---- a tile on its way: codes are loaded a tile ahead of their use, page numbers two.  The tile is 2 U units, U of keys (32
+// columns of a row each) and U of values (8 columns of 4 rows each), dealt to the threads in that order: a thread has one kind or
+// the other at a time and holds both in the same registers.
+template <int BITS, int D, int KT, int NTH>
 struct Fetch {
-  static constexpr int U = KT * D / 32;                  // units of keys (a row's 32 columns) and of values (4 rows x 8 columns)
-  static constexpr int NU = (U + 255) / 256;
+  static constexpr int U = KT * D / 32, N = (2 * U + NTH - 1) / NTH;
   static constexpr int W = BITS / 4;                     // code words of 8 columns
-  int kpage[NU], vpage[NU];                              // -1: the row does not exist
-  int fk[NU];
-  unsigned kw[NU][4 * W], vw[NU][4][W];
-  unsigned ks[NU];
-  unsigned vs[NU][4];
-  int vleft[NU], fleft[NU];
-  float offs[NU];
+  static constexpr bool EVEN = 2 * U % NTH == 0;
+  int page[N], left[N];                                  // of the next tile; page -1: the row does not exist
+  int fpage[N], fleft[N];                                // of the tile whose codes are under way
+  unsigned w[N][4 * W], sc[N][4];                        // keys: scale byte and offset in sc[0], sc[1]
+
+  // unit i of this thread: keys? and its number among its kind
+  __device__ __forceinline__ static bool keys(int i, int tid) {
+    return NTH * (i + 1) <= U ? true : NTH * i >= U ? false : tid + NTH * i < U;
+  }
+  __device__ __forceinline__ static int row(int i, int tid) {
+    const int u = tid + NTH * i;
+    return keys(i, tid) ? u / (D / 32) : (u - U) / (D / 8) * 4;
+  }
 
   // page numbers of the rows from p0 on
   template <class Rows>
   __device__ __forceinline__ void pages(const Rows& rows, unsigned p0, int tid) {
 #pragma unroll
-    for (int i = 0; i < NU; ++i) {
-      const int u = tid + 256 * i, x = 255 - tid + 256 * i;
-      const unsigned kr = p0 + u / (D / 32), vr = p0 + x / (D / 8) * 4;
-      kpage[i] = u < U ? rows.page(kr) : -1;
-      vpage[i] = x < U ? rows.page(vr) : -1;
-      vleft[i] = rows.left(vr);
+    for (int i = 0; i < N; ++i) {
+      const unsigned r = p0 + row(i, tid);
+      page[i] = rows.page(r);
+      left[i] = rows.left(r);
     }
   }
 
-  // codes, scales and offsets of the rows whose pages were fetched last
+  // codes, scales and offsets of the rows whose pages were fetched last; for a row that does not exist, some other one's
   __device__ __forceinline__ void codes(const gpsr_bank& bk, int h, int pshift, unsigned p0, int tid) {
     const unsigned mask = (1u << pshift) - 1;
 #pragma unroll
-    for (int i = 0; i < NU; ++i) {
-      const int u = tid + 256 * i, x = 255 - tid + 256 * i;
-      fk[i] = kpage[i];
-      if (kpage[i] >= 0) {
-        const int r = u / (D / 32), g = u % (D / 32);
-        const size_t row = (((size_t)kpage[i] * bk.heads + h) << pshift) + ((p0 + r) & mask);
-        const u4v* src = (const u4v*)(bk.k_codes + row * (size_t)(D * BITS / 8) + g * (4 * BITS));
+    for (int i = 0; i < N; ++i) {
+      const int u = tid + NTH * i;
+      fpage[i] = page[i]; fleft[i] = page[i] >= 0 ? left[i] : 0;
+      if (!EVEN && u >= 2 * U) continue;
+      const size_t at = (((size_t)max(page[i], 0) * bk.heads + h) << pshift) + ((p0 + row(i, tid)) & mask);
+      if (keys(i, tid)) {
+        const int g = u % (D / 32);
+        const u4v* src = (const u4v*)(bk.k_codes + at * (size_t)(D * BITS / 8) + g * (4 * BITS));
 #pragma unroll
         for (int j = 0; j < W; ++j) {
           const u4v a = src[j];
-          kw[i][4 * j] = a.x; kw[i][4 * j + 1] = a.y; kw[i][4 * j + 2] = a.z; kw[i][4 * j + 3] = a.w;
+          w[i][4 * j] = a.x; w[i][4 * j + 1] = a.y; w[i][4 * j + 2] = a.z; w[i][4 * j + 3] = a.w;
         }
-        ks[i] = bk.k_scales[row * (size_t)(D / 32) + g];
-        if (g == 0) offs[i] = bk.offset[row];
-      }
-      fleft[i] = vpage[i] >= 0 ? vleft[i] : 0;
-      if (vpage[i] >= 0) {
-        const int r = x / (D / 8) * 4, c = x % (D / 8);
-        const size_t row = (((size_t)vpage[i] * bk.heads + h) << pshift) + ((p0 + r) & mask);
-        const uint8_t* src = bk.v_codes + row * (size_t)(D * BITS / 8) + c * BITS;
-        const uint8_t* sc = bk.v_scales + row * (size_t)(D / 32) + c / 4;
+        sc[i][0] = bk.k_scales[at * (size_t)(D / 32) + g];
+        sc[i][1] = __float_as_uint(bk.offset[at]);
+      } else {
+        const int c = (u - U) % (D / 8);
+        const uint8_t* src = bk.v_codes + at * (size_t)(D * BITS / 8) + c * BITS;
+        const uint8_t* scale = bk.v_scales + at * (size_t)(D / 32) + c / 4;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {   // rows of one page: P is a multiple of 16
-          if constexpr (W == 1) vw[i][j][0] = *(const unsigned*)(src + j * (D * BITS / 8));
-          else { const u2v a = *(const u2v*)(src + j * (D * BITS / 8)); vw[i][j][0] = a.x; vw[i][j][1] = a.y; }
-          vs[i][j] = sc[j * (D / 32)];
+        for (int j = 0; j < 4; ++j) {   // rows of one page: page_rows is a multiple of 16
+          if constexpr (W == 1) w[i][j] = *(const unsigned*)(src + j * (D * BITS / 8));
+          else { const u2v a = *(const u2v*)(src + j * (D * BITS / 8)); w[i][2 * j] = a.x; w[i][2 * j + 1] = a.y; }
+          sc[i][j] = scale[j * (D / 32)];
         }
       }
     }
@@ -181,39 +197,39 @@ struct Fetch {
   // decodes them to LDS; rows that do not exist become zeros with an offset of -inf
   __device__ __forceinline__ void store(const Tile<D, KT>& tile, int tid, unsigned number) {
 #pragma unroll
-    for (int i = 0; i < NU; ++i) {
-      const int u = tid + 256 * i, x = 255 - tid + 256 * i;
-      if (u < U) {
-        const int r = u / (D / 32), g = u % (D / 32);
-        const bool there = fk[i] >= 0;
+    for (int i = 0; i < N; ++i) {
+      const int u = tid + NTH * i;
+      if (!EVEN && u >= 2 * U) continue;
+      const int r = row(i, tid);
+      if (keys(i, tid)) {
+        const int g = u % (D / 32);
+        const bool there = fpage[i] >= 0;
         u4v* dst = (u4v*)(tile.k + r * Tile<D, KT>::KS + g * 32);
-        const float s = scale_of(there ? ks[i] : 127u);
+        const float s = scale_of(there ? sc[i][0] : 127u);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const unsigned w0 = there ? kw[i][W * j] : 0u, w1 = there ? kw[i][W * j + W - 1] : 0u;
+          const unsigned w0 = there ? w[i][W * j] : 0u, w1 = there ? w[i][W * j + W - 1] : 0u;
           dst[j] = u4v{pair<BITS, 0>(w0, w1, s), pair<BITS, 1>(w0, w1, s), pair<BITS, 2>(w0, w1, s), pair<BITS, 3>(w0, w1, s)};
         }
-        if (g == 0) tile.off[r] = there ? offs[i] : -__builtin_inff();
-      }
-      if (x < U) {
-        const int r = x / (D / 8) * 4, c = x % (D / 8);
+        if (g == 0) tile.off[r] = there ? __uint_as_float(sc[i][1]) : -__builtin_inff();
+      } else {
+        const int c = (u - U) % (D / 8);
         unsigned y[4][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const bool here = j < fleft[i], nan = here && vs[i][j] == 255u, there = here && !nan;
+          const bool here = j < fleft[i], nan = here && sc[i][j] == 255u, there = here && !nan;
           if (nan) { tile.mark[(r + j) * (D / 32) + c / 4] = number; tile.mark[KT * (D / 32)] = number; }
-          const float s = scale_of(there ? vs[i][j] : 127u);
-          const unsigned w0 = there ? vw[i][j][0] : 0u, w1 = there ? vw[i][j][W - 1] : 0u;
+          const float s = scale_of(there ? sc[i][j] : 127u);
+          const unsigned w0 = there ? w[i][W * j] : 0u, w1 = there ? w[i][W * j + W - 1] : 0u;
           y[j][0] = pair<BITS, 0>(w0, w1, s); y[j][1] = pair<BITS, 1>(w0, w1, s);
           y[j][2] = pair<BITS, 2>(w0, w1, s); y[j][3] = pair<BITS, 3>(w0, w1, s);
         }
         // rows r .. r + 3 of the tile are 4 neighbouring slots of a column
         const int k16 = r & 15, slot = (r & ~15) + ((k16 >> 2) & 1) * 8 + (k16 >> 3) * 4;
-        uint16_t* dst = tile.v + (c * 8) * Tile<D, KT>::VS + slot;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          *(u2v*)(dst + (2 * e) * Tile<D, KT>::VS) = u2v{pack_lo(y[0][e], y[1][e]), pack_lo(y[2][e], y[3][e])};
-          *(u2v*)(dst + (2 * e + 1) * Tile<D, KT>::VS) = u2v{pack_hi(y[0][e], y[1][e]), pack_hi(y[2][e], y[3][e])};
+          *(u2v*)(tile.v + Tile<D, KT>::at(c * 8 + 2 * e, slot)) = u2v{pack_lo(y[0][e], y[1][e]), pack_lo(y[2][e], y[3][e])};
+          *(u2v*)(tile.v + Tile<D, KT>::at(c * 8 + 2 * e + 1, slot)) = u2v{pack_hi(y[0][e], y[1][e]), pack_hi(y[2][e], y[3][e])};
         }
       }
     }
@@ -249,7 +265,8 @@ __device__ __forceinline__ void tile_logits(const Tile<D, KT>& tile, int wrow, i
 
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
 
-// ---- running softmax of a wave's columns: m the maximum raw logit, l this half's sum of weights, o = sum of weights * values
+// ---- running softmax of a wave's columns: m the power of two that weights are taken against
+// (logit * log2 e; -inf: no row seen), l this half's sum of weights, o = sum of weights * values
 template <int D, int NQ>
 struct Soft {
   f16v o[D / 32][NQ];
@@ -265,6 +282,19 @@ struct Soft {
         for (int e = 0; e < 16; ++e) o[d][n][e] = 0.f;
     }
   }
+  __device__ __forceinline__ bool wants_move() const {
+    bool x = false;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) x |= m[n] == -__builtin_inff() || l[n] > 0x1p40f;
+    return __ballot(x) != 0;
+  }
+  // whether a sum ran out of range (or met a NaN: then a second walk changes nothing)
+  __device__ __forceinline__ bool lost() const {
+    bool x = false;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) x |= !(l[n] < __builtin_inff());
+    return x;
+  }
   __device__ __forceinline__ void rescale(int n, float a) {
     l[n] *= a;
 #pragma unroll
@@ -275,7 +305,7 @@ struct Soft {
   __device__ __forceinline__ void spoil() {
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-      const unsigned all = nan[n] | __shfl_xor(nan[n], 32);
+      const unsigned all = nan[n];
       if (__ballot(all != 0))
 #pragma unroll
         for (int d = 0; d < D / 32; ++d)
@@ -285,7 +315,7 @@ struct Soft {
     }
   }
   // divides; l becomes the whole sum
-  __device__ __forceinline__ void finish(int n, float c2) {
+  __device__ __forceinline__ void finish(int n) {
     l[n] += other_half(l[n]);
     const float r = l[n] == 0.f ? 0.f : 1.f / l[n];
 #pragma unroll
@@ -293,12 +323,12 @@ struct Soft {
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[d][n][e] *= r;
   }
-  __device__ __forceinline__ float lse(int n, float c2) const {
-    return l[n] == 0.f ? -__builtin_inff() : (log2f(l[n]) + m[n] * c2) * 0.6931471805599453f;
+  __device__ __forceinline__ float lse(int n) const {
+    return l[n] == 0.f ? -__builtin_inff() : (log2f(l[n]) + m[n]) * 0.6931471805599453f;
   }
   // wave 0 gets the sum over WK waves that held the same columns; buf: 64 x (D / 2 + 2) floats for each block of columns
   template <int WK>
-  __device__ __forceinline__ void join(float* buf, int wave, int lane, float c2) {
+  __device__ __forceinline__ void join(float* buf, int wave, int lane) {
     for (int w = 1; w < WK; ++w) {
       if (wave == w) {
 #pragma unroll
@@ -317,7 +347,7 @@ struct Soft {
         for (int n = 0; n < NQ; ++n) {
           const float* p = buf + n * 64 * (D / 2 + 2);
           const float m2 = p[lane], mn = fmaxf(m[n], m2), safe = mn == -__builtin_inff() ? 0.f : mn;
-          const float a = exp2f((m[n] - safe) * c2), b = exp2f((m2 - safe) * c2);
+          const float a = exp2f(m[n] - safe), b = exp2f(m2 - safe);
           m[n] = mn;
           l[n] = l[n] * a + p[64 + lane] * b;
 #pragma unroll
@@ -331,46 +361,51 @@ struct Soft {
   }
 };
 
-// rows that a column sees and whose values are NaN
-template <int D, int KT, int NQ, int NB>
-__device__ __forceinline__ void tile_marks(const Tile<D, KT>& tile, int wrow, int half, unsigned number, const f16v (&s)[NB][NQ],
-                                           Soft<D, NQ>& st) {
+// Rows of the tile that a column sees and whose values are NaN; seen(n, r): whether column n does not skip row r of the wave's.
+template <int D, int KT, int NQ, int KW, class Seen>
+__device__ __forceinline__ void tile_marks(const Tile<D, KT>& tile, int wrow, unsigned number, Soft<D, NQ>& st, const Seen& seen) {
   if (tile.mark[KT * (D / 32)] != number) return;
+#pragma unroll 1
+  for (int r = 0; r < KW; ++r) {
+    if (tile.off[wrow + r] == -__builtin_inff()) continue;
+    unsigned bits = 0;
+    for (int g = 0; g < D / 32; ++g) bits |= (tile.mark[(wrow + r) * (D / 32) + g] == number ? 1u : 0u) << g;
 #pragma unroll
-  for (int n = 0; n < NQ; ++n)
-#pragma unroll
-    for (int kb = 0; kb < NB; ++kb)
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (s[kb][n][e] != -__builtin_inff())
-          for (int g = 0; g < D / 32; ++g)
-            if (tile.mark[(wrow + kb * 32 + 8 * (e >> 2) + 4 * half + (e & 3)) * (D / 32) + g] == number) st.nan[n] |= 1u << g;
+    for (int n = 0; n < NQ; ++n) st.nan[n] |= seen(n, r) ? bits : 0u;
+  }
 }
 
-// one step of the running softmax: logits in, weights times values added to the state
-template <int D, int KT, int NT, int NQ, int NB>
+// One step of the running softmax: logits in, weights times values added to the state.
+//   MOVE: the reference becomes the maximum so far, as a power of two (weights are at most 1), and the state is rescaled.
+//   otherwise it stays, which saves the maximum of every tile and the wait for it: bf16 and the sums have range to spare, and
+//     their precision is relative.  Soft::wants_move says when it has to be moved (nothing seen yet, or a sum past 2^40); a
+//     weight past 2^127 makes the sum infinite, which the caller has to look for (Soft::lost) and walk again with MOVE only.
+template <int D, int KT, int NT, int NQ, int NB, bool MOVE>
 __device__ __forceinline__ void tile_accumulate(const Tile<D, KT>& tile, int wrow, int col, int half, float c2, f16v (&s)[NB][NQ],
                                                 Soft<D, NQ>& st) {
+  if constexpr (MOVE) {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      float mx = s[0][n][0];
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[kb][n][e]);
+      float mn = fmaxf(st.m[n], fmaxf(mx, other_half(mx)) * c2);
+      if (fmaxf(st.l[n], other_half(st.l[n])) > 0x1p40f) mn = fmaxf(mn, st.m[n] + 40.f);
+      st.rescale(n, mn == -__builtin_inff() ? 1.f : exp2f(st.m[n] - mn));
+      st.m[n] = mn;
+    }
+  }
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
-    float mx = s[0][n][0];
-#pragma unroll
-    for (int kb = 0; kb < NB; ++kb)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[kb][n][e]);
-    mx = fmaxf(mx, other_half(mx));
-    const float mn = fmaxf(st.m[n], mx);
-    const float safe = mn == -__builtin_inff() ? 0.f : mn;
-    // most tiles bring no new maximum once the first few have been seen
-    if (__ballot(mn > st.m[n])) st.rescale(n, exp2f((st.m[n] - safe) * c2));
-    st.m[n] = mn;
-    const float nb = -safe * c2;
+    const float ref = st.m[n] == -__builtin_inff() ? 0.f : -st.m[n];
     float sum = 0.f;
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const float w = __builtin_amdgcn_exp2f(fmaf(s[kb][n][e], c2, nb));
+        const float w = __builtin_amdgcn_exp2f(fmaf(s[kb][n][e], c2, ref));
         s[kb][n][e] = w;
         sum += w;
       }
@@ -388,10 +423,9 @@ __device__ __forceinline__ void tile_accumulate(const Tile<D, KT>& tile, int wro
         for (int e = 0; e < 8; ++e) y[e] = s[kb][n][8 * k + e];
         split_terms<NT>(y, p[n]);
       }
-      const uint16_t* base = tile.v + col * Tile<D, KT>::VS + wrow + kb * 32 + k * 16 + half * 8;
 #pragma unroll
       for (int d = 0; d < D / 32; ++d) {
-        const bf8 a = *(const bf8*)(base + d * 32 * Tile<D, KT>::VS);
+        const bf8 a = *(const bf8*)(tile.v + Tile<D, KT>::at(d * 32 + col, wrow + kb * 32 + k * 16 + half * 8));
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
 #pragma unroll
@@ -421,7 +455,7 @@ __device__ __forceinline__ void store_column(typename Row<DT>::T* __restrict__ o
     }
 }
 
-// [D] sums, maximum raw logit, sum of weights
+// [D] sums, reference logit, sum of weights
 template <int D, int NQ>
 __device__ __forceinline__ void store_partial(float* __restrict__ p, int half, Soft<D, NQ>& st, int n) {
   const float l = st.l[n] + other_half(st.l[n]);
@@ -439,7 +473,7 @@ __device__ __forceinline__ void store_partial(float* __restrict__ p, int half, S
 template <int DT, int D>
 __global__ void __launch_bounds__(256)
 k_bank_join(const float* __restrict__ part, int T, int G, int H, int64_t C, int n, size_t per_bh, size_t per_g, size_t per_t,
-            size_t per_i, float c2, typename Row<DT>::T* __restrict__ out, float* __restrict__ lse) {
+            size_t per_i, typename Row<DT>::T* __restrict__ out, float* __restrict__ lse) {
   const int lane = threadIdx.x & 63;
   const int64_t c = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (c >= C) return;
@@ -457,7 +491,7 @@ k_bank_join(const float* __restrict__ part, int T, int G, int H, int64_t C, int 
   for (int i = 0; i < n; ++i) {
     const float li = p[i * step + D + 1];
     if (li == 0.f) continue;             // saw nothing: its sums were not written
-    const float w = exp2f((p[i * step + D] - safe) * c2);
+    const float w = exp2f(p[i * step + D] - safe);
     l = fmaf(w, li, l);
 #pragma unroll
     for (int e = 0; e < E; ++e) if (e * 64 + lane < D) acc[e] = fmaf(w, p[i * step + e * 64 + lane], acc[e]);
@@ -466,7 +500,7 @@ k_bank_join(const float* __restrict__ part, int T, int G, int H, int64_t C, int 
 #pragma unroll
   for (int e = 0; e < E; ++e)
     if (e * 64 + lane < D) o[e * 64 + lane] = from_f32<DT>(l == 0.f ? 0.f : acc[e] / l);
-  if (lse && lane == 0) lse[((size_t)b * (H * G) + hq) * T + t] = l == 0.f ? -__builtin_inff() : (log2f(l) + m * c2) * 0.6931471805599453f;
+  if (lse && lane == 0) lse[((size_t)b * (H * G) + hq) * T + t] = l == 0.f ? -__builtin_inff() : (log2f(l) + m) * 0.6931471805599453f;
 }
 
 // ---- host side
