@@ -296,17 +296,23 @@ k_bank_select_pick(gpsr_bank bk, const int32_t* __restrict__ table, int J, int p
       const int64_t page = lp < n_all ? table[(size_t)b * J + lp] : -1;
       if (page >= 0 && page < bk.pages && !(lp >= slo && lp < shi)) {
         const f4v* c = (const f4v*)(bk.centroid + ((size_t)page * H + h) * D);
-        double dot = 0.0, sq = 0.0;
-        for (int d = 0; d < D / 4; ++d) {
-          const f4v y = c[d];
+        // 32 columns on their way at a time, four chains of sums
+        double dot[4] = {0, 0, 0, 0}, sq[4] = {0, 0, 0, 0};
+        for (int g = 0; g < D / 32; ++g) {
+          f4v y[8];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const double z = (double)y[j];
-            dot = fma(qv[slot][4 * d + j], z, dot);
-            if (rbf) sq = fma(z, z, sq);
-          }
+          for (int d = 0; d < 8; ++d) y[d] = c[8 * g + d];
+#pragma unroll
+          for (int d = 0; d < 8; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const double z = (double)y[d][j];
+              dot[j] = fma(qv[slot][32 * g + 4 * d + j], z, dot[j]);
+              if (rbf) sq[j] = fma(z, z, sq[j]);
+            }
         }
-        const double s = rbf ? dot - 0.5 * G * sq : dot;
+        const double all = (dot[0] + dot[1]) + (dot[2] + dot[3]);
+        const double s = rbf ? all - 0.5 * G * ((sq[0] + sq[1]) + (sq[2] + sq[3])) : all;
         if (s == s) x = {s, lp};
       }
     }

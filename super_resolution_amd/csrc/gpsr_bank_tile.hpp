@@ -468,8 +468,10 @@ __device__ __forceinline__ void store_partial(float* __restrict__ p, int half, S
   if (half == 0) { p[D] = st.m[n]; p[D + 1] = l; }
 }
 
-// Joins the partial results of one column: one wave per column, lanes over the dim.  Column (t, g) of bank head bh has its n
-// partials [D + 2] at bh * per_bh + t * per_t + g * per_g + i * per_i.
+// Joins the partial results of one column, at most 64: one wave per column.  First lane i weighs partial i, then the lanes
+// spread over the dim and eight partials are on their way at a time (with the weights formed along the way each load waited for
+// the one before it: 30 against 9 us for 64 partials of 96 columns).  Column (t, g) of bank head bh has its n partials [D + 2]
+// at bh * per_bh + t * per_t + g * per_g + i * per_i.
 template <int DT, int D>
 __global__ void __launch_bounds__(256)
 k_bank_join(const float* __restrict__ part, int T, int G, int H, int64_t C, int n, size_t per_bh, size_t per_g, size_t per_t,
@@ -482,25 +484,35 @@ k_bank_join(const float* __restrict__ part, int T, int G, int H, int64_t C, int 
   const int g = (int)(c - t * G), hq = h * G + g;
   const float* p = part + ((size_t)(b * H + h) * per_bh + t * per_t + g * per_g) * (D + 2);
   const size_t step = per_i * (D + 2);
-  float m = -__builtin_inff();
-  for (int i = lane; i < n; i += 64) if (p[i * step + D + 1] != 0.f) m = fmaxf(m, p[i * step + D]);
-  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-  const float safe = m == -__builtin_inff() ? 0.f : m;
+  float m = -__builtin_inff(), l = 0.f;
+  if (lane < n) { l = p[lane * step + D + 1]; m = p[lane * step + D]; }
+  const unsigned long long used = __ballot(l != 0.f);      // the others saw nothing, and their sums were not written
+  float top = l != 0.f ? m : -__builtin_inff();
+  for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  const float w = l != 0.f ? exp2f(m - (top == -__builtin_inff() ? 0.f : top)) : 0.f;
+  l = l != 0.f ? l * w : 0.f;
+  for (int o = 32; o; o >>= 1) l += __shfl_xor(l, o);
   constexpr int E = (D + 63) / 64;
-  float acc[E] = {}, l = 0.f;
-  for (int i = 0; i < n; ++i) {
-    const float li = p[i * step + D + 1];
-    if (li == 0.f) continue;             // saw nothing: its sums were not written
-    const float w = exp2f(p[i * step + D] - safe);
-    l = fmaf(w, li, l);
+  float acc[E] = {};
+  for (int i0 = 0; i0 < n; i0 += 8) {
+    float y[8][E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) if (e * 64 + lane < D) acc[e] = fmaf(w, p[i * step + e * 64 + lane], acc[e]);
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int e = 0; e < E; ++e) y[j][e] = p[min(i0 + j, n - 1) * step + min(e * 64 + lane, D - 1)];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const bool use = used >> (i0 + j) & 1;
+      const float wj = __shfl(w, i0 + j);
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = use ? fmaf(wj, y[j][e], acc[e]) : acc[e];
+    }
   }
   typename Row<DT>::T* o = out + (((size_t)b * T + t) * (size_t)(H * G) + hq) * D;
 #pragma unroll
   for (int e = 0; e < E; ++e)
     if (e * 64 + lane < D) o[e * 64 + lane] = from_f32<DT>(l == 0.f ? 0.f : acc[e] / l);
-  if (lse && lane == 0) lse[((size_t)b * (H * G) + hq) * T + t] = l == 0.f ? -__builtin_inff() : (log2f(l) + m) * 0.6931471805599453f;
+  if (lse && lane == 0) lse[((size_t)b * (H * G) + hq) * T + t] = l == 0.f ? -__builtin_inff() : (log2f(l) + top) * 0.6931471805599453f;
 }
 
 // ---- host side

@@ -4,6 +4,7 @@ PyTorch is plumbing here: it owns device memory and the HIP stream; all
 arithmetic on the path happens in libgpsr.so.  Every function requires CUDA
 (ROCm) tensors and raises otherwise -- there is no CPU path.
 """
+import ctypes
 from typing import NamedTuple
 
 import numpy as np
@@ -17,7 +18,7 @@ BLOCK = 112
 
 
 def _stream():
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _p(t, dtype=None):
@@ -404,6 +405,7 @@ BANK_GROUP = 32                              # columns that share a scale byte
 BANK_DIMS = (32, 64, 96, 128, 192, 256)
 BANK_PAGE_ROWS = (16, 32, 64, 128, 256)
 _BANK_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_I64x3 = ctypes.c_int64 * 3
 
 
 class Bank(NamedTuple):
@@ -435,89 +437,116 @@ def bank_alloc(pages, heads, dim, page_rows=64, bits=4, kernel_id=RBF, device=No
     return Bank(u8(width), u8(groups), u8(width), u8(groups), f32(page_rows), f32(dim), bits, kernel_id)
 
 
-def _bank(bank):
-    """The checked gpsr_bank of a Bank, and (pages, heads, page_rows, dim)."""
-    import ctypes
-    pages, H, P, width = bank.k_codes.shape
-    if bank.bits not in (4, 8):
-        raise _lib.GpsrError(f"bank: bits must be 4 or 8, got {bank.bits}")
-    D = width * 8 // bank.bits
-    want = ((pages, H, P, width), (pages, H, P, D // BANK_GROUP)) * 2 + ((pages, H, P), (pages, H, D))
-    got = tuple(tuple(t.shape) for t in bank[:6])
-    if got != want:
-        raise _lib.GpsrError(f"bank: array shapes {got}, expected {want}")
-    ptrs = [_p(t, torch.uint8) for t in bank[:4]] + [_p(t, torch.float32) for t in bank[4:6]]
-    s = _lib.Bank(*ptrs, pages, H, P, D, bank.bits, bank.kernel_id)
-    return ctypes.byref(s), (pages, H, P, D)
+# The bank_* calls take a dozen tensors and some of them run for a few microseconds: the checks below ask torch as little as
+# they can and leave the words of a refusal to _p.
+def _ptr(t, dtype, dev):
+    if t.get_device() != dev or t.dtype is not dtype or not t.is_contiguous():
+        return _p(t, dtype)
+    return t.data_ptr()
 
 
-def _strided(t, shape, what):
-    """Pointer, dtype code and (first three) element strides of a [B,T,H,D] tensor whose columns are contiguous."""
-    import ctypes
-    if t.dim() != 4 or any(w is not None and w != g for w, g in zip(shape, t.shape)):
-        raise _lib.GpsrError(f"{what}: expected [B,T,heads,dim] = {shape}, got {tuple(t.shape)}")
-    if t.dtype not in _BANK_TYPES:
+def _bank_device(t):
+    dev = t.get_device()
+    if dev < 0 or dev != torch.cuda.current_device():
+        _p(t)                            # says what is wrong
+    return dev
+
+
+def _bank(bank, dev):
+    """The checked gpsr_bank of a Bank, and its heads and dim."""
+    kc, ks, vc, vs, off, cent, bits, kernel_id = bank
+    if kc.dim() != 4 or bits not in (4, 8):
+        raise _lib.GpsrError(f"bank: bits must be 4 or 8 and codes [pages,H,P,width], got {bits}, {tuple(kc.shape)}")
+    pages, H, P, width = shape = kc.shape
+    D = width * 8 // bits
+    groups = (pages, H, P, D // BANK_GROUP)
+    if vc.shape != shape or ks.shape != groups or vs.shape != groups or off.shape != (pages, H, P) or cent.shape != (pages, H, D):
+        raise _lib.GpsrError(f"bank: array shapes {[tuple(t.shape) for t in bank[:6]]} do not belong together")
+    u8, f32 = torch.uint8, torch.float32
+    return ctypes.byref(_lib.Bank(_ptr(kc, u8, dev), _ptr(ks, u8, dev), _ptr(vc, u8, dev), _ptr(vs, u8, dev), _ptr(off, f32, dev),
+                                  _ptr(cent, f32, dev), pages, H, P, D, bits, kernel_id)), H, D
+
+
+def _strided(t, B, H, D, dev, what):
+    """Pointer, dtype code and (first three) element strides of a [B,T,H,D] tensor whose columns are contiguous (H None: any)."""
+    shape = t.shape
+    if len(shape) != 4 or shape[0] != B or shape[3] != D or (H is not None and shape[2] != H):
+        raise _lib.GpsrError(f"{what}: expected [{B},T,{'heads' if H is None else H},{D}], got {tuple(shape)}")
+    code = _BANK_TYPES.get(t.dtype)
+    if code is None:
         raise _lib.GpsrError(f"{what}: expected bfloat16, float16 or float32, got {t.dtype}")
-    if t.shape[3] > 1 and t.stride(3) != 1:
+    sb, st, sh, sd = t.stride()
+    if sd != 1:
         raise _lib.GpsrError(f"{what}: the columns must be contiguous")
-    _p(t.as_strided((0,), (1,)))     # device checks
-    return t.data_ptr(), _BANK_TYPES[t.dtype], (ctypes.c_int64 * 3)(*t.stride()[:3])
+    if t.get_device() != dev:
+        _p(t.as_strided((0,), (1,)))     # says what is wrong
+    return t.data_ptr(), code, _I64x3(sb, st, sh)
 
 
-def _bank_index(table, per_entry, what):
+def _bank_index(table, per_entry, dev, what):
     """Pointers of table [B,J] and of one int32 per entry."""
-    if table.dim() != 2 or any(t.shape != (table.shape[0],) for t in per_entry):
+    if table.dim() != 2 or any(t.shape != table.shape[:1] for t in per_entry):
         raise _lib.GpsrError(f"{what}: expected a [B,J] table and [B] integers, got {tuple(table.shape)}, "
                              f"{[tuple(t.shape) for t in per_entry]}")
-    return _p(table, torch.int32), [_p(t, torch.int32) for t in per_entry]
+    return (_ptr(table, torch.int32, dev), *[_ptr(t, torch.int32, dev) for t in per_entry])
 
 
 def bank_write(bank, table, start, count, k, v):
     """Rounds rows k, v [B,T,H,D] (bfloat16 / float16 / float32, any strides with contiguous columns) into the bank, in place:
     row t < count[b] goes to position start[b] + t of entry b, whose pages table [B,J] (int32) names; refreshes offsets and
     centroids (gpsr_bank_write).  A page may be written by one entry of a call only."""
-    lib = _lib.load()
-    ref, (_, H, P, D) = _bank(bank)
-    tp, (sp, cp) = _bank_index(table, (start, count), "bank_write")
-    B = table.shape[0]
-    kp, dt, kst = _strided(k, (B, None, H, D), "bank_write: k")
-    if v.shape != k.shape or v.dtype != k.dtype:
+    lib, dev = _lib.load(), _bank_device(table)
+    ref, H, D = _bank(bank, dev)
+    tp, sp, cp = _bank_index(table, (start, count), dev, "bank_write")
+    B, J = table.shape
+    kp, code, kst = _strided(k, B, H, D, dev, "bank_write: k")
+    if v.shape != k.shape or v.dtype is not k.dtype:
         raise _lib.GpsrError(f"bank_write: v {tuple(v.shape)} {v.dtype} does not fit k {tuple(k.shape)} {k.dtype}")
-    vp, _, vst = _strided(v, (B, None, H, D), "bank_write: v")
-    _lib.check(lib.gpsr_bank_write(ref, tp, B, table.shape[1], sp, cp, kp, vp, dt, k.shape[1], kst, vst, _stream()), "gpsr_bank_write")
+    vp, _, vst = _strided(v, B, H, D, dev, "bank_write: v")
+    _lib.check(lib.gpsr_bank_write(ref, tp, B, J, sp, cp, kp, vp, code, k.shape[1], kst, vst, _stream()), "gpsr_bank_write")
 
 
 def bank_read(bank, table, start, count, rows, dtype=torch.float32):
     """-> k, v [B,rows,H,D]: the values that positions start[b] .. start[b] + count[b] - 1 hold, zeros behind them (gpsr_bank_read)."""
-    lib = _lib.load()
-    ref, (_, H, P, D) = _bank(bank)
-    tp, (sp, cp) = _bank_index(table, (start, count), "bank_read")
-    if dtype not in _BANK_TYPES:
+    lib, dev = _lib.load(), _bank_device(table)
+    ref, H, D = _bank(bank, dev)
+    tp, sp, cp = _bank_index(table, (start, count), dev, "bank_read")
+    code = _BANK_TYPES.get(dtype)
+    if code is None:
         raise _lib.GpsrError(f"bank_read: expected bfloat16, float16 or float32, got {dtype}")
-    B = table.shape[0]
+    B, J = table.shape
     k, v = (torch.empty((B, rows, H, D), dtype=dtype, device=table.device) for _ in range(2))
-    _lib.check(lib.gpsr_bank_read(ref, tp, B, table.shape[1], sp, cp, k.data_ptr(), v.data_ptr(), _BANK_TYPES[dtype], rows,
-                                  _stream()), "gpsr_bank_read")
+    _lib.check(lib.gpsr_bank_read(ref, tp, B, J, sp, cp, k.data_ptr(), v.data_ptr(), code, rows, _stream()), "gpsr_bank_read")
     return k, v
 
 
 def _bank_query(bank, table, length, q, skip, what):
-    ref, (_, H, P, D) = _bank(bank)
-    tp, (lp,) = _bank_index(table, (length,), what)
-    B = table.shape[0]
-    qp, dt, qst = _strided(q, (B, None, None, D), what + ": q")
+    """(the arguments up to q's strides, q's sizes, pointer of skip, the library, the device)."""
+    lib, dev = _lib.load(), _bank_device(table)
+    ref, H, D = _bank(bank, dev)
+    tp, lp = _bank_index(table, (length,), dev, what)
+    B, J = table.shape
+    qp, code, qst = _strided(q, B, None, D, dev, what + ": q")
     T, Hq = q.shape[1], q.shape[2]
     if Hq < 1 or Hq % H:
         raise _lib.GpsrError(f"{what}: {Hq} query heads are no multiple of the bank's {H}")
     if skip is not None and skip.shape != (B, T, 2):
         raise _lib.GpsrError(f"{what}: skip must be [{B},{T},2], got {tuple(skip.shape)}")
-    return ref, (tp, B, table.shape[1], lp, qp, dt, T, Hq, qst), _p(skip, torch.int32), (B, T, H, Hq, D)
+    sk = None if skip is None else _ptr(skip, torch.int32, dev)
+    return (ref, tp, B, J, lp, qp, code, T, Hq, qst), (ref, B, J, T, Hq), (B, T, H, Hq, D), code, sk, lib, dev
 
 
 def _bank_out(q, want_lse, B, T, Hq):
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device) if want_lse else None
-    return out, lse
+    return out, lse, None if lse is None else lse.data_ptr()
+
+
+def _bank_workspace(nbytes, q):
+    if not nbytes:
+        return None, None
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    return ws, ws.data_ptr()
 
 
 def bank_attend(bank, table, length, q, scale, skip=None, want_lse=False):
@@ -525,43 +554,39 @@ def bank_attend(bank, table, length, q, scale, skip=None, want_lse=False):
     exp(-scale |q - k|^2 / 2) (RBF) or exp(scale q.k) (LINEAR); with want_lse also the log of the sum of the weights
     [B,Hq,T] (RBF: without its factor exp(-scale |q|^2 / 2)).  skip [B,T,2] int32: positions lo <= r < hi that a query does
     not see; one that sees none gets zeros and -inf (gpsr_bank_attend)."""
-    lib = _lib.load()
-    ref, args, sk, (B, T, H, Hq, D) = _bank_query(bank, table, length, q, skip, "bank_attend")
-    out, lse = _bank_out(q, want_lse, B, T, Hq)
-    nbytes = lib.gpsr_bank_attend_workspace_bytes(ref, B, table.shape[1], T, Hq, args[5])
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    _lib.check(lib.gpsr_bank_attend(ref, *args, float(scale), sk, out.data_ptr(), _p(lse), _p(ws), nbytes, _stream()), "gpsr_bank_attend")
+    args, sizes, (B, T, H, Hq, D), code, sk, lib, dev = _bank_query(bank, table, length, q, skip, "bank_attend")
+    out, lse, lse_p = _bank_out(q, want_lse, B, T, Hq)
+    nbytes = lib.gpsr_bank_attend_workspace_bytes(*sizes, code)
+    ws, ws_p = _bank_workspace(nbytes, q)
+    _lib.check(lib.gpsr_bank_attend(*args, scale, sk, out.data_ptr(), lse_p, ws_p, nbytes, _stream()), "gpsr_bank_attend")
     return (out, lse) if want_lse else out
 
 
 def bank_select(bank, table, length, q, n_sel, skip=None):
     """-> int32 [B,T,H,n_sel]: the n_sel (1..64) pages of entry b (columns of its table row) whose centroids suit the query
     best, ascending, -1 behind the last; the heads that share a bank head choose together (gpsr_bank_select)."""
-    lib = _lib.load()
-    ref, args, sk, (B, T, H, Hq, D) = _bank_query(bank, table, length, q, skip, "bank_select")
-    n_sel = int(n_sel)
+    args, sizes, (B, T, H, Hq, D), code, sk, lib, dev = _bank_query(bank, table, length, q, skip, "bank_select")
     if not 1 <= n_sel <= 64:
         raise _lib.GpsrError(f"bank_select: n_sel must be in 1..64, got {n_sel}")
     sel = torch.empty((B, T, H, n_sel), dtype=torch.int32, device=q.device)
-    nbytes = lib.gpsr_bank_select_workspace_bytes(ref, B, table.shape[1], T, Hq, n_sel, args[5])
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    _lib.check(lib.gpsr_bank_select(ref, *args, n_sel, sk, sel.data_ptr(), _p(ws), nbytes, _stream()), "gpsr_bank_select")
+    nbytes = lib.gpsr_bank_select_workspace_bytes(*sizes, n_sel, code)
+    ws, ws_p = _bank_workspace(nbytes, q)
+    _lib.check(lib.gpsr_bank_select(*args, n_sel, sk, sel.data_ptr(), ws_p, nbytes, _stream()), "gpsr_bank_select")
     return sel
 
 
 def bank_attend_pages(bank, table, length, q, pages, scale, skip=None, want_lse=False):
     """bank_attend over the rows of each query's own pages [B,T,H,S] (S in 1..64; bank_select gives them) only.  Numbers outside the
     table and repeats are passed over (gpsr_bank_attend_pages)."""
-    lib = _lib.load()
-    ref, args, sk, (B, T, H, Hq, D) = _bank_query(bank, table, length, q, skip, "bank_attend_pages")
+    args, sizes, (B, T, H, Hq, D), code, sk, lib, dev = _bank_query(bank, table, length, q, skip, "bank_attend_pages")
     if pages.dim() != 4 or pages.shape[:3] != (B, T, H) or not 1 <= pages.shape[3] <= 64:
         raise _lib.GpsrError(f"bank_attend_pages: pages must be [{B},{T},{H},1..64], got {tuple(pages.shape)}")
-    out, lse = _bank_out(q, want_lse, B, T, Hq)
-    n_sel = pages.shape[3]
-    nbytes = lib.gpsr_bank_attend_pages_workspace_bytes(ref, B, table.shape[1], T, Hq, n_sel, args[5])
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    _lib.check(lib.gpsr_bank_attend_pages(ref, *args, _p(pages, torch.int32), n_sel, float(scale), sk, out.data_ptr(), _p(lse),
-                                          _p(ws), nbytes, _stream()), "gpsr_bank_attend_pages")
+    pp, n_sel = _ptr(pages, torch.int32, dev), pages.shape[3]
+    out, lse, lse_p = _bank_out(q, want_lse, B, T, Hq)
+    nbytes = lib.gpsr_bank_attend_pages_workspace_bytes(*sizes, n_sel, code)
+    ws, ws_p = _bank_workspace(nbytes, q)
+    _lib.check(lib.gpsr_bank_attend_pages(*args, pp, n_sel, scale, sk, out.data_ptr(), lse_p, ws_p, nbytes, _stream()),
+               "gpsr_bank_attend_pages")
     return (out, lse) if want_lse else out
 
 
