@@ -20,6 +20,9 @@ typedef unsigned u4v __attribute__((ext_vector_type(4)));
 
 struct Strides { int64_t b, t, h; };   // elements between entries, rows, heads
 
+// the wave's number, as the uniform value that it is: what follows from it needs no lanes and no masks
+__device__ __forceinline__ int wave_of(int tid) { return __builtin_amdgcn_readfirstlane(tid >> 6); }
+
 __device__ __forceinline__ float scale_of(unsigned byte) { return __uint_as_float(byte << 23); }
 
 // 8 columns of a row as held: w0 (and w1 for 8 bits) are the code words, s the scale

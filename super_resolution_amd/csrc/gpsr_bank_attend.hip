@@ -19,7 +19,7 @@ k_bank_attend(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, 
   constexpr int CW = (NW / WK) * 32, NQ = 1;                     // columns of the workgroup
   __shared__ __attribute__((aligned(16))) char sm[tile_lds(D, KT)];
   Tile<D, KT> tile(sm);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_of(tid), half = lane >> 5, col = lane & 31;
   const int h = blockIdx.y, b = blockIdx.z, H = bk.heads;
   const int split = blockIdx.x % splits;
   const int64_t C = (int64_t)T * G, c0 = (int64_t)(blockIdx.x / splits) * CW + (WK == 1 ? wave * 32 : 0);

@@ -21,7 +21,7 @@ k_bank_pages_query(gpsr_bank bk, const int32_t* __restrict__ table, int table_pa
   __shared__ __attribute__((aligned(16))) char sm[tile_lds(D, KT)];
   __shared__ int phys[64], rown[64], first[64], total;
   Tile<D, KT> tile(sm);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_of(tid), half = lane >> 5, col = lane & 31;
   const int h = blockIdx.y, b = blockIdx.z, H = bk.heads, P = 1 << pshift;
   const int split = blockIdx.x % splits, group = blockIdx.x / splits % groups;
   const int64_t t = blockIdx.x / splits / groups;
@@ -122,7 +122,8 @@ k_bank_pages_count(const int32_t* __restrict__ sel, int n_sel, const int32_t* __
     const int lp = s0[e];
     bool ok = (unsigned)lp < (unsigned)table_pages && ((int64_t)lp << pshift) < len;
     if (ok) ok = (uint64_t)(int64_t)table[(size_t)b * table_pages + lp] < (uint64_t)pages;
-    for (int k = 1; k <= s; ++k) ok = ok && s0[e - k] != lp;
+#pragma unroll 4
+    for (int k = 1; k <= s; ++k) ok &= s0[e - k] != lp;      // all of them, so that the loads do not wait for each other
     rank[b * per + e] = ok ? atomicAdd(&mine[h * table_pages + lp], 1) : -1;
     if (!ok)      // the join passes over partials whose sum of weights is 0
       for (int g = 0; g < G; ++g) part[(((((size_t)b * H + h) * T + th / H) * n_sel + s) * G + g) * D2 + D2 - 1] = 0.f;
@@ -139,12 +140,12 @@ k_bank_pages_shares(int* __restrict__ hist, int buckets, int chunks, int* __rest
   if (i >= buckets) return;
   int* p = hist + (size_t)b * chunks * buckets + i;
   int sum = 0;
-  for (int c0 = 0; c0 < chunks; c0 += 8) {
-    int n[8];
+  for (int c0 = 0; c0 < chunks; c0 += 32) {
+    int n[32];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) n[j] = c0 + j < chunks ? p[(size_t)(c0 + j) * buckets] : 0;
+    for (int j = 0; j < 32; ++j) n[j] = c0 + j < chunks ? p[(size_t)(c0 + j) * buckets] : 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < 32; ++j) {
       if (c0 + j < chunks) p[(size_t)(c0 + j) * buckets] = sum;
       sum += n[j];
     }
@@ -156,7 +157,7 @@ k_bank_pages_shares(int* __restrict__ hist, int buckets, int chunks, int* __rest
 __global__ void __launch_bounds__(1024)
 k_bank_pages_scan(const int* __restrict__ count, int buckets, int G, int cw, int* __restrict__ start, int* __restrict__ wgs) {
   __shared__ int sc[16], sw[16];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_of(tid);
   const int per = (buckets + 1023) / 1024;
   const int i0 = min(tid * per, buckets), i1 = min(i0 + per, buckets);
   int c = 0, w = 0;
@@ -201,7 +202,7 @@ k_bank_pages_page(gpsr_bank bk, const int32_t* __restrict__ table, int table_pag
   constexpr int NT = Terms<DT>::N, NB = KT / 32, CW = 128;
   __shared__ __attribute__((aligned(16))) char sm[tile_lds(D, KT)];
   Tile<D, KT> tile(sm);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_of(tid), half = lane >> 5, col = lane & 31;
   const int w = blockIdx.x;
   if (w >= wgs[buckets]) return;
   int a = 0, z = buckets;                 // the last bucket whose first workgroup is not behind this one

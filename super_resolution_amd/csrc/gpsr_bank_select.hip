@@ -3,23 +3,24 @@
 // The choice is defined by scores in 64 bits, but for many queries nearly all pages can be told apart with fewer:
 //   prepare: each page's centroid as two bf16 terms (16 bits), its offset, and for 32 pages at a time bounds on the norms
 //   screen:  scores a = q.c + offset on the matrix units, off by at most eps (below).  First pass: the pages are dealt to 128
-//            groups and each group keeps its largest a - eps; the n_sel-th largest of those, tau, is a lower bound on the
+//            groups (64 for n_sel <= 16) and each group keeps its largest a - eps; the n_sel-th largest of those, tau, is a lower bound on the
 //            n_sel-th best exact score.  Second pass, the same products again: every page with a + eps >= tau is a candidate.
-//   pick:    exact scores of the candidates (or of all pages: few queries, few pages, or more candidates than fit), sorted
-//            across a wave by (score, page).
+//   pick:    where the screened scores of the n_sel-th and the next candidate differ by more than 2 eps, the choice is known;
+//            otherwise exact scores of the candidates (or of all pages: few queries, few pages, or more candidates than
+//            fit), sorted across a wave by (score, page).
 // With Cauchy-Schwarz, and u = 2^-8 the half step of bf16: two terms of q and of c and their three larger products leave out
-// at most 3 u^2 |q||c|; the 32-bit sum of 3 dim products and the offset o adds (3 dim + 2) 2^-23 (|q||c| + |o|); 1e-35 (1 +
-// |q| + |c|) covers subnormal terms.  Norms above 1e18 or not finite are not screened: their pages are all candidates.
+// at most 3 u^2 |q||c| (one exact term of q: u^2 |q||c|); the 32-bit sum of n products and the offset o adds (n + 2) 2^-23
+// (|q||c| + |o|), n = 3 dim (2 dim); 1e-35 (1 + |q| + |c|) covers subnormal terms.  Norms above 1e18 or not finite are not screened: their pages are all candidates.
 #include "gpsr_bank_tile.hpp"
 
 #define SE_MAX 64
-#define SE_SLOTS 64
 
-struct SelectPlan { bool screen; int waves, J, blocks, cap; size_t hl, off, bound, count, cand, bytes; };
+struct SelectPlan { bool screen; int waves, J, blocks, slots; size_t off, bound, count, cand, bytes; };
 
 // ---------------------------------------------------------------- prepare
-// Row r of block k is page r * blocks + k: neighbouring pages, often alike, fall into different groups.  A workgroup has one
-// block, 8 threads a page.
+// Row r of block k is page r * blocks + k: neighbouring pages, often alike, fall into different groups.  The terms lie as the
+// matrix instructions take them, [16 columns][high, low][lane][8], so that a wave's load is one contiguous kilobyte (as rows,
+// each load touched 32 cache lines: 132 against 50 us).  A workgroup has one block, 8 threads a page.
 template <int D>
 __global__ void __launch_bounds__(256)
 k_bank_select_prepare(gpsr_bank bk, const int32_t* __restrict__ table, int J, int pshift, const int32_t* __restrict__ length, int G,
@@ -30,7 +31,7 @@ k_bank_select_prepare(gpsr_bank bk, const int32_t* __restrict__ table, int J, in
   int64_t page = -1;
   if (lp < J && (lp << pshift) < length[b]) page = table[(size_t)b * J + lp];
   const bool there = page >= 0 && page < bk.pages;
-  __bf16* row = hl + (((size_t)(b * H + h) * blocks + k) * 32 + r) * (2 * D);
+  __bf16* to = hl + ((size_t)(b * H + h) * blocks + k) * 32 * (2 * D) + r * 8;
   double sq = 0.0;
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) {    // 4 columns at a time
@@ -44,8 +45,9 @@ k_bank_select_prepare(gpsr_bank bk, const int32_t* __restrict__ table, int J, in
       hi[j / 2][j % 2] = t; lo[j / 2][j % 2] = (__bf16)(y[j] - (float)t);
       sq = fma((double)y[j], (double)y[j], sq);
     }
-    *(u2v*)(row + c) = u2v{__builtin_bit_cast(unsigned, hi[0]), __builtin_bit_cast(unsigned, hi[1])};
-    *(u2v*)(row + D + c) = u2v{__builtin_bit_cast(unsigned, lo[0]), __builtin_bit_cast(unsigned, lo[1])};
+    const int at = (c / 16) * 1024 + (c / 8 % 2) * 256 + c % 8;
+    *(u2v*)(to + at) = u2v{__builtin_bit_cast(unsigned, hi[0]), __builtin_bit_cast(unsigned, hi[1])};
+    *(u2v*)(to + at + 512) = u2v{__builtin_bit_cast(unsigned, lo[0]), __builtin_bit_cast(unsigned, lo[1])};
   }
   sq += __shfl_xor(sq, 1); sq += __shfl_xor(sq, 2); sq += __shfl_xor(sq, 4);
   const float o = bk.kernel_id == GPSR_KERNEL_RBF ? (float)(-0.5 * G * sq) : 0.f;
@@ -65,166 +67,241 @@ k_bank_select_prepare(gpsr_bank bk, const int32_t* __restrict__ table, int J, in
 __device__ __forceinline__ int ordered(float x) { const int i = __float_as_int(x); return i ^ ((i >> 31) & 0x7fffffff); }
 __device__ __forceinline__ float unordered(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7fffffff)); }
 
-// the pages that a query skips altogether: [skipped.x, skipped.y)
-__device__ __forceinline__ void skipped_pages(const int32_t* __restrict__ skip, int64_t at, int64_t len, int pshift, int64_t& lo, int64_t& hi) {
-  lo = hi = 0;
-  if (!skip) return;
-  const int64_t P = (int64_t)1 << pshift, a = skip[2 * at] > 0 ? skip[2 * at] : 0, z = skip[2 * at + 1];
-  if (z <= a) return;
-  lo = (a + P - 1) >> pshift;
-  hi = z >= len ? (int64_t)1 << 40 : z >> pshift;   // the last page ends with the bank
+// minimum over the wave, by moves between neighbouring lanes, rows of 16 and halves
+__device__ __forceinline__ float wave_min(float x) {
+#define STEP(ctrl) x = fminf(x, __int_as_float(__builtin_amdgcn_update_dpp(0x7f800000, __float_as_int(x), ctrl, 0xf, 0xf, false)))
+  STEP(0x111); STEP(0x112); STEP(0x114); STEP(0x118);   // row_shr 1, 2, 4, 8
+  STEP(0x142); STEP(0x143);                             // row_bcast 15, 31
+#undef STEP
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
 }
 
-// NT: bf16 terms of the queries (1: bf16 rows taken singly, exact; 2: everything else)
-template <int DT, int D, int NT>
-__global__ void __launch_bounds__(256)
+// the pages that a query skips altogether: [skipped.x, skipped.y)
+__device__ __forceinline__ void skipped_pages(const int32_t* __restrict__ skip, int64_t at, int len, int pshift, int& lo, int& hi) {
+  lo = hi = 0;
+  if (!skip) return;
+  const int a = max(skip[2 * at], 0), z = skip[2 * at + 1];
+  if (z <= a) return;
+  lo = (int)(((int64_t)a + (1 << pshift) - 1) >> pshift);
+  hi = z >= len ? 0x7fffffff : z >> pshift;   // the last page ends with the bank
+}
+
+// A workgroup has 64 queries (32 of many columns) in blocks of 32, which every wave holds; its waves share out the blocks of
+// pages and read them straight from L2 into operand registers, one block ahead, with no barrier between.
+// NT: bf16 terms of the queries (1: bf16 rows taken singly, exact; 2: everything else).  SLOTS: groups of one lane in each wave
+// (a column has 8 times as many); 8 halve the LDS where n_sel leaves them fine enough.
+struct Candidate { int page; float a; };
+// candidates that are kept for a query
+static constexpr int screen_cap(int slots) { return slots * 8; }
+// blocks of columns: as many as the queries' operands leave registers for
+static constexpr int screen_nq(int d, int nt) { return nt * d <= 256 ? 2 : 1; }
+template <int DT, int D, int NT, int SLOTS>
+__global__ void __launch_bounds__(256, D * NT <= 64 ? 3 : D * NT <= 128 ? 2 : 1)
 k_bank_select_screen(int H, const int32_t* __restrict__ length, int pshift, const typename Row<DT>::T* __restrict__ q, int T, int G,
                      Strides qs, bool qwide, int n_sel, const int32_t* __restrict__ skip, int J, int blocks,
-                     const __bf16* __restrict__ hl, const float* __restrict__ off, const f2v* __restrict__ bound, int cap,
-                     int* __restrict__ count, int* __restrict__ cand) {
-  constexpr int KS = 2 * D + 8;
-  __shared__ __attribute__((aligned(16))) __bf16 tile[32 * KS];
-  __shared__ __attribute__((aligned(16))) float toff[32];
-  __shared__ float best[SE_SLOTS][256];    // [slot][thread]: each lane's own groups
-  __shared__ int found[128];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+                     const __bf16* __restrict__ hl, const float* __restrict__ off, const f2v* __restrict__ bound, int* __restrict__ count,
+                     int32_t* __restrict__ cand, int32_t* __restrict__ sel) {
+  constexpr int NQ = screen_nq(D, NT), CAP = screen_cap(SLOTS);
+  __shared__ float best[4][SLOTS][NQ][64];    // each lane's own groups
+  __shared__ float thr_of[NQ][32], eps_of[4][NQ][32];
+  __shared__ Candidate list[32 * NQ][CAP];    // in LDS: a store to memory among the loads ahead would be waited for with them
+  __shared__ int found[32 * NQ];
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_of(tid), half = lane >> 5, col = lane & 31;
   const int h = blockIdx.y, b = blockIdx.z;
-  const int64_t t = (int64_t)blockIdx.x * 128 + wave * 32 + col;
-  const bool there = t < T;
-  if (tid < 128) found[tid] = 0;
-  for (int s = 0; s < SE_SLOTS; ++s) best[s][tid] = -__builtin_inff();
+  const int64_t t0 = (int64_t)blockIdx.x * (32 * NQ);
+#pragma unroll
+  for (int s = 0; s < SLOTS; ++s)
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) best[wave][s][n][lane] = -__builtin_inff();
 
-  // the group's heads, summed in 64 bits and rounded once
-  bf8 qf[NT][D / 16];
-  float qn = 0.f;
+  // the heads that share the bank head, summed in 64 bits and rounded once
+  bf8 qf[NQ][NT][D / 16];
+  float qn[NQ], eps_most[NQ];
+  int slo[NQ], shi[NQ];
+  bool skips = false;
 #pragma unroll
-  for (int s = 0; s < D / 16; ++s) {
-    float y[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (there) {
-      const typename Row<DT>::T* p = q + b * qs.b + t * qs.t + (int64_t)(h * G) * qs.h + s * 16 + half * 8;
-      load8<DT>(p, qwide, y);
-      if (G > 1) {
-        double sum[8];
+  for (int n = 0; n < NQ; ++n) {
+    const int64_t t = t0 + n * 32 + col;
+    const bool there = t < T;
+    qn[n] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum[i] = y[i];
-        for (int g = 1; g < G; ++g) {
-          float z[8];
-          load8<DT>(p + g * qs.h, qwide, z);
+    for (int s = 0; s < D / 16; ++s) {
+      float y[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (there) {
+        const typename Row<DT>::T* p = q + b * qs.b + t * qs.t + (int64_t)(h * G) * qs.h + s * 16 + half * 8;
+        load8<DT>(p, qwide, y);
+        if (G > 1) {
+          double sum[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) sum[i] += (double)z[i];
+          for (int i = 0; i < 8; ++i) sum[i] = y[i];
+          for (int g = 1; g < G; ++g) {
+            float z[8];
+            load8<DT>(p + g * qs.h, qwide, z);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[i] += (double)z[i];
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] = (float)sum[i];
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = (float)sum[i];
       }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) qn[n] = fmaf(y[i], y[i], qn[n]);
+      bf8 x[NT];
+      split_terms<NT>(y, x);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) qf[n][i][s] = x[i];
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) qn = fmaf(y[i], y[i], qn);
-    bf8 x[NT];
-    split_terms<NT>(y, x);
-#pragma unroll
-    for (int n = 0; n < NT; ++n) qf[n][s] = x[n];
+    qn[n] += __shfl_xor(qn[n], 32);
+    qn[n] = qn[n] < 1e36f ? 1.01f * sqrtf(qn[n]) : __builtin_inff();
+    eps_most[n] = 0.f;
+    skipped_pages(there ? skip : nullptr, (int64_t)b * T + t, length[b], pshift, slo[n], shi[n]);
+    skips |= slo[n] < shi[n];
   }
-  qn += __shfl_xor(qn, 32);
-  qn = qn < 1e36f ? 1.01f * sqrtf(qn) : __builtin_inff();
-  int64_t slo, shi;
-  skipped_pages(there ? skip : nullptr, (int64_t)b * T + t, length[b], pshift, slo, shi);
-  const bool skips = __ballot(slo < shi) != 0;
+  skips = __ballot(skips) != 0;
 
   const size_t base = (size_t)(b * H + h) * blocks;
-  const float k1 = 3.1f / 65536.f + (3 * D + 2) / 8388608.f, k2 = (3 * D + 3) / 8388608.f;
-  float thr = 0.f;
-  u4v next[D / 32];     // a block is 32 rows of 2 D bf16: D / 32 loads of 16 bytes for each thread
-  float noff = 0.f;
-  const auto load = [&](int k) {
-    const u4v* src = (const u4v*)(hl + (base + k) * 32 * (2 * D));
+  constexpr int ADDS = (NT + 1) * D + 2;
+  const float k1 = (NT == 1 ? 1.05f : 3.1f) / 65536.f + ADDS / 8388608.f, k2 = (ADDS + 1) / 8388608.f;
+  float thr[NQ];
+  if (tid < 32 * NQ) found[tid] = 0;      // before the barriers between the passes
+  bf8 hi[D / 16], lo[D / 16];
+  f4v o4[4];
+  const auto load = [&](int k) {       // behind the last block the last one again
+    const __bf16* from = hl + (base + min(k, blocks - 1)) * 32 * (2 * D) + lane * 8;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) next[i] = src[tid + 256 * i];
-    if (tid < 32) noff = off[(base + k) * 32 + tid];
+    for (int d = 0; d < D / 16; ++d) { hi[d] = *(const bf8*)(from + d * 1024); lo[d] = *(const bf8*)(from + d * 1024 + 512); }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o4[i] = *(const f4v*)(off + (base + min(k, blocks - 1)) * 32 + 8 * i + 4 * half);
   };
   for (int pass = 0; pass < 2; ++pass) {
-    load(0);
-    for (int k = 0; k < blocks; ++k) {
+    load(wave);
+    for (int k = wave; k < blocks; k += 4) {
       const f2v nb = bound[base + k];
-      __syncthreads();
+      f16v s[NQ], o;
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        const int u = tid + 256 * i;
-        *(u4v*)(tile + u / (D / 4) * KS + u % (D / 4) * 8) = next[i];
-      }
-      if (tid < 32) toff[tid] = noff;
-      __syncthreads();
-      if (k + 1 < blocks) load(k + 1);
-      f16v s;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f4v a = *(const f4v*)(toff + 8 * i + 4 * half);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[4 * i + j] = a[j];
-      }
-      const __bf16* row = tile + col * KS + half * 8;
+      for (int i = 0; i < 16; ++i) o[i] = o4[i / 4][i % 4];
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) {
-        const bf8 hi = *(const bf8*)(row + d * 16), lo = *(const bf8*)(row + D + d * 16);
-        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi, qf[0][d], s, 0, 0, 0);
-        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lo, qf[0][d], s, 0, 0, 0);
-        if constexpr (NT > 1) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi, qf[1][d], s, 0, 0, 0);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi[d], qf[n][0][d], d ? s[n] : o, 0, 0, 0);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lo[d], qf[n][0][d], s[n], 0, 0, 0);
+        if constexpr (NT > 1)
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi[d], qf[n][1][d], s[n], 0, 0, 0);
       }
-      const float eps = qn * nb.x * k1 + nb.y * k2 + 1e-35f * (1.f + qn + nb.x);
-      const bool blind = !(eps < 1e37f);      // not screened: of no use as a bound, candidates all
+      load(k + 4);
       if (skips) {
+        asm volatile("");
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int64_t lp = (int64_t)(8 * (e >> 2) + 4 * half + (e & 3)) * blocks + k;
-          if (lp >= slo && lp < shi) s[e] = -__builtin_inff();
-        }
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int lp = (8 * (e >> 2) + 4 * half + (e & 3)) * blocks + k;
+            if (lp >= slo[n] && lp < shi[n]) s[n][e] = -__builtin_inff();
+          }
       }
-      float mx = s[0];
 #pragma unroll
-      for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
-      if (pass == 0) {
-        if (!blind) { float* p = &best[k % SE_SLOTS][tid]; *p = fmaxf(*p, mx - eps); }
-      } else if (there && (blind || mx >= thr - eps)) {
-        int* mine = cand + (((size_t)(b * H + h) * T) + t) * cap;
+      for (int n = 0; n < NQ; ++n) {
+        const float eps = qn[n] * nb.x * k1 + nb.y * k2 + 1e-35f * (1.f + qn[n] + nb.x);
+        const bool blind = !(eps < 1e37f);      // not screened: of no use as a bound, candidates all
+        if (pass == 0) {
+          float mx = s[n][0];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int64_t lp = (int64_t)(8 * (e >> 2) + 4 * half + (e & 3)) * blocks + k;
-          if (lp < J && (blind || (s[e] > -__builtin_inff() && s[e] >= thr - eps))) {
-            const int at = atomicAdd(&found[wave * 32 + col], 1);
-            if (at < cap) mine[at] = (int)lp;
+          for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[n][e]);
+          float* p = &best[wave][(k >> 2) % SLOTS][n][lane];
+          if (!blind) *p = fmaxf(*p, mx - eps);
+          eps_most[n] = blind ? __builtin_inff() : fmaxf(eps_most[n], eps);
+        } else {
+          // which of the lane's 16 pages, then one of them for each lane at a time
+          const float least = fmaxf(thr[n] - eps, -3.4e38f);
+          unsigned hits = 0;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) hits |= blind || s[n][e] >= least ? 1u << e : 0u;
+          if (t0 + n * 32 + col >= T) hits = 0;
+          while (__ballot(hits != 0)) {
+            const int e = __builtin_ctz(hits | 0x10000u);
+            const int lp = (8 * (e >> 2) + 4 * half + (e & 3)) * blocks + k;
+            float a = 0.f;
+#pragma unroll
+            for (int x = 0; x < 16; ++x) a = x == e ? s[n][x] : a;
+            if (hits && lp < J) {
+              const int at = atomicAdd(&found[n * 32 + col], 1);
+              if (at < CAP) list[n * 32 + col][at] = {lp, a};
+            }
+            hits &= hits - 1;
           }
         }
       }
     }
     if (pass == 0) {
-      // tau by bisection over the lane's groups and those of its other half; a value a little below will do
-      float v[SE_SLOTS], top = -__builtin_inff(), low = __builtin_inff();
-      int n = 0;
 #pragma unroll
-      for (int s = 0; s < SE_SLOTS; ++s) {
-        v[s] = best[s][tid];
-        top = fmaxf(top, v[s]);
-        if (v[s] > -__builtin_inff()) { low = fminf(low, v[s]); ++n; }
+      for (int n = 0; n < NQ; ++n) if (half == 0) eps_of[wave][n][col] = eps_most[n];
+      __syncthreads();
+      // Wave w finds tau for block w of the columns, by bisection over the column's groups; a value a little below will do
+      if (wave < NQ) {
+      float v[4 * SLOTS], top = -__builtin_inff(), low = __builtin_inff(), tau = -__builtin_inff();
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < 4 * SLOTS; ++i) {
+        v[i] = best[i / SLOTS][i % SLOTS][wave][lane];
+        top = fmaxf(top, v[i]);
+        if (v[i] > -__builtin_inff()) { low = fminf(low, v[i]); ++c; }
       }
-      n += __shfl_xor(n, 32);
+      c += __shfl_xor(c, 32);
       top = fmaxf(top, other_half(top)); low = fminf(low, other_half(low));
-      thr = -__builtin_inff();
-      if (n >= n_sel) {
-        int64_t a = ordered(low), z = (int64_t)ordered(top) + 1;      // at least n_sel groups are >= a, fewer >= z
-        for (int i = 0; i < 20 && z - a > 1; ++i) {
-          const int mid = (int)((a + z) >> 1);
-          const float x = unordered(mid);
-          int c = 0;
+      int64_t a = ordered(low), z = (int64_t)ordered(top) + 1;      // at least n_sel groups are >= a, fewer >= z
+      const bool enough = c >= n_sel;
+      for (int i = 0; i < 20; ++i) {
+        const int mid = (int)((a + z) >> 1);
+        const float x = unordered(mid);
+        c = 0;
 #pragma unroll
-          for (int s = 0; s < SE_SLOTS; ++s) c += v[s] >= x;
-          c += __shfl_xor(c, 32);
-          if (c >= n_sel) a = mid; else z = mid;
-        }
-        thr = unordered((int)a);
+        for (int s = 0; s < 4 * SLOTS; ++s) c += v[s] >= x;
+        c += __shfl_xor(c, 32);
+        if (c >= n_sel) a = mid; else z = mid;
       }
+      if (enough) tau = unordered((int)a);
+      if (half == 0) {
+        thr_of[wave][col] = tau;
+      }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) thr[n] = thr_of[n][col];
     }
   }
   __syncthreads();
-  if (there && half == 0) count[((size_t)(b * H + h) * T) + t] = found[wave * 32 + col];
+  // Where the n_sel-th and the next best screened score are further apart than both can be off, the choice is made; count says
+  // -2 for such a query, -1 for one with more candidates than were kept, and how many there are otherwise.
+  for (int x = wave; x < 32 * NQ && t0 + x < T; x += 4) {
+    const int64_t bth = ((int64_t)b * H + h) * T + t0 + x;
+    const int n = __builtin_amdgcn_readfirstlane(found[x]), none = 0x7fffffff;
+    const float eps = fmaxf(fmaxf(eps_of[0][x / 32][x % 32], eps_of[1][x / 32][x % 32]), fmaxf(eps_of[2][x / 32][x % 32], eps_of[3][x / 32][x % 32]));
+    if (n <= 64 && eps < 1e37f) {
+      const Candidate c = lane < n ? list[x][lane] : Candidate{none, -__builtin_inff()};
+      // the few that are too many go one after the other, the smallest first
+      unsigned long long chosen = n < 64 ? (1ull << n) - 1 : ~0ull;
+      float most = -__builtin_inff();
+      while (__popcll(chosen) > n_sel) {
+        const bool in = chosen >> lane & 1;
+        most = wave_min(in ? c.a : __builtin_inff());
+        chosen &= ~__ballot(in && c.a == most);
+      }
+      const bool in = chosen >> lane & 1;
+      if (n <= n_sel || (__popcll(chosen) == n_sel && wave_min(in ? c.a : __builtin_inff()) - most > 2.01f * eps)) {
+        int32_t* const to = sel + (((size_t)b * T + t0 + x) * H + h) * n_sel;
+        int place = 0;
+        for (unsigned long long left = chosen; left; left &= left - 1) place += __builtin_amdgcn_readlane(c.page, __builtin_ctzll(left)) < c.page;
+        if (in) to[place] = c.page;
+        if (lane >= __popcll(chosen) && lane < n_sel) to[lane] = -1;
+        if (lane == 0) count[bth] = -2;
+        continue;
+      }
+    }
+    if (lane == 0) count[bth] = n <= CAP ? n : -1;
+    for (int i = lane; i < min(n, CAP); i += 64) cand[(size_t)bth * CAP + i] = list[x][i].page;
+  }
 }
 
 // ---------------------------------------------------------------- pick
@@ -233,9 +310,11 @@ __device__ __forceinline__ bool before(const Scored& a, const Scored& b) { retur
 __device__ __forceinline__ Scored from_lane(const Scored& a, int x) { return {__shfl_xor(a.s, x), __shfl_xor(a.at, x)}; }
 
 // lanes in the order of before(), or the other way round
+// (N = 32: the first 32 lanes, where the others have none)
+template <int N = 64>
 __device__ __forceinline__ void sort64(Scored& a, int lane, bool best_first) {
 #pragma unroll
-  for (int k = 2; k <= 64; k <<= 1)
+  for (int k = 2; k <= N; k <<= 1)
 #pragma unroll
     for (int j = k >> 1; j; j >>= 1) {
       const Scored o = from_lane(a, j);
@@ -258,64 +337,87 @@ template <int DT, int W>
 __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W)
 k_bank_select_pick(gpsr_bank bk, const int32_t* __restrict__ table, int J, int pshift, const int32_t* __restrict__ length,
                    const typename Row<DT>::T* __restrict__ q, int T, int G, Strides qs, int n_sel, const int32_t* __restrict__ skip,
-                   int cap, const int* __restrict__ count, const int* __restrict__ cand, int32_t* __restrict__ sel) {
+                   int cap, const int* __restrict__ count, const int32_t* __restrict__ cand, int32_t* __restrict__ sel) {
   constexpr int Q = W == 1 ? 4 : 1;
   __shared__ double qv[Q][256];
   __shared__ double ms[W == 1 ? 1 : W][64];
   __shared__ int ma[W == 1 ? 1 : W][64];
-  const int D = bk.dim, H = bk.heads, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int D = bk.dim, H = bk.heads, tid = threadIdx.x, lane = tid & 63, wave = wave_of(tid);
   const int slot = W == 1 ? wave : 0, h = blockIdx.y, b = blockIdx.z;
   const int64_t t = (int64_t)blockIdx.x * Q + slot;
-  const bool there = t < T;
-  if (there)
-    for (int i = W == 1 ? lane : tid; i < D; i += W == 1 ? 64 : 64 * W) {
-      double s = 0.0;
-      for (int g = 0; g < G; ++g) s += (double)to_f32<DT>(q[b * qs.b + t * qs.t + (int64_t)(h * G + g) * qs.h + i]);
-      qv[slot][i] = s;
-    }
-  __syncthreads();
-  if (!there) return;              // W == 1: a whole wave, and no barrier follows
+  if (t >= T) return;              // W == 1: a whole wave, and no barrier follows; W > 1: never
   const int none = 0x7fffffff;
   const double worst = -__builtin_inf();
   const int64_t len = length[b], bth = ((int64_t)b * H + h) * T + t;
   const int64_t pages = len <= 0 ? 0 : (len + (1 << pshift) - 1) >> pshift;
   const int n_all = (int)(pages < J ? pages : J);
+  int32_t* const to = sel + (((size_t)b * T + t) * H + h) * n_sel;
   int n = n_all;
-  const int* mine = nullptr;
-  if (count && count[bth] <= cap) { n = count[bth]; mine = cand + (size_t)bth * cap; }
-  int64_t slo, shi;
-  skipped_pages(skip, (int64_t)b * T + t, len, pshift, slo, shi);
+  const int32_t* mine = nullptr;
+  if (W == 1 && count) {
+    const int c = count[bth];
+    if (c == -2) return;
+    if (c >= 0) { n = c; mine = cand + (size_t)bth * cap; }
+  }
+  for (int i = W == 1 ? lane : tid; i < D; i += W == 1 ? 64 : 64 * W) {
+    double s = 0.0;
+    for (int g = 0; g < G; ++g) s += (double)to_f32<DT>(q[b * qs.b + t * qs.t + (int64_t)(h * G + g) * qs.h + i]);
+    qv[slot][i] = s;
+  }
+  if (W > 1) __syncthreads();
+  int slo, shi;
+  skipped_pages(skip, (int64_t)b * T + t, length[b], pshift, slo, shi);
   const bool rbf = bk.kernel_id == GPSR_KERNEL_RBF;
   Scored best = {worst, none};
   bool empty = true;
+  const int part = lane & 3;
   for (int64_t i0 = (int64_t)(W == 1 ? 0 : wave) * 64; i0 < n; i0 += W == 1 ? 64 : 64 * W) {
     Scored x = {worst, none};
-    const int64_t i = i0 + lane;
-    if (i < n) {
-      const int lp = mine ? mine[i] : (int)i;
-      const int64_t page = lp < n_all ? table[(size_t)b * J + lp] : -1;
-      if (page >= 0 && page < bk.pages && !(lp >= slo && lp < shi)) {
-        const f4v* c = (const f4v*)(bk.centroid + ((size_t)page * H + h) * D);
-        // 32 columns on their way at a time, four chains of sums
-        double dot[4] = {0, 0, 0, 0}, sq[4] = {0, 0, 0, 0};
-        for (int g = 0; g < D / 32; ++g) {
-          f4v y[8];
+    // four lanes a page, 16 pages at a time; page i0 + i ends up in lane i
+    int lp[4];
+    const f4v* c[4];
+    bool ok[4];
+    const auto look_up = [&](int sub) {
+      const int64_t i = i0 + sub * 16 + (lane >> 2);
+      lp[sub] = i < n ? mine ? mine[i] : (int)i : none;
+      const int64_t page = lp[sub] < n_all ? table[(size_t)b * J + lp[sub]] : -1;
+      ok[sub] = page >= 0 && page < bk.pages && !(lp[sub] >= slo && lp[sub] < shi);
+      c[sub] = (const f4v*)(bk.centroid + ((size_t)(ok[sub] ? page : 0) * H + h) * D);
+    };
+    const auto score = [&](int sub) {
+      double dot[4] = {0, 0, 0, 0}, sq[4] = {0, 0, 0, 0};
+      for (int g = 0; g < D / 32; ++g) {
+        f4v y[2];
 #pragma unroll
-          for (int d = 0; d < 8; ++d) y[d] = c[8 * g + d];
+        for (int d = 0; d < 2; ++d) y[d] = c[sub][8 * g + 4 * d + part];
 #pragma unroll
-          for (int d = 0; d < 8; ++d)
+        for (int d = 0; d < 2; ++d)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const double z = (double)y[d][j];
-              dot[j] = fma(qv[slot][32 * g + 4 * d + j], z, dot[j]);
-              if (rbf) sq[j] = fma(z, z, sq[j]);
-            }
-        }
-        const double all = (dot[0] + dot[1]) + (dot[2] + dot[3]);
-        const double s = rbf ? all - 0.5 * G * ((sq[0] + sq[1]) + (sq[2] + sq[3])) : all;
-        if (s == s) x = {s, lp};
+          for (int j = 0; j < 4; ++j) {
+            const double z = (double)y[d][j];
+            dot[j] = fma(qv[slot][32 * g + 16 * d + 4 * part + j], z, dot[j]);
+            if (rbf) sq[j] = fma(z, z, sq[j]);
+          }
       }
+      double s = (dot[0] + dot[1]) + (dot[2] + dot[3]);
+      if (rbf) s -= 0.5 * G * ((sq[0] + sq[1]) + (sq[2] + sq[3]));
+      s += __shfl_xor(s, 1); s += __shfl_xor(s, 2);
+      Scored y = {worst, none};
+      if (ok[sub] && s == s) y = {s, lp[sub]};
+      y.s = __shfl(y.s, (lane & 15) * 4); y.at = __shfl(y.at, (lane & 15) * 4);
+      if ((lane >> 4) == sub) x = y;
+    };
+    if constexpr (W > 1) {         // few waves on the chip: the look-ups of all 64 pages wait together
+#pragma unroll
+      for (int sub = 0; sub < 4; ++sub) look_up(sub);
+#pragma unroll
+      for (int sub = 0; sub < 4; ++sub) score(sub);
+    } else {                       // some 20 candidates: no work for pages that are not there
+#pragma unroll
+      for (int sub = 0; sub < 4; ++sub)
+        if (i0 + sub * 16 < n) { look_up(sub); score(sub); }
     }
+    if (empty && n <= 32) { sort64<32>(x, lane, true); best = x; break; }
     if (empty) { sort64(x, lane, true); best = x; empty = false; continue; }
     const Scored last = {__shfl(best.s, n_sel - 1), __shfl(best.at, n_sel - 1)};
     if (!__ballot(before(x, last))) continue;
@@ -336,7 +438,7 @@ k_bank_select_pick(gpsr_bank bk, const int32_t* __restrict__ table, int J, int p
   if (lane >= n_sel) best.at = none;
   int rank = 0;
   for (int i = 0; i < n_sel; ++i) { const int o = __shfl(best.at, i); rank += o < best.at || (o == best.at && i < lane); }
-  if (lane < n_sel) sel[(((size_t)b * T + t) * H + h) * n_sel + rank] = best.at == none ? -1 : best.at;
+  if (lane < n_sel) to[rank] = best.at == none ? -1 : best.at;
 }
 
 // ---------------------------------------------------------------- host
@@ -348,13 +450,13 @@ static SelectPlan plan_of(const gpsr_bank* bk, int B, int table_pages, int T, in
   p.waves = !p.screen && table_pages > 64 ? 16 : 1;
   if (p.screen) {
     p.blocks = (table_pages + 31) / 32;
-    p.cap = 2 * n_sel + 64;
+    p.slots = n_sel <= 16 ? 8 : 16;
     const size_t rows = (size_t)B * bk->heads * p.blocks * 32;
     size_t at = align256(rows * 2 * bk->dim * 2);
     p.off = at; at += align256(rows * 4);
     p.bound = at; at += align256(rows / 32 * 8);
     p.count = at; at += align256((size_t)queries * 4);
-    p.cand = at; at += align256((size_t)queries * p.cap * 4);
+    p.cand = at; at += align256((size_t)queries * screen_cap(p.slots) * 4);
     p.bytes = at;
   }
   return p;
@@ -370,22 +472,24 @@ static void launch_select(const SelectPlan& p, const gpsr_bank& bk, const int32_
                           int T, int G, Strides qs, bool qwide, int n_sel, const int32_t* skip, int32_t* sel, char* ws, hipStream_t st) {
   typedef typename Row<DT>::T E;
   const int pshift = __builtin_ctz((unsigned)bk.page_rows), H = bk.heads;
-  const int *count = nullptr, *cand = nullptr;
+  int *count = nullptr, *cand = nullptr;
   if (p.screen) {
     __bf16* hl = (__bf16*)ws;
     float* off = (float*)(ws + p.off);
     f2v* bound = (f2v*)(ws + p.bound);
-    count = (const int*)(ws + p.count); cand = (const int*)(ws + p.cand);
+    count = (int*)(ws + p.count); cand = (int*)(ws + p.cand);
     hipLaunchKernelGGL((k_bank_select_prepare<D>), dim3((unsigned)p.blocks, (unsigned)H, (unsigned)B), dim3(256), 0, st, bk, table, p.J,
                        pshift, length, G, p.blocks, hl, off, bound);
-    const dim3 grid((unsigned)(((int64_t)T + 127) / 128), (unsigned)H, (unsigned)B);
-#define SCREEN(NT) hipLaunchKernelGGL((k_bank_select_screen<DT, D, NT>), grid, dim3(256), 0, st, H, length, pshift, (const E*)q, T, G, qs, \
-    qwide, n_sel, skip, p.J, p.blocks, hl, off, bound, p.cap, (int*)count, (int*)cand)
-    if constexpr (DT == GPSR_BF16) { if (G == 1) SCREEN(1); else SCREEN(2); } else SCREEN(2);
+#define SCREEN(NT) if (p.slots == 8) SCREEN_(NT, 8); else SCREEN_(NT, 16)
+#define SCREEN_(NT, SLOTS) hipLaunchKernelGGL((k_bank_select_screen<DT, D, NT, SLOTS>), \
+    dim3((unsigned)(((int64_t)T + 32 * screen_nq(D, NT) - 1) / (32 * screen_nq(D, NT))), (unsigned)H, (unsigned)B), dim3(256), 0, st, H, length, pshift, (const E*)q, T, G, qs, \
+    qwide, n_sel, skip, p.J, p.blocks, hl, off, bound, count, cand, sel)
+    if constexpr (DT == GPSR_BF16) { if (G == 1) { SCREEN(1); } else { SCREEN(2); } } else { SCREEN(2); }
 #undef SCREEN
+#undef SCREEN_
   }
 #define PICK(W, Q) hipLaunchKernelGGL((k_bank_select_pick<DT, W>), dim3((unsigned)(((int64_t)T + Q - 1) / Q), (unsigned)H, (unsigned)B), \
-    dim3(W == 1 ? 256 : 64 * W), 0, st, bk, table, p.J, pshift, length, (const E*)q, T, G, qs, n_sel, skip, p.cap, count, cand, sel)
+    dim3(W == 1 ? 256 : 64 * W), 0, st, bk, table, p.J, pshift, length, (const E*)q, T, G, qs, n_sel, skip, screen_cap(p.slots), count, cand, sel)
   if (p.waves == 1) PICK(1, 4); else PICK(16, 1);
 #undef PICK
 }
@@ -398,6 +502,7 @@ extern "C" int gpsr_bank_select(const gpsr_bank* bank, const int32_t* table, int
   if ((!table && table_pages) || !length || !q || !qst || !sel) return arg_fail("bank_select: null pointer");
   if (!type_ok(dtype)) return arg_fail("bank_select: dtype");
   if (B > 65535) return arg_fail("bank_select: more than 65535 entries");
+  if (table_pages > 0x7fffff00) return arg_fail("bank_select: table_pages");
   if (table_pages < 0) return arg_fail("bank_select: table_pages");
   if (q_heads < 1 || q_heads > 65535 || q_heads % bank->heads) return arg_fail("bank_select: query heads must be a multiple of the bank's heads, up to 65535");
   if (n_sel < 1 || n_sel > SE_MAX) return arg_fail("bank_select: n_sel must be in 1..64");
