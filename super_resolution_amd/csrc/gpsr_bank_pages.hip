@@ -11,17 +11,18 @@
 #include "gpsr_bank_tile.hpp"
 
 // ---------------------------------------------------------------- by query
-template <int DT, int BITS, int D>
-__global__ void __launch_bounds__(256, tile_waves(D, Terms<DT>::N, 1, 1))
+template <int DT, int BITS, int D, int W>
+__global__ void __launch_bounds__(256, 2)
 k_bank_pages_query(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, int pshift, const int32_t* __restrict__ length,
                    const typename Row<DT>::T* __restrict__ q, int T, int G, Strides qs, bool qwide, const int32_t* __restrict__ sel,
                    int n_sel, float scale, const int32_t* __restrict__ skip, typename Row<DT>::T* __restrict__ out,
-                   float* __restrict__ lse, int groups, int splits, float* __restrict__ part) {
-  constexpr int NT = Terms<DT>::N, KT = 128;
+                   float* __restrict__ lse, int groups, int splits, float* __restrict__ partials) {
+  typedef Geo<W> X;
+  constexpr int NT = Terms<DT>::N, KT = 128, NB = 32 / W;
   __shared__ __attribute__((aligned(16))) char sm[tile_lds(D, KT)];
   __shared__ int phys[64], rown[64], first[64], total;
   Tile<D, KT> tile(sm);
-  const int tid = threadIdx.x, lane = tid & 63, wave = wave_of(tid), half = lane >> 5, col = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_of(tid), part = lane / W, col = lane % W;
   const int h = blockIdx.y, b = blockIdx.z, H = bk.heads, P = 1 << pshift;
   const int split = blockIdx.x % splits, group = blockIdx.x / splits % groups;
   const int64_t t = blockIdx.x / splits / groups;
@@ -44,12 +45,12 @@ k_bank_pages_query(gpsr_bank bk, const int32_t* __restrict__ table, int table_pa
     if (tid == 0) total = __popcll(all);
   }
   tile.clear_marks(tid, 256);
-  const int g = group * 32 + col;
+  const int g = group * W + col;
   const bool there = g < G;
-  bf8 qf[1][NT][D / 16];
-  load_query<DT, D>(q + b * qs.b + t * qs.t + (int64_t)(h * G + (there ? g : 0)) * qs.h, qwide, there, half, qf[0]);
+  bf8 qf[NT][D / X::STEP];
+  load_query<DT, D, W>(q + b * qs.b + t * qs.t + (int64_t)(h * G + (there ? g : 0)) * qs.h, qwide, there, part, qf);
   const int64_t lo = skip ? skip[((size_t)b * T + t) * 2] : 0, hi = skip ? skip[((size_t)b * T + t) * 2 + 1] : 0;
-  Soft<D, 1> st;
+  Soft<D, W> st;
   st.clear();
   const float c2 = scale * 1.4426950408889634f;
   __syncthreads();
@@ -64,7 +65,7 @@ k_bank_pages_query(gpsr_bank bk, const int32_t* __restrict__ table, int table_pa
   }
   for (unsigned i = i0; i < i1; ++i) {
     __syncthreads();
-    f.store(tile, tid, i + 1);
+    f.template store<W>(tile, tid, i + 1);
     __syncthreads();
     f.codes(bk, h, pshift, (i + 1) * KT, tid);
     f.pages(rows, (i + 2) * KT, tid);
@@ -73,17 +74,18 @@ k_bank_pages_query(gpsr_bank bk, const int32_t* __restrict__ table, int table_pa
       const int64_t pos = slot < (unsigned)total ? (int64_t)first[slot] * P + (v & (P - 1)) : -1;
       return pos >= lo && pos < hi;
     };
-    tile_marks<D, KT, 1, 32>(tile, wrow, i + 1, st, [&](int, int r) { return !skips(i * KT + wrow + r); });
-    f16v s[1][1];
-    tile_logits<D, KT, NT, 1, 1>(tile, wrow, col, half, qf, s);
+    tile_marks<D, KT, 32>(tile, wrow, i + 1, st, [&](int r) { return !skips(i * KT + wrow + r); });
+    typename X::Acc s[NB];
+    tile_logits<D, KT, NT, NB, W>(tile, wrow, col, part, qf, s);
     if (lo < hi) {
       asm volatile("");
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        if (skips(i * KT + wrow + 8 * (e >> 2) + 4 * half + (e & 3))) s[0][0][e] = -__builtin_inff();
-      }
+      for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+        for (int e = 0; e < X::E; ++e)
+          if (skips(i * KT + wrow + kb * W + X::row(part, e))) s[kb][e] = -__builtin_inff();
     }
-    tile_accumulate<D, KT, NT, 1, 1, true>(tile, wrow, col, half, c2, s, st);
+    tile_accumulate<D, KT, NT, NB, W, true>(tile, wrow, col, part, c2, s, st);
   }
   st.spoil();
   __syncthreads();
@@ -91,11 +93,11 @@ k_bank_pages_query(gpsr_bank bk, const int32_t* __restrict__ table, int table_pa
   if (wave || !there) return;
   const int hq = h * G + g;
   if (splits == 1) {
-    st.finish(0);
-    store_column<DT, D>(out + (((size_t)b * T + t) * (size_t)(H * G) + hq) * D, half, st.o, 0);
-    if (lse && half == 0) lse[((size_t)b * (H * G) + hq) * T + t] = st.lse(0);
+    st.finish();
+    st.template store<DT>(out + (((size_t)b * T + t) * (size_t)(H * G) + hq) * D, part);
+    if (lse && part == 0) lse[((size_t)b * (H * G) + hq) * T + t] = st.lse();
   } else {
-    store_partial<D>(part + ((((size_t)(b * H + h) * T + t) * splits + split) * G + g) * (D + 2), half, st, 0);
+    st.store_partial(partials + ((((size_t)(b * H + h) * T + t) * splits + split) * G + g) * (D + 2), part);
   }
 }
 
@@ -194,15 +196,16 @@ k_bank_pages_fill(const int32_t* __restrict__ sel, int n_sel, int table_pages, i
 }
 
 template <int DT, int BITS, int D, int KT>
-__global__ void __launch_bounds__(256, tile_waves(D, Terms<DT>::N, 1, KT / 32))
+__global__ void __launch_bounds__(256, tile_waves(D, Terms<DT>::N, KT / 32))
 k_bank_pages_page(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, int pshift, const int32_t* __restrict__ length,
                   const typename Row<DT>::T* __restrict__ q, int T, int G, Strides qs, bool qwide, int n_sel, float scale,
                   const int32_t* __restrict__ skip, const int* __restrict__ start, const int* __restrict__ wgs, int buckets,
-                  const int* __restrict__ list, float* __restrict__ part) {
-  constexpr int NT = Terms<DT>::N, NB = KT / 32, CW = 128;
+                  const int* __restrict__ list, float* __restrict__ partials) {
+  constexpr int NT = Terms<DT>::N, NB = KT / 32, CW = 128, W = 32;
+  typedef Geo<W> X;
   __shared__ __attribute__((aligned(16))) char sm[tile_lds(D, KT)];
   Tile<D, KT> tile(sm);
-  const int tid = threadIdx.x, lane = tid & 63, wave = wave_of(tid), half = lane >> 5, col = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_of(tid), part = lane / W, col = lane % W;
   const int w = blockIdx.x;
   if (w >= wgs[buckets]) return;
   int a = 0, z = buckets;                 // the last bucket whose first workgroup is not behind this one
@@ -214,13 +217,13 @@ k_bank_pages_page(gpsr_bank bk, const int32_t* __restrict__ table, int table_pag
   const bool there = c < (int64_t)n * G;
   const int id = there ? list[start[a] + (int)(c / G)] : 0, g = (int)(c % G);
   const int t = id / n_sel;
-  bf8 qf[1][NT][D / 16];
-  load_query<DT, D>(q + b * qs.b + t * qs.t + (int64_t)(h * G + (there ? g : 0)) * qs.h, qwide, there, half, qf[0]);
+  bf8 qf[NT][D / X::STEP];
+  load_query<DT, D>(q + b * qs.b + t * qs.t + (int64_t)(h * G + (there ? g : 0)) * qs.h, qwide, there, part, qf);
   int64_t lo = 0, hi = 0;
   if (skip && there) { lo = skip[((size_t)b * T + t) * 2]; hi = skip[((size_t)b * T + t) * 2 + 1]; }
   const int64_t pos0 = (int64_t)lp << pshift;
   const OnePage rows = {table[(size_t)b * table_pages + lp], (int)min((int64_t)P, length[b] - pos0)};
-  Soft<D, 1> st;
+  Soft<D, W> st;
   st.clear();
   const float c2 = scale * 1.4426950408889634f;
   tile.clear_marks(tid, 256);
@@ -229,27 +232,27 @@ k_bank_pages_page(gpsr_bank bk, const int32_t* __restrict__ table, int table_pag
   f.codes(bk, h, pshift, 0, tid);
   for (int v = 0; v < rows.rows; v += KT) {
     __syncthreads();
-    f.store(tile, tid, v / KT + 1);
+    f.template store<W>(tile, tid, v / KT + 1);
     __syncthreads();
     f.pages(rows, v + KT, tid);
     f.codes(bk, h, pshift, v + KT, tid);
-    tile_marks<D, KT, 1, KT>(tile, 0, v / KT + 1, st, [&](int, int r) { return !(pos0 + v + r >= lo && pos0 + v + r < hi); });
-    f16v s[NB][1];
-    tile_logits<D, KT, NT, 1, NB>(tile, 0, col, half, qf, s);
+    tile_marks<D, KT, KT>(tile, 0, v / KT + 1, st, [&](int r) { return !(pos0 + v + r >= lo && pos0 + v + r < hi); });
+    typename X::Acc s[NB];
+    tile_logits<D, KT, NT, NB, W>(tile, 0, col, part, qf, s);
     if (skip && __ballot(lo < pos0 + v + KT && hi > pos0 + v && lo < hi)) {
       asm volatile("");
 #pragma unroll
       for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int64_t pos = pos0 + v + kb * 32 + 8 * (e >> 2) + 4 * half + (e & 3);
-          if (pos >= lo && pos < hi) s[kb][0][e] = -__builtin_inff();
+        for (int e = 0; e < X::E; ++e) {
+          const int64_t pos = pos0 + v + kb * W + X::row(part, e);
+          if (pos >= lo && pos < hi) s[kb][e] = -__builtin_inff();
         }
     }
-    tile_accumulate<D, KT, NT, 1, NB, true>(tile, 0, col, half, c2, s, st);
+    tile_accumulate<D, KT, NT, NB, W, true>(tile, 0, col, part, c2, s, st);
   }
   st.spoil();
-  if (there) store_partial<D>(part + (((size_t)bh * T * n_sel + id) * G + g) * (D + 2), half, st, 0);
+  if (there) st.store_partial(partials + (((size_t)bh * T * n_sel + id) * G + g) * (D + 2), part);
 }
 
 // ---------------------------------------------------------------- host
@@ -274,7 +277,8 @@ static PagesPlan plan_of(const gpsr_bank* bk, int B, int table_pages, int T, int
     p.part = at; at += (size_t)p.entries * G * (bk->dim + 2) * sizeof(float);
     p.bytes = at;
   } else {
-    p.groups = (G + 31) / 32;
+    const int width = G <= 16 ? 16 : 32;
+    p.groups = (G + width - 1) / width;
     const int64_t wgs = (int64_t)B * T * H * p.groups, tiles = ((int64_t)n_sel * bk->page_rows + 127) / 128;
     int64_t s = 512 / wgs;
     if (s < 1) s = 1;
@@ -299,9 +303,11 @@ static void launch_pages(const PagesPlan& p, const gpsr_bank& bk, const int32_t*
   const dim3 join((unsigned)((C + 3) / 4), (unsigned)H, (unsigned)B);
   if (!p.by_page) {
     float* part = (float*)ws;
-    hipLaunchKernelGGL((k_bank_pages_query<DT, BITS, D>), dim3((unsigned)((int64_t)T * p.groups * p.splits), (unsigned)H, (unsigned)B),
-                       dim3(256), 0, st, bk, table, table_pages, pshift, length, (const E*)q, T, G, qs, qwide, sel, n_sel, scale, skip,
-                       (E*)out, lse, p.groups, p.splits, part);
+#define QUERY(W) hipLaunchKernelGGL((k_bank_pages_query<DT, BITS, D, W>), dim3((unsigned)((int64_t)T * p.groups * p.splits), (unsigned)H, \
+    (unsigned)B), dim3(256), 0, st, bk, table, table_pages, pshift, length, (const E*)q, T, G, qs, qwide, sel, n_sel, scale, skip, (E*)out, \
+    lse, p.groups, p.splits, part)
+    if (G <= 16) QUERY(16); else QUERY(32);
+#undef QUERY
     if (p.splits > 1)
       hipLaunchKernelGGL((k_bank_join<DT, D>), join, dim3(256), 0, st, part, T, G, H, C, p.splits, (size_t)p.splits * C, (size_t)1,
                          (size_t)p.splits * G, (size_t)G, (E*)out, lse);

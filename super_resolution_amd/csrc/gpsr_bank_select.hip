@@ -249,7 +249,7 @@ k_bank_select_screen(int H, const int32_t* __restrict__ length, int pshift, cons
         if (v[i] > -__builtin_inff()) { low = fminf(low, v[i]); ++c; }
       }
       c += __shfl_xor(c, 32);
-      top = fmaxf(top, other_half(top)); low = fminf(low, other_half(low));
+      top = fmaxf(top, __shfl_xor(top, 32)); low = fminf(low, __shfl_xor(low, 32));
       int64_t a = ordered(low), z = (int64_t)ordered(top) + 1;      // at least n_sel groups are >= a, fewer >= z
       const bool enough = c >= n_sel;
       for (int i = 0; i < 20; ++i) {
@@ -384,38 +384,59 @@ k_bank_select_pick(gpsr_bank bk, const int32_t* __restrict__ table, int J, int p
       ok[sub] = page >= 0 && page < bk.pages && !(lp[sub] >= slo && lp[sub] < shi);
       c[sub] = (const f4v*)(bk.centroid + ((size_t)(ok[sub] ? page : 0) * H + h) * D);
     };
-    const auto score = [&](int sub) {
-      double dot[4] = {0, 0, 0, 0}, sq[4] = {0, 0, 0, 0};
-      for (int g = 0; g < D / 32; ++g) {
-        f4v y[2];
-#pragma unroll
-        for (int d = 0; d < 2; ++d) y[d] = c[sub][8 * g + 4 * d + part];
-#pragma unroll
-        for (int d = 0; d < 2; ++d)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const double z = (double)y[d][j];
-            dot[j] = fma(qv[slot][32 * g + 16 * d + 4 * part + j], z, dot[j]);
-            if (rbf) sq[j] = fma(z, z, sq[j]);
-          }
-      }
-      double s = (dot[0] + dot[1]) + (dot[2] + dot[3]);
-      if (rbf) s -= 0.5 * G * ((sq[0] + sq[1]) + (sq[2] + sq[3]));
+    const auto place = [&](int sub, double s, double sq) {
+      if (rbf) s -= 0.5 * G * sq;
       s += __shfl_xor(s, 1); s += __shfl_xor(s, 2);
       Scored y = {worst, none};
       if (ok[sub] && s == s) y = {s, lp[sub]};
       y.s = __shfl(y.s, (lane & 15) * 4); y.at = __shfl(y.at, (lane & 15) * 4);
       if ((lane >> 4) == sub) x = y;
     };
-    if constexpr (W > 1) {         // few waves on the chip: the look-ups of all 64 pages wait together
+    if constexpr (W > 1) {         // few waves on the chip: the look-ups of all 64 pages wait together, and 32 columns of them
 #pragma unroll
       for (int sub = 0; sub < 4; ++sub) look_up(sub);
+      double dot[4] = {0, 0, 0, 0}, sq[4] = {0, 0, 0, 0};
+#pragma unroll 2
+      for (int g = 0; g < D / 32; ++g) {
+        f4v y[4][2];
 #pragma unroll
-      for (int sub = 0; sub < 4; ++sub) score(sub);
+        for (int sub = 0; sub < 4; ++sub)
+#pragma unroll
+          for (int d = 0; d < 2; ++d) y[sub][d] = c[sub][8 * g + 4 * d + part];
+#pragma unroll
+        for (int sub = 0; sub < 4; ++sub)
+#pragma unroll
+          for (int d = 0; d < 2; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const double z = (double)y[sub][d][j];
+              dot[sub] = fma(qv[slot][32 * g + 16 * d + 4 * part + j], z, dot[sub]);
+              if (rbf) sq[sub] = fma(z, z, sq[sub]);
+            }
+      }
+#pragma unroll
+      for (int sub = 0; sub < 4; ++sub) place(sub, dot[sub], sq[sub]);
     } else {                       // some 20 candidates: no work for pages that are not there
 #pragma unroll
       for (int sub = 0; sub < 4; ++sub)
-        if (i0 + sub * 16 < n) { look_up(sub); score(sub); }
+        if (i0 + sub * 16 < n) {
+          look_up(sub);
+          double dot[4] = {0, 0, 0, 0}, sq[4] = {0, 0, 0, 0};
+          for (int g = 0; g < D / 32; ++g) {
+            f4v y[2];
+#pragma unroll
+            for (int d = 0; d < 2; ++d) y[d] = c[sub][8 * g + 4 * d + part];
+#pragma unroll
+            for (int d = 0; d < 2; ++d)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const double z = (double)y[d][j];
+                dot[j] = fma(qv[slot][32 * g + 16 * d + 4 * part + j], z, dot[j]);
+                if (rbf) sq[j] = fma(z, z, sq[j]);
+              }
+          }
+          place(sub, (dot[0] + dot[1]) + (dot[2] + dot[3]), (sq[0] + sq[1]) + (sq[2] + sq[3]));
+        }
     }
     if (empty && n <= 32) { sort64<32>(x, lane, true); best = x; break; }
     if (empty) { sort64(x, lane, true); best = x; empty = false; continue; }

@@ -1,26 +1,49 @@
-// gpsr_bank_tile.hpp -- a tile of bank rows against 32-column blocks of queries on the matrix units.
+// gpsr_bank_tile.hpp -- a tile of bank rows against blocks of W = 32 or 16 query columns on the matrix units.
 //
-// Logits are formed transposed, S^T = K Q^T (rows of the bank down, columns = queries across), with v_mfma_f32_32x32x16_bf16:
-// a lane then holds 16 logits of ONE query for each 32 rows, so the softmax statistics are lane-local but for one exchange
-// between the wave's halves, and the accumulator registers, rounded to bf16, are the second product's operand as they are:
-// O^T = V^T P^T contracts over rows, and the order of a contraction is free as long as both operands agree, so V^T is laid
-// out in LDS in the order in which the accumulators hold the rows (within 16 rows: 0-3, 8-11 | 4-7, 12-15).
+// Logits are formed transposed, S^T = K Q^T (rows of the bank down, columns = queries across), with
+// v_mfma_f32_32x32x16_bf16 (16x16x32 for up to 16 columns): a lane then holds logits of ONE query, 16 of 32 rows (4 of 16), so
+// the softmax statistics are lane-local but for an exchange between the wave's parts, and the accumulator registers, rounded
+// to bf16, are the second product's operand as they are: O^T = V^T P^T contracts over rows, and the order of a contraction is
+// free as long as both operands agree, so V^T is laid out in LDS in the order in which the accumulators hold the rows.
 // Held values have at most 4 significant bits: bf16 holds them exactly.  Queries and weights are split into Terms<DT>::N bf16
 // terms (8 bits each: bf16 queries 1, f16 2, f32 3), so that the products lose nothing that the caller's type can hold.
 #pragma once
 #include "gpsr_bank.hpp"
+
+// What an accumulator of W columns holds: lane = part * W + column, E values, value e of row row(part, e).  A product contracts
+// over STEP indices, 8 neighbouring ones for each part; slot(r) is where row r of a STEP goes for the second product.
+template <int W> struct Geo;
+template <> struct Geo<32> {
+  typedef f16v Acc;
+  static constexpr int E = 16, STEP = 16;
+  __device__ __forceinline__ static int row(int part, int e) { return 8 * (e >> 2) + 4 * part + (e & 3); }
+  __device__ __forceinline__ static int slot(int r) { return ((r >> 2) & 1) * 8 + (r >> 3) * 4 + (r & 3); }   // 0-3, 8-11 | 4-7, 12-15
+  __device__ __forceinline__ static Acc mul(bf8 a, bf8 b, Acc c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+  template <class F> __device__ __forceinline__ static float parts(float x, const F& f) { return f(x, __shfl_xor(x, 32)); }
+};
+template <> struct Geo<16> {
+  typedef f4v Acc;
+  static constexpr int E = 4, STEP = 32;
+  __device__ __forceinline__ static int row(int part, int e) { return 4 * part + e; }
+  __device__ __forceinline__ static int slot(int r) { return ((r >> 2) & 3) * 8 + (r >> 4) * 4 + (r & 3); }   // 0-3, 16-19 | 4-7, 20-23 | ..
+  __device__ __forceinline__ static Acc mul(bf8 a, bf8 b, Acc c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+  template <class F> __device__ __forceinline__ static float parts(float x, const F& f) {
+    x = f(x, __shfl_xor(x, 16));
+    return f(x, __shfl_xor(x, 32));
+  }
+};
+__device__ __forceinline__ float max2(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ float add2(float a, float b) { return a + b; }
 
 template <int DT> struct Terms;
 template <> struct Terms<GPSR_BF16> { static constexpr int N = 1; };
 template <> struct Terms<GPSR_F16> { static constexpr int N = 2; };
 template <> struct Terms<GPSR_F32> { static constexpr int N = 3; };
 
-// registers that a wave of NQ x 32 columns and NB x 32 rows at a time needs, roughly: sums, logits, query terms, the rest
-static constexpr int tile_regs(int d, int nt, int nq, int nb) { return nq * (d / 2 + 16 * nb + nt * d / 4) + 64; }
+// registers that a wave of 32 columns and NB x 32 rows at a time needs, roughly: sums, logits, query terms, the rest
+static constexpr int tile_regs(int d, int nt, int nb) { return d / 2 + 16 * nb + nt * d / 4 + 64; }
 // waves per SIMD that they are budgeted for
-static constexpr int tile_waves(int d, int nt, int nq, int nb) {
-  return tile_regs(d, nt, nq, nb) <= 128 ? 4 : tile_regs(d, nt, nq, nb) <= 250 ? 2 : 1;
-}
+static constexpr int tile_waves(int d, int nt, int nb) { return tile_regs(d, nt, nb) <= 128 ? 4 : tile_regs(d, nt, nb) <= 250 ? 2 : 1; }
 
 template <int DT>
 __device__ __forceinline__ typename Row<DT>::T from_f32(float y) {
@@ -42,14 +65,14 @@ __device__ __forceinline__ void split_terms(const float* y, bf8* t) {
     }
 }
 
-template <int DT, int D>
-__device__ __forceinline__ void load_query(const typename Row<DT>::T* __restrict__ p, bool wide, bool there, int half,
-                                           bf8 (&qf)[Terms<DT>::N][D / 16]) {
+template <int DT, int D, int W = 32>
+__device__ __forceinline__ void load_query(const typename Row<DT>::T* __restrict__ p, bool wide, bool there, int part,
+                                           bf8 (&qf)[Terms<DT>::N][D / Geo<W>::STEP]) {
   constexpr int NT = Terms<DT>::N;
 #pragma unroll
-  for (int s = 0; s < D / 16; ++s) {
+  for (int s = 0; s < D / Geo<W>::STEP; ++s) {
     float y[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (there) load8<DT>(p + s * 16 + half * 8, wide, y);
+    if (there) load8<DT>(p + s * Geo<W>::STEP + part * 8, wide, y);
     bf8 t[NT];
     split_terms<NT>(y, t);
 #pragma unroll
@@ -135,11 +158,11 @@ struct OnePage {
 template <int BITS, int D, int KT, int NTH>
 struct Fetch {
   static constexpr int U = KT * D / 32, N = (2 * U + NTH - 1) / NTH;
-  static constexpr int W = BITS / 4;                     // code words of 8 columns
+  static constexpr int CW = BITS / 4;                    // code words of 8 columns
   static constexpr bool EVEN = 2 * U % NTH == 0;
   int page[N], left[N];                                  // of the next tile; page -1: the row does not exist
   int fpage[N], fleft[N];                                // of the tile whose codes are under way
-  unsigned w[N][4 * W], sc[N][4];                        // keys: scale byte and offset in sc[0], sc[1]
+  unsigned w[N][4 * CW], sc[N][4];                        // keys: scale byte and offset in sc[0], sc[1]
 
   // unit i of this thread: keys? and its number among its kind
   __device__ __forceinline__ static bool keys(int i, int tid) {
@@ -174,7 +197,7 @@ struct Fetch {
         const int g = u % (D / 32);
         const u4v* src = (const u4v*)(bk.k_codes + at * (size_t)(D * BITS / 8) + g * (4 * BITS));
 #pragma unroll
-        for (int j = 0; j < W; ++j) {
+        for (int j = 0; j < CW; ++j) {
           const u4v a = src[j];
           w[i][4 * j] = a.x; w[i][4 * j + 1] = a.y; w[i][4 * j + 2] = a.z; w[i][4 * j + 3] = a.w;
         }
@@ -186,7 +209,7 @@ struct Fetch {
         const uint8_t* scale = bk.v_scales + at * (size_t)(D / 32) + c / 4;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {   // rows of one page: page_rows is a multiple of 16
-          if constexpr (W == 1) w[i][j] = *(const unsigned*)(src + j * (D * BITS / 8));
+          if constexpr (CW == 1) w[i][j] = *(const unsigned*)(src + j * (D * BITS / 8));
           else { const u2v a = *(const u2v*)(src + j * (D * BITS / 8)); w[i][2 * j] = a.x; w[i][2 * j + 1] = a.y; }
           sc[i][j] = scale[j * (D / 32)];
         }
@@ -195,6 +218,7 @@ struct Fetch {
   }
 
   // decodes them to LDS; rows that do not exist become zeros with an offset of -inf
+  template <int W>
   __device__ __forceinline__ void store(const Tile<D, KT>& tile, int tid, unsigned number) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -208,7 +232,7 @@ struct Fetch {
         const float s = scale_of(there ? sc[i][0] : 127u);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const unsigned w0 = there ? w[i][W * j] : 0u, w1 = there ? w[i][W * j + W - 1] : 0u;
+          const unsigned w0 = there ? w[i][CW * j] : 0u, w1 = there ? w[i][CW * j + CW - 1] : 0u;
           dst[j] = u4v{pair<BITS, 0>(w0, w1, s), pair<BITS, 1>(w0, w1, s), pair<BITS, 2>(w0, w1, s), pair<BITS, 3>(w0, w1, s)};
         }
         if (g == 0) tile.off[r] = there ? __uint_as_float(sc[i][1]) : -__builtin_inff();
@@ -220,12 +244,12 @@ struct Fetch {
           const bool here = j < fleft[i], nan = here && sc[i][j] == 255u, there = here && !nan;
           if (nan) { tile.mark[(r + j) * (D / 32) + c / 4] = number; tile.mark[KT * (D / 32)] = number; }
           const float s = scale_of(there ? sc[i][j] : 127u);
-          const unsigned w0 = there ? w[i][W * j] : 0u, w1 = there ? w[i][W * j + W - 1] : 0u;
+          const unsigned w0 = there ? w[i][CW * j] : 0u, w1 = there ? w[i][CW * j + CW - 1] : 0u;
           y[j][0] = pair<BITS, 0>(w0, w1, s); y[j][1] = pair<BITS, 1>(w0, w1, s);
           y[j][2] = pair<BITS, 2>(w0, w1, s); y[j][3] = pair<BITS, 3>(w0, w1, s);
         }
         // rows r .. r + 3 of the tile are 4 neighbouring slots of a column
-        const int k16 = r & 15, slot = (r & ~15) + ((k16 >> 2) & 1) * 8 + (k16 >> 3) * 4;
+        const int slot = (r & ~(Geo<W>::STEP - 1)) + Geo<W>::slot(r & (Geo<W>::STEP - 1));
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           *(u2v*)(tile.v + Tile<D, KT>::at(c * 8 + 2 * e, slot)) = u2v{pack_lo(y[0][e], y[1][e]), pack_lo(y[2][e], y[3][e])};
@@ -236,142 +260,141 @@ struct Fetch {
   }
 };
 
-// raw logits q.k + offset of the wave's NB x 32 rows (from wrow on) for its NQ x 32 columns
-template <int D, int KT, int NT, int NQ, int NB>
-__device__ __forceinline__ void tile_logits(const Tile<D, KT>& tile, int wrow, int col, int half, const bf8 (&qf)[NQ][NT][D / 16],
-                                            f16v (&s)[NB][NQ]) {
+// raw logits q.k + offset of NB x W rows (from r0 on) for a wave's W columns
+template <int D, int KT, int NT, int NB, int W>
+__device__ __forceinline__ void tile_logits(const Tile<D, KT>& tile, int r0, int col, int part, const bf8 (&qf)[NT][D / Geo<W>::STEP],
+                                            typename Geo<W>::Acc (&s)[NB]) {
+  typedef Geo<W> X;
 #pragma unroll
   for (int kb = 0; kb < NB; ++kb) {
-    f16v o;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const f4v a = *(const f4v*)(tile.off + wrow + kb * 32 + 8 * i + 4 * half);
+    for (int e = 0; e < X::E; e += 4) {
+      const f4v a = *(const f4v*)(tile.off + r0 + kb * W + X::row(part, e));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[4 * i + j] = a[j];
+      for (int j = 0; j < 4; ++j) s[kb][e + j] = a[j];
     }
+    const uint16_t* base = tile.k + (r0 + kb * W + col) * Tile<D, KT>::KS + part * 8;
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) s[kb][n] = o;
-    const uint16_t* base = tile.k + (wrow + kb * 32 + col) * Tile<D, KT>::KS + half * 8;
+    for (int d = 0; d < D / X::STEP; ++d) {
+      const bf8 a = *(const bf8*)(base + d * X::STEP);
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d) {
-      const bf8 a = *(const bf8*)(base + d * 16);
-#pragma unroll
-      for (int n = 0; n < NQ; ++n)
-#pragma unroll
-        for (int t = 0; t < NT; ++t) s[kb][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, qf[n][t][d], s[kb][n], 0, 0, 0);
+      for (int t = 0; t < NT; ++t) s[kb] = X::mul(a, qf[t][d], s[kb]);
     }
   }
 }
 
-__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
+typedef float f4u __attribute__((ext_vector_type(4), aligned(8)));     // partial results: rows of D + 2 floats
 
-// ---- running softmax of a wave's columns: m the power of two that weights are taken against
-// (logit * log2 e; -inf: no row seen), l this half's sum of weights, o = sum of weights * values
-template <int D, int NQ>
+// ---- running softmax of a wave's columns: m the power of two that weights are taken against (logit * log2 e; -inf: no row
+// seen), l this part's sum of weights, o = sum of weights * values
+template <int D, int W>
 struct Soft {
-  f16v o[D / 32][NQ];
-  float m[NQ], l[NQ];
-  unsigned nan[NQ];     // bit g: a row that the column sees is NaN in columns 32 g .. of its values
+  typedef Geo<W> X;
+  typename X::Acc o[D / W];
+  float m, l;
+  unsigned nan;         // bit g: a row that the column sees is NaN in columns 32 g .. of its values
   __device__ __forceinline__ void clear() {
+    m = -__builtin_inff(); l = 0.f; nan = 0;
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      m[n] = -__builtin_inff(); l[n] = 0.f; nan[n] = 0;
+    for (int d = 0; d < D / W; ++d)
 #pragma unroll
-      for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[d][n][e] = 0.f;
-    }
+      for (int e = 0; e < X::E; ++e) o[d][e] = 0.f;
   }
-  __device__ __forceinline__ bool wants_move() const {
-    bool x = false;
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) x |= m[n] == -__builtin_inff() || l[n] > 0x1p40f;
-    return __ballot(x) != 0;
-  }
+  __device__ __forceinline__ bool wants_move() const { return __ballot(m == -__builtin_inff() || l > 0x1p40f) != 0; }
   // whether a sum ran out of range (or met a NaN: then a second walk changes nothing)
-  __device__ __forceinline__ bool lost() const {
-    bool x = false;
+  __device__ __forceinline__ bool lost() const { return !(l < __builtin_inff()); }
+  __device__ __forceinline__ void rescale(float a) {
+    l *= a;
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) x |= !(l[n] < __builtin_inff());
-    return x;
-  }
-  __device__ __forceinline__ void rescale(int n, float a) {
-    l[n] *= a;
+    for (int d = 0; d < D / W; ++d)
 #pragma unroll
-    for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) o[d][n][e] *= a;
+      for (int e = 0; e < X::E; ++e) o[d][e] *= a;
   }
   __device__ __forceinline__ void spoil() {
+    if (__ballot(nan != 0))
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      const unsigned all = nan[n];
-      if (__ballot(all != 0))
+      for (int d = 0; d < D / W; ++d)
+        if (nan >> (d * W / 32) & 1)
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d)
-          if (all >> d & 1)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[d][n][e] = __builtin_nanf("");
-    }
+          for (int e = 0; e < X::E; ++e) o[d][e] = __builtin_nanf("");
   }
   // divides; l becomes the whole sum
-  __device__ __forceinline__ void finish(int n) {
-    l[n] += other_half(l[n]);
-    const float r = l[n] == 0.f ? 0.f : 1.f / l[n];
+  __device__ __forceinline__ void finish() {
+    l = X::parts(l, add2);
+    const float r = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-    for (int d = 0; d < D / 32; ++d)
+    for (int d = 0; d < D / W; ++d)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) o[d][n][e] *= r;
+      for (int e = 0; e < X::E; ++e) o[d][e] *= r;
   }
-  __device__ __forceinline__ float lse(int n) const {
-    return l[n] == 0.f ? -__builtin_inff() : (log2f(l[n]) + m[n]) * 0.6931471805599453f;
-  }
-  // wave 0 gets the sum over WK waves that held the same columns; buf: 64 x (D / 2 + 2) floats for each block of columns
+  __device__ __forceinline__ float lse() const { return l == 0.f ? -__builtin_inff() : (log2f(l) + m) * 0.6931471805599453f; }
+  // wave 0 gets the sum over WK waves that held the same columns; buf: 64 (D W / 64 + 2) floats
   template <int WK>
   __device__ __forceinline__ void join(float* buf, int wave, int lane) {
     for (int w = 1; w < WK; ++w) {
       if (wave == w) {
+        buf[lane] = m; buf[64 + lane] = l;
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-          float* p = buf + n * 64 * (D / 2 + 2);
-          p[lane] = m[n]; p[64 + lane] = l[n];
+        for (int d = 0; d < D / W; ++d)
 #pragma unroll
-          for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) p[(2 + d * 16 + e) * 64 + lane] = o[d][n][e];
-        }
+          for (int e = 0; e < X::E; ++e) buf[(2 + d * X::E + e) * 64 + lane] = o[d][e];
       }
       __syncthreads();
       if (wave == 0) {
+        const float m2 = buf[lane], mn = fmaxf(m, m2), safe = mn == -__builtin_inff() ? 0.f : mn;
+        const float a = exp2f(m - safe), b = exp2f(m2 - safe);
+        m = mn;
+        l = l * a + buf[64 + lane] * b;
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-          const float* p = buf + n * 64 * (D / 2 + 2);
-          const float m2 = p[lane], mn = fmaxf(m[n], m2), safe = mn == -__builtin_inff() ? 0.f : mn;
-          const float a = exp2f(m[n] - safe), b = exp2f(m2 - safe);
-          m[n] = mn;
-          l[n] = l[n] * a + p[64 + lane] * b;
+        for (int d = 0; d < D / W; ++d)
 #pragma unroll
-          for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[d][n][e] = o[d][n][e] * a + p[(2 + d * 16 + e) * 64 + lane] * b;
-        }
+          for (int e = 0; e < X::E; ++e) o[d][e] = o[d][e] * a + buf[(2 + d * X::E + e) * 64 + lane] * b;
       }
       __syncthreads();
     }
   }
+  // a lane's part of its column: 4 neighbouring dims at a time
+  template <int DT>
+  __device__ __forceinline__ void store(typename Row<DT>::T* __restrict__ out, int part) const {
+#pragma unroll
+    for (int d = 0; d < D / W; ++d)
+#pragma unroll
+      for (int e = 0; e < X::E; e += 4) {
+        typename Row<DT>::T* p = out + d * W + X::row(part, e);
+        if constexpr (DT == GPSR_F32) {
+          *(f4v*)p = f4v{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
+        } else {
+          unsigned w[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            w[j] = (unsigned)__builtin_bit_cast(uint16_t, from_f32<DT>(o[d][e + 2 * j])) |
+                   ((unsigned)__builtin_bit_cast(uint16_t, from_f32<DT>(o[d][e + 2 * j + 1])) << 16);
+          *(u2v*)p = u2v{w[0], w[1]};
+        }
+      }
+  }
+  // [D] sums, reference, sum of weights
+  __device__ __forceinline__ void store_partial(float* __restrict__ p, int part) const {
+    const float all = X::parts(l, add2);
+#pragma unroll
+    for (int d = 0; d < D / W; ++d)
+#pragma unroll
+      for (int e = 0; e < X::E; e += 4)
+        *(f4u*)(p + d * W + X::row(part, e)) = f4u{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
+    if (part == 0) *(f2v*)(p + D) = f2v{m, all};
+  }
 };
 
-// Rows of the tile that a column sees and whose values are NaN; seen(n, r): whether column n does not skip row r of the wave's.
-template <int D, int KT, int NQ, int KW, class Seen>
-__device__ __forceinline__ void tile_marks(const Tile<D, KT>& tile, int wrow, unsigned number, Soft<D, NQ>& st, const Seen& seen) {
+// Rows of the tile that a column sees and whose values are NaN; seen(r): whether it does not skip row r of the wave's KW.
+template <int D, int KT, int KW, int W, class Seen>
+__device__ __forceinline__ void tile_marks(const Tile<D, KT>& tile, int wrow, unsigned number, Soft<D, W>& st, const Seen& seen) {
   if (tile.mark[KT * (D / 32)] != number) return;
 #pragma unroll 1
   for (int r = 0; r < KW; ++r) {
     if (tile.off[wrow + r] == -__builtin_inff()) continue;
     unsigned bits = 0;
     for (int g = 0; g < D / 32; ++g) bits |= (tile.mark[(wrow + r) * (D / 32) + g] == number ? 1u : 0u) << g;
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) st.nan[n] |= seen(n, r) ? bits : 0u;
+    st.nan |= seen(r) ? bits : 0u;
   }
 }
 
@@ -380,92 +403,52 @@ __device__ __forceinline__ void tile_marks(const Tile<D, KT>& tile, int wrow, un
 //   otherwise it stays, which saves the maximum of every tile and the wait for it: bf16 and the sums have range to spare, and
 //     their precision is relative.  Soft::wants_move says when it has to be moved (nothing seen yet, or a sum past 2^40); a
 //     weight past 2^127 makes the sum infinite, which the caller has to look for (Soft::lost) and walk again with MOVE only.
-template <int D, int KT, int NT, int NQ, int NB, bool MOVE>
-__device__ __forceinline__ void tile_accumulate(const Tile<D, KT>& tile, int wrow, int col, int half, float c2, f16v (&s)[NB][NQ],
-                                                Soft<D, NQ>& st) {
+template <int D, int KT, int NT, int NB, int W, bool MOVE>
+__device__ __forceinline__ void tile_accumulate(const Tile<D, KT>& tile, int r0, int col, int part, float c2,
+                                                typename Geo<W>::Acc (&s)[NB], Soft<D, W>& st) {
+  typedef Geo<W> X;
   if constexpr (MOVE) {
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      float mx = s[0][n][0];
-#pragma unroll
-      for (int kb = 0; kb < NB; ++kb)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[kb][n][e]);
-      float mn = fmaxf(st.m[n], fmaxf(mx, other_half(mx)) * c2);
-      if (fmaxf(st.l[n], other_half(st.l[n])) > 0x1p40f) mn = fmaxf(mn, st.m[n] + 40.f);
-      st.rescale(n, mn == -__builtin_inff() ? 1.f : exp2f(st.m[n] - mn));
-      st.m[n] = mn;
-    }
-  }
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    const float ref = st.m[n] == -__builtin_inff() ? 0.f : -st.m[n];
-    float sum = 0.f;
+    float mx = s[0][0];
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float w = __builtin_amdgcn_exp2f(fmaf(s[kb][n][e], c2, ref));
-        s[kb][n][e] = w;
-        sum += w;
-      }
-    st.l[n] += sum;
+      for (int e = 0; e < X::E; ++e) mx = fmaxf(mx, s[kb][e]);
+    float mn = fmaxf(st.m, X::parts(mx, max2) * c2);
+    if (X::parts(st.l, max2) > 0x1p40f) mn = fmaxf(mn, st.m + 40.f);
+    st.rescale(mn == -__builtin_inff() ? 1.f : exp2f(st.m - mn));
+    st.m = mn;
   }
+  const float ref = st.m == -__builtin_inff() ? 0.f : -st.m;
+  float sum = 0.f;
 #pragma unroll
   for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {       // 16 rows
-      bf8 p[NQ][NT];
-#pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        float y[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = s[kb][n][8 * k + e];
-        split_terms<NT>(y, p[n]);
-      }
-#pragma unroll
-      for (int d = 0; d < D / 32; ++d) {
-        const bf8 a = *(const bf8*)(tile.v + Tile<D, KT>::at(d * 32 + col, wrow + kb * 32 + k * 16 + half * 8));
-#pragma unroll
-        for (int n = 0; n < NQ; ++n)
-#pragma unroll
-          for (int t = 0; t < NT; ++t) st.o[d][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, p[n][t], st.o[d][n], 0, 0, 0);
-      }
+    for (int e = 0; e < X::E; ++e) {
+      const float w = __builtin_amdgcn_exp2f(fmaf(s[kb][e], c2, ref));
+      s[kb][e] = w;
+      sum += w;
     }
-}
-
-// a lane's half of one column: 4 neighbouring dims at a time
-template <int DT, int D, int NQ>
-__device__ __forceinline__ void store_column(typename Row<DT>::T* __restrict__ out, int half, const f16v (&o)[D / 32][NQ], int n) {
+  st.l += sum;
+  constexpr int CH = NB * W / X::STEP;     // contractions of STEP rows
 #pragma unroll
-  for (int d = 0; d < D / 32; ++d)
+  for (int k = 0; k < CH; ++k) {
+    float y[8];
+    if constexpr (W == 32) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      typename Row<DT>::T* p = out + d * 32 + 8 * i + 4 * half;
-      if constexpr (DT == GPSR_F32) {
-        *(f4v*)p = f4v{o[d][n][4 * i], o[d][n][4 * i + 1], o[d][n][4 * i + 2], o[d][n][4 * i + 3]};
-      } else {
-        unsigned w[2];
+      for (int e = 0; e < 8; ++e) y[e] = s[k / 2][8 * (k % 2) + e];
+    } else {
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          w[j] = (unsigned)__builtin_bit_cast(uint16_t, from_f32<DT>(o[d][n][4 * i + 2 * j])) |
-                 ((unsigned)__builtin_bit_cast(uint16_t, from_f32<DT>(o[d][n][4 * i + 2 * j + 1])) << 16);
-        *(u2v*)p = u2v{w[0], w[1]};
-      }
+      for (int e = 0; e < 8; ++e) y[e] = s[2 * k + e / 4][e % 4];
     }
-}
-
-// [D] sums, reference logit, sum of weights
-template <int D, int NQ>
-__device__ __forceinline__ void store_partial(float* __restrict__ p, int half, Soft<D, NQ>& st, int n) {
-  const float l = st.l[n] + other_half(st.l[n]);
+    bf8 p[NT];
+    split_terms<NT>(y, p);
 #pragma unroll
-  for (int d = 0; d < D / 32; ++d)
+    for (int d = 0; d < D / W; ++d) {
+      const bf8 a = *(const bf8*)(tile.v + Tile<D, KT>::at(d * W + col, r0 + k * X::STEP + part * 8));
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) p[d * 32 + 8 * i + 4 * half + j] = st.o[d][n][4 * i + j];
-  if (half == 0) { p[D] = st.m[n]; p[D + 1] = l; }
+      for (int t = 0; t < NT; ++t) st.o[d] = X::mul(a, p[t], st.o[d]);
+    }
+  }
 }
 
 // Joins the partial results of one column, at most 64: one wave per column.  First lane i weighs partial i, then the lanes

@@ -485,10 +485,17 @@ def _strided(t, B, H, D, dev, what):
 
 def _bank_index(table, per_entry, dev, what):
     """Pointers of table [B,J] and of one int32 per entry."""
-    if table.dim() != 2 or any(t.shape != table.shape[:1] for t in per_entry):
+    shape = table.shape
+    if len(shape) == 2:
+        B = shape[:1]
+        fits = True
+        for t in per_entry:
+            fits = fits and t.shape == B
+    if len(shape) != 2 or not fits:
         raise _lib.GpsrError(f"{what}: expected a [B,J] table and [B] integers, got {tuple(table.shape)}, "
                              f"{[tuple(t.shape) for t in per_entry]}")
-    return (_ptr(table, torch.int32, dev), *[_ptr(t, torch.int32, dev) for t in per_entry])
+    i32 = torch.int32
+    return (_ptr(table, i32, dev), *[_ptr(t, i32, dev) for t in per_entry])
 
 
 def bank_write(bank, table, start, count, k, v):
@@ -515,7 +522,8 @@ def bank_read(bank, table, start, count, rows, dtype=torch.float32):
     if code is None:
         raise _lib.GpsrError(f"bank_read: expected bfloat16, float16 or float32, got {dtype}")
     B, J = table.shape
-    k, v = (torch.empty((B, rows, H, D), dtype=dtype, device=table.device) for _ in range(2))
+    k = table.new_empty((B, rows, H, D), dtype=dtype)
+    v = torch.empty_like(k)
     _lib.check(lib.gpsr_bank_read(ref, tp, B, J, sp, cp, k.data_ptr(), v.data_ptr(), code, rows, _stream()), "gpsr_bank_read")
     return k, v
 
@@ -537,15 +545,15 @@ def _bank_query(bank, table, length, q, skip, what):
 
 
 def _bank_out(q, want_lse, B, T, Hq):
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device) if want_lse else None
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = q.new_empty((B, Hq, T), dtype=torch.float32) if want_lse else None
     return out, lse, None if lse is None else lse.data_ptr()
 
 
 def _bank_workspace(nbytes, q):
     if not nbytes:
         return None, None
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    ws = q.new_empty(nbytes, dtype=torch.uint8)
     return ws, ws.data_ptr()
 
 
@@ -568,7 +576,7 @@ def bank_select(bank, table, length, q, n_sel, skip=None):
     args, sizes, (B, T, H, Hq, D), code, sk, lib, dev = _bank_query(bank, table, length, q, skip, "bank_select")
     if not 1 <= n_sel <= 64:
         raise _lib.GpsrError(f"bank_select: n_sel must be in 1..64, got {n_sel}")
-    sel = torch.empty((B, T, H, n_sel), dtype=torch.int32, device=q.device)
+    sel = q.new_empty((B, T, H, n_sel), dtype=torch.int32)
     nbytes = lib.gpsr_bank_select_workspace_bytes(*sizes, n_sel, code)
     ws, ws_p = _bank_workspace(nbytes, q)
     _lib.check(lib.gpsr_bank_select(*args, n_sel, sk, sel.data_ptr(), ws_p, nbytes, _stream()), "gpsr_bank_select")
