@@ -15,7 +15,7 @@ __global__ void __launch_bounds__(64 * NW, WK > 1 ? 2 : tile_waves(D, Terms<DT>:
 k_bank_attend(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, int pshift, const int32_t* __restrict__ length,
               const typename Row<DT>::T* __restrict__ q, int T, int G, Strides qs, bool qwide, float scale,
               const int32_t* __restrict__ skip, typename Row<DT>::T* __restrict__ out, float* __restrict__ lse, int splits,
-              float* __restrict__ partials) {
+              float* __restrict__ sums, f2v* __restrict__ stats) {
   typedef Geo<W> X;
   constexpr int NT = Terms<DT>::N, KW = KT / WK;                 // rows of one wave
   constexpr int CW = (NW / WK) * W;                              // columns of the workgroup
@@ -116,7 +116,8 @@ k_bank_attend(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, 
     st.template store<DT>(out + (((size_t)b * T + t) * (size_t)(H * G) + hq) * D, part);
     if (lse && part == 0) lse[((size_t)b * (H * G) + hq) * T + t] = st.lse();
   } else {
-    st.store_partial(partials + (((size_t)(b * H + h) * splits + split) * C + c) * (D + 2), part);
+    const size_t at = ((size_t)(b * H + h) * splits + split) * C + c;
+    st.store_partial(sums + at * D, stats + at, part);
   }
 }
 
@@ -151,27 +152,29 @@ static Plan plan_of(const gpsr_bank* bk, int B, int table_pages, int T, int q_he
 extern "C" size_t gpsr_bank_attend_workspace_bytes(const gpsr_bank* bank, int B, int table_pages, int T, int q_heads, int dtype) {
   if (bank_wrong(bank) || B <= 0 || T <= 0 || table_pages < 0 || q_heads < 1 || q_heads % bank->heads || !type_ok(dtype)) return 0;
   const Plan p = plan_of(bank, B, table_pages, T, q_heads, dtype);
-  return p.splits == 1 ? 0 : (size_t)p.splits * B * T * q_heads * (bank->dim + 2) * sizeof(float);
+  return p.splits == 1 ? 0 : (size_t)p.splits * B * T * q_heads * (bank->dim * sizeof(float) + sizeof(f2v));
 }
 
 template <int DT, int BITS, int D>
 static void launch_attend(const Plan& p, const gpsr_bank& bk, const int32_t* table, int B, int table_pages, const int32_t* length,
                           const void* q, int T, int G, Strides qs, bool qwide, float scale, const int32_t* skip, void* out,
-                          float* lse, float* part, hipStream_t st) {
+                          float* lse, void* ws, hipStream_t st) {
   typedef typename Row<DT>::T E;
+  float* sums = (float*)ws;          // every row a multiple of 128 bytes: the statistics behind them stay aligned
+  f2v* stats = (f2v*)(sums + (size_t)p.splits * B * T * G * bk.heads * D);
   constexpr int NT = Terms<DT>::N, NW = many_nw(D, NT);
   const int pshift = __builtin_ctz((unsigned)bk.page_rows);
   const dim3 grid((unsigned)(p.groups * p.splits), (unsigned)bk.heads, (unsigned)B);
 #define ATTEND(W, NW_, WK, KT, NB, AHEAD) hipLaunchKernelGGL((k_bank_attend<DT, BITS, D, W, NW_, WK, KT, NB, AHEAD>), grid, \
-    dim3(64 * NW_), 0, st, bk, table, table_pages, pshift, length, (const E*)q, T, G, qs, qwide, scale, skip, (E*)out, lse, p.splits, part)
+    dim3(64 * NW_), 0, st, bk, table, table_pages, pshift, length, (const E*)q, T, G, qs, qwide, scale, skip, (E*)out, lse, p.splits, sums, stats)
   if (p.few && (int64_t)T * G <= 16) ATTEND(16, 4, 4, 128, 2, few_ahead(D, BITS, NT));
   else if (p.few) ATTEND(32, 4, 4, 128, 1, 1);
   else ATTEND(32, NW, 1, many_kt(D, NT), many_nb(D, NT), 1);
 #undef ATTEND
   if (p.splits > 1) {
     const int64_t C = (int64_t)T * G;
-    hipLaunchKernelGGL((k_bank_join<DT, D>), dim3((unsigned)((C + 3) / 4), (unsigned)bk.heads, (unsigned)B), dim3(256), 0, st, part,
-                       T, G, bk.heads, C, p.splits, (size_t)p.splits * C, (size_t)1, (size_t)G, (size_t)C,
+    hipLaunchKernelGGL((k_bank_join<DT, D, float>), dim3((unsigned)((C + 3) / 4), (unsigned)bk.heads, (unsigned)B), dim3(256), 0, st, sums,
+                       stats, T, G, bk.heads, C, p.splits, (size_t)p.splits * C, (size_t)1, (size_t)G, (size_t)C,
                        (E*)out, lse);
   }
 }
@@ -191,7 +194,7 @@ extern "C" int gpsr_bank_attend(const gpsr_bank* bank, const int32_t* table, int
   const int G = q_heads / bank->heads;
   hipStream_t st = (hipStream_t)stream;
 #define ATTEND(DT, BITS, D) launch_attend<DT, BITS, D>(p, *bank, table, B, table_pages, length, q, T, G, qs, wide, scale, skip, \
-                                                       out, lse, (float*)workspace, st)
+                                                       out, lse, workspace, st)
   BANK_DISPATCH(ATTEND, dtype, bank->bits, bank->dim);
 #undef ATTEND
   CHECK_LAUNCH("k_bank_attend");

@@ -16,7 +16,7 @@ __global__ void __launch_bounds__(256, 2)
 k_bank_pages_query(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, int pshift, const int32_t* __restrict__ length,
                    const typename Row<DT>::T* __restrict__ q, int T, int G, Strides qs, bool qwide, const int32_t* __restrict__ sel,
                    int n_sel, float scale, const int32_t* __restrict__ skip, typename Row<DT>::T* __restrict__ out,
-                   float* __restrict__ lse, int groups, int splits, float* __restrict__ partials) {
+                   float* __restrict__ lse, int groups, int splits, float* __restrict__ sums, f2v* __restrict__ stats) {
   typedef Geo<W> X;
   constexpr int NT = Terms<DT>::N, KT = 128, NB = 32 / W;
   __shared__ __attribute__((aligned(16))) char sm[tile_lds(D, KT)];
@@ -97,7 +97,8 @@ k_bank_pages_query(gpsr_bank bk, const int32_t* __restrict__ table, int table_pa
     st.template store<DT>(out + (((size_t)b * T + t) * (size_t)(H * G) + hq) * D, part);
     if (lse && part == 0) lse[((size_t)b * (H * G) + hq) * T + t] = st.lse();
   } else {
-    st.store_partial(partials + ((((size_t)(b * H + h) * T + t) * splits + split) * G + g) * (D + 2), part);
+    const size_t at = (((size_t)(b * H + h) * T + t) * splits + split) * G + g;
+    st.store_partial(sums + at * D, stats + at, part);
   }
 }
 
@@ -109,8 +110,8 @@ k_bank_pages_query(gpsr_bank bk, const int32_t* __restrict__ table, int table_pa
 #define PG_BUCKETS 16384      // of one entry: 64 KB of LDS
 __global__ void __launch_bounds__(512)
 k_bank_pages_count(const int32_t* __restrict__ sel, int n_sel, const int32_t* __restrict__ table, int table_pages, int64_t pages,
-                   int pshift, const int32_t* __restrict__ length, int T, int H, int G, int D2, int chunks, int* __restrict__ hist,
-                   int* __restrict__ rank, float* __restrict__ part) {
+                   int pshift, const int32_t* __restrict__ length, int T, int H, int G, int chunks, int* __restrict__ hist,
+                   int* __restrict__ rank, f2v* __restrict__ stats) {
   extern __shared__ int mine[];
   const int b = blockIdx.y, tid = threadIdx.x, buckets = H * table_pages;
   const int64_t per = (int64_t)T * H * n_sel, e0 = (int64_t)blockIdx.x * PG_CHUNK;
@@ -128,7 +129,7 @@ k_bank_pages_count(const int32_t* __restrict__ sel, int n_sel, const int32_t* __
     for (int k = 1; k <= s; ++k) ok &= s0[e - k] != lp;      // all of them, so that the loads do not wait for each other
     rank[b * per + e] = ok ? atomicAdd(&mine[h * table_pages + lp], 1) : -1;
     if (!ok)      // the join passes over partials whose sum of weights is 0
-      for (int g = 0; g < G; ++g) part[(((((size_t)b * H + h) * T + th / H) * n_sel + s) * G + g) * D2 + D2 - 1] = 0.f;
+      for (int g = 0; g < G; ++g) stats[((((size_t)b * H + h) * T + th / H) * n_sel + s) * G + g] = f2v{0.f, 0.f};
   }
   __syncthreads();
   int* to = hist + ((size_t)b * chunks + blockIdx.x) * buckets;
@@ -155,9 +156,11 @@ k_bank_pages_shares(int* __restrict__ hist, int buckets, int chunks, int* __rest
   count[(size_t)b * buckets + i] = sum;
 }
 
-// exclusive sums of the counts and of the workgroups that each bucket needs; one workgroup
+// exclusive sums of the counts and of the workgroups that each bucket needs, and each workgroup's bucket (found by bisection
+// over the sums instead, it was a third of the 66 us of the product kernel); one workgroup
 __global__ void __launch_bounds__(1024)
-k_bank_pages_scan(const int* __restrict__ count, int buckets, int G, int cw, int* __restrict__ start, int* __restrict__ wgs) {
+k_bank_pages_scan(const int* __restrict__ count, int buckets, int G, int cw, int* __restrict__ start, int* __restrict__ wgs,
+                  int* __restrict__ owner) {
   __shared__ int sc[16], sw[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_of(tid);
   const int per = (buckets + 1023) / 1024;
@@ -176,7 +179,8 @@ k_bank_pages_scan(const int* __restrict__ count, int buckets, int G, int cw, int
   for (int i = i0; i < i1; ++i) {
     start[i] = oc; wgs[i] = ow;
     const int n = count[i];
-    oc += n; ow += (int)(((int64_t)n * G + cw - 1) / cw);
+    oc += n;
+    for (int k = (int)(((int64_t)n * G + cw - 1) / cw); k > 0; --k) owner[ow++] = i;
   }
   if (tid == 1023) { start[buckets] = pc; wgs[buckets] = pw; }
 }
@@ -195,21 +199,27 @@ k_bank_pages_fill(const int32_t* __restrict__ sel, int n_sel, int table_pages, i
   list[start[(size_t)b * buckets + bucket] + share + r] = (int)(th / H * n_sel + (e - th * n_sel));
 }
 
+// What a partial is kept in: bf16 outputs take f16 (11 bits against the 8 that the result has), scaled by a power of two so
+// that the largest of its columns is between 1 and 2, which goes into its reference; half the bytes to write and read again.
+template <int DT> struct Partial { typedef float T; };
+template <> struct Partial<GPSR_BF16> { typedef _Float16 T; };
+static constexpr int page_lds(int d, int kt) { return tile_lds(d, kt) > 256 * (d + 4) ? tile_lds(d, kt) : 256 * (d + 4); }
+
 template <int DT, int BITS, int D, int KT>
-__global__ void __launch_bounds__(256, tile_waves(D, Terms<DT>::N, KT / 32))
+__global__ void __launch_bounds__(256, tile_regs(D, Terms<DT>::N, KT / 32) <= 144 ? 3 : tile_waves(D, Terms<DT>::N, KT / 32))
 k_bank_pages_page(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, int pshift, const int32_t* __restrict__ length,
                   const typename Row<DT>::T* __restrict__ q, int T, int G, Strides qs, bool qwide, int n_sel, float scale,
                   const int32_t* __restrict__ skip, const int* __restrict__ start, const int* __restrict__ wgs, int buckets,
-                  const int* __restrict__ list, float* __restrict__ partials) {
+                  const int* __restrict__ owner, const int* __restrict__ list, typename Partial<DT>::T* __restrict__ sums,
+                  f2v* __restrict__ stats) {
   constexpr int NT = Terms<DT>::N, NB = KT / 32, CW = 128, W = 32;
   typedef Geo<W> X;
-  __shared__ __attribute__((aligned(16))) char sm[tile_lds(D, KT)];
+  __shared__ __attribute__((aligned(16))) char sm[page_lds(D, KT)];
   Tile<D, KT> tile(sm);
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_of(tid), part = lane / W, col = lane % W;
   const int w = blockIdx.x;
+  const int a = owner[w];                 // of a workgroup behind the last one: whatever the memory held, and not used
   if (w >= wgs[buckets]) return;
-  int a = 0, z = buckets;                 // the last bucket whose first workgroup is not behind this one
-  while (z - a > 1) { const int mid = (a + z) >> 1; if (wgs[mid] <= w) a = mid; else z = mid; }
   const int lp = a % table_pages, H = bk.heads, P = 1 << pshift;
   const int bh = a / table_pages, h = bh % H, b = bh / H;
   const int n = start[a + 1] - start[a];
@@ -252,12 +262,47 @@ k_bank_pages_page(gpsr_bank bk, const int32_t* __restrict__ table, int table_pag
     tile_accumulate<D, KT, NT, NB, W, true>(tile, 0, col, part, c2, s, st);
   }
   st.spoil();
-  if (there) st.store_partial(partials + (((size_t)bh * T * n_sel + id) * G + g) * (D + 2), part);
+  const size_t at = ((size_t)bh * T * n_sel + id) * G + g;
+  if constexpr (DT != GPSR_BF16) {
+    if (there) st.store_partial(sums + at * D, stats + at, part);
+  } else {
+    float big = 0.f;
+#pragma unroll
+    for (int d = 0; d < D / W; ++d)
+#pragma unroll
+      for (int e = 0; e < X::E; ++e) big = fmaxf(big, fabsf(st.o[d][e]));
+    big = X::parts(big, max2);
+    const int ex = big > 0.f && big < __builtin_inff() ? __builtin_amdgcn_frexp_expf(big) - 1 : 0;
+    // through LDS, so that a row leaves in whole cache lines: stored from the accumulators, 32 bytes of 32 rows at a time, the
+    // stores were a third of the kernel
+    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+    _Float16* mine = (_Float16*)sm + wave * (32 * (D + 4));
+    __syncthreads();
+#pragma unroll
+    for (int d = 0; d < D / W; ++d)
+#pragma unroll
+      for (int e = 0; e < X::E; e += 4) {
+        h4 y;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = (_Float16)ldexpf(st.o[d][e + j], -ex);
+        *(h4*)(mine + col * (D + 4) + d * W + X::row(part, e)) = y;
+      }
+    const float all = X::parts(st.l, add2);
+    if (there && part == 0) stats[at] = f2v{st.m + (float)ex, ldexpf(all, -ex)};
+    __syncthreads();
+    constexpr int PER = D / 4;             // lanes for a row
+#pragma unroll 4
+    for (int i = lane; i < 32 * PER; i += 64) {
+      const int r = i / PER;
+      const size_t to = __shfl(at, r);
+      if (__shfl((int)there, r)) *(h4*)(sums + to * D + i % PER * 4) = *(const h4*)(mine + r * (D + 4) + i % PER * 4);
+    }
+  }
 }
 
 // ---------------------------------------------------------------- host
-struct PagesPlan { bool by_page; int groups, splits, chunks; int64_t entries, buckets, most_wgs; size_t hist, rank, start, wgs, list, part, bytes; };
-static PagesPlan plan_of(const gpsr_bank* bk, int B, int table_pages, int T, int q_heads, int n_sel) {
+struct PagesPlan { bool by_page; int groups, splits, chunks; int64_t entries, buckets, most_wgs; size_t hist, rank, start, wgs, owner, list, stats, sums, bytes; };
+static PagesPlan plan_of(const gpsr_bank* bk, int B, int table_pages, int T, int q_heads, int n_sel, int dtype) {
   PagesPlan p = {};
   const int H = bk->heads, G = q_heads / H;
   p.entries = (int64_t)B * T * H * n_sel;
@@ -273,8 +318,10 @@ static PagesPlan plan_of(const gpsr_bank* bk, int B, int table_pages, int T, int
     p.rank = at; at += align256((size_t)p.entries * 4);
     p.start = at; at += align256((size_t)(p.buckets + 1) * 4);
     p.wgs = at; at += align256((size_t)(p.buckets + 1) * 4);
+    p.owner = at; at += align256((size_t)p.most_wgs * 4);
     p.list = at; at += align256((size_t)p.entries * 4);
-    p.part = at; at += (size_t)p.entries * G * (bk->dim + 2) * sizeof(float);
+    p.stats = at; at += align256((size_t)p.entries * G * sizeof(f2v));
+    p.sums = at; at += (size_t)p.entries * G * bk->dim * (dtype == GPSR_BF16 ? 2 : 4);
     p.bytes = at;
   } else {
     const int width = G <= 16 ? 16 : 32;
@@ -283,14 +330,14 @@ static PagesPlan plan_of(const gpsr_bank* bk, int B, int table_pages, int T, int
     int64_t s = 512 / wgs;
     if (s < 1) s = 1;
     p.splits = (int)(s > tiles ? tiles : s);
-    if (p.splits > 1) p.bytes = (size_t)p.splits * B * T * q_heads * (bk->dim + 2) * sizeof(float);
+    if (p.splits > 1) p.bytes = (size_t)p.splits * B * T * q_heads * (bk->dim * sizeof(float) + sizeof(f2v));
   }
   return p;
 }
 
 extern "C" size_t gpsr_bank_attend_pages_workspace_bytes(const gpsr_bank* bank, int B, int table_pages, int T, int q_heads, int n_sel, int dtype) {
   if (bank_wrong(bank) || B <= 0 || T <= 0 || table_pages < 0 || q_heads < 1 || q_heads % bank->heads || n_sel < 1 || n_sel > 64 || !type_ok(dtype)) return 0;
-  return plan_of(bank, B, table_pages, T, q_heads, n_sel).bytes;
+  return plan_of(bank, B, table_pages, T, q_heads, n_sel, dtype).bytes;
 }
 
 template <int DT, int BITS, int D>
@@ -302,33 +349,37 @@ static void launch_pages(const PagesPlan& p, const gpsr_bank& bk, const int32_t*
   const int64_t C = (int64_t)T * G;
   const dim3 join((unsigned)((C + 3) / 4), (unsigned)H, (unsigned)B);
   if (!p.by_page) {
-    float* part = (float*)ws;
+    float* sums = (float*)ws;
+    f2v* stats = (f2v*)(sums + (size_t)p.splits * B * T * q_heads * D);
 #define QUERY(W) hipLaunchKernelGGL((k_bank_pages_query<DT, BITS, D, W>), dim3((unsigned)((int64_t)T * p.groups * p.splits), (unsigned)H, \
     (unsigned)B), dim3(256), 0, st, bk, table, table_pages, pshift, length, (const E*)q, T, G, qs, qwide, sel, n_sel, scale, skip, (E*)out, \
-    lse, p.groups, p.splits, part)
+    lse, p.groups, p.splits, sums, stats)
     if (G <= 16) QUERY(16); else QUERY(32);
 #undef QUERY
     if (p.splits > 1)
-      hipLaunchKernelGGL((k_bank_join<DT, D>), join, dim3(256), 0, st, part, T, G, H, C, p.splits, (size_t)p.splits * C, (size_t)1,
+      hipLaunchKernelGGL((k_bank_join<DT, D, float>), join, dim3(256), 0, st, sums, stats, T, G, H, C, p.splits, (size_t)p.splits * C, (size_t)1,
                          (size_t)p.splits * G, (size_t)G, (E*)out, lse);
     return;
   }
   int *count = (int*)ws, *rank = (int*)(ws + p.rank), *start = (int*)(ws + p.start), *wgs = (int*)(ws + p.wgs), *list = (int*)(ws + p.list);
-  float* part = (float*)(ws + p.part);
+  typedef typename Partial<DT>::T P;
+  P* sums = (P*)(ws + p.sums);
+  f2v* stats = (f2v*)(ws + p.stats);
+  int* owner = (int*)(ws + p.owner);
   const int64_t per = (int64_t)T * H * n_sel;
   const int buckets = H * table_pages;
   int* hist = (int*)(ws + p.hist);
   hipLaunchKernelGGL(k_bank_pages_count, dim3((unsigned)p.chunks, (unsigned)B), dim3(512), (size_t)buckets * 4, st, sel, n_sel, table,
-                     table_pages, bk.pages, pshift, length, T, H, G, D + 2, p.chunks, hist, rank, part);
+                     table_pages, bk.pages, pshift, length, T, H, G, p.chunks, hist, rank, stats);
   hipLaunchKernelGGL(k_bank_pages_shares, dim3((unsigned)((buckets + 63) / 64), (unsigned)B), dim3(64), 0, st, hist, buckets, p.chunks, count);
-  hipLaunchKernelGGL(k_bank_pages_scan, dim3(1), dim3(1024), 0, st, count, (int)p.buckets, G, 128, start, wgs);
+  hipLaunchKernelGGL(k_bank_pages_scan, dim3(1), dim3(1024), 0, st, count, (int)p.buckets, G, 128, start, wgs, owner);
   hipLaunchKernelGGL(k_bank_pages_fill, dim3((unsigned)((per + 255) / 256), (unsigned)B), dim3(256), 0, st, sel, n_sel, table_pages, T,
                      H, p.chunks, hist, rank, start, list);
 #define PAGE(KT) hipLaunchKernelGGL((k_bank_pages_page<DT, BITS, D, KT>), dim3((unsigned)p.most_wgs), dim3(256), 0, st, bk, table, \
-    table_pages, pshift, length, (const E*)q, T, G, qs, qwide, n_sel, scale, skip, start, wgs, (int)p.buckets, list, part)
+    table_pages, pshift, length, (const E*)q, T, G, qs, qwide, n_sel, scale, skip, start, wgs, (int)p.buckets, owner, list, sums, stats)
   if (bk.page_rows <= 32) PAGE(32); else PAGE(64);
 #undef PAGE
-  hipLaunchKernelGGL((k_bank_join<DT, D>), join, dim3(256), 0, st, part, T, G, H, C, n_sel, (size_t)n_sel * C, (size_t)1,
+  hipLaunchKernelGGL((k_bank_join<DT, D, P>), join, dim3(256), 0, st, sums, stats, T, G, H, C, n_sel, (size_t)n_sel * C, (size_t)1,
                      (size_t)n_sel * G, (size_t)G, (E*)out, lse);
 }
 
@@ -340,7 +391,7 @@ extern "C" int gpsr_bank_attend_pages(const gpsr_bank* bank, const int32_t* tabl
   if (const char* w = attend_wrong(bank, table, B, table_pages, length, q, dtype, q_heads, qst, scale, out)) return arg_fail(w);
   if (!sel) return arg_fail("bank_attend_pages: null pointer");
   if (n_sel < 1 || n_sel > 64) return arg_fail("bank_attend_pages: n_sel must be in 1..64");
-  const PagesPlan p = plan_of(bank, B, table_pages, T, q_heads, n_sel);
+  const PagesPlan p = plan_of(bank, B, table_pages, T, q_heads, n_sel, dtype);
   if (p.by_page ? p.most_wgs > 0x7fffffff : (int64_t)T * p.groups * p.splits > 0x7fffffff)
     return arg_fail("bank_attend_pages: too many queries for one call");
   if (workspace_bytes < p.bytes || (p.bytes && !workspace)) return arg_fail("workspace too small");

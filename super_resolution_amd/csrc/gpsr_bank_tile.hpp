@@ -283,8 +283,6 @@ __device__ __forceinline__ void tile_logits(const Tile<D, KT>& tile, int r0, int
   }
 }
 
-typedef float f4u __attribute__((ext_vector_type(4), aligned(8)));     // partial results: rows of D + 2 floats
-
 // ---- running softmax of a wave's columns: m the power of two that weights are taken against (logit * log2 e; -inf: no row
 // seen), l this part's sum of weights, o = sum of weights * values
 template <int D, int W>
@@ -373,15 +371,14 @@ struct Soft {
         }
       }
   }
-  // [D] sums, reference, sum of weights
-  __device__ __forceinline__ void store_partial(float* __restrict__ p, int part) const {
+  // a partial result: sums [D], and the reference and the sum of weights
+  __device__ __forceinline__ void store_partial(float* __restrict__ p, f2v* __restrict__ stat, int part) const {
     const float all = X::parts(l, add2);
 #pragma unroll
     for (int d = 0; d < D / W; ++d)
 #pragma unroll
-      for (int e = 0; e < X::E; e += 4)
-        *(f4u*)(p + d * W + X::row(part, e)) = f4u{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
-    if (part == 0) *(f2v*)(p + D) = f2v{m, all};
+      for (int e = 0; e < X::E; e += 4) *(f4v*)(p + d * W + X::row(part, e)) = f4v{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
+    if (part == 0) *stat = f2v{m, all};
   }
 };
 
@@ -453,22 +450,23 @@ __device__ __forceinline__ void tile_accumulate(const Tile<D, KT>& tile, int r0,
 
 // Joins the partial results of one column, at most 64: one wave per column.  First lane i weighs partial i, then the lanes
 // spread over the dim and eight partials are on their way at a time (with the weights formed along the way each load waited for
-// the one before it: 30 against 9 us for 64 partials of 96 columns).  Column (t, g) of bank head bh has its n partials [D + 2]
-// at bh * per_bh + t * per_t + g * per_g + i * per_i.
-template <int DT, int D>
+// the one before it: 30 against 9 us for 64 partials of 96 columns).  Column (t, g) of bank head bh has its n partials at
+// numbers bh * per_bh + t * per_t + g * per_g + i * per_i.
+template <int DT, int D, class P>
 __global__ void __launch_bounds__(256)
-k_bank_join(const float* __restrict__ part, int T, int G, int H, int64_t C, int n, size_t per_bh, size_t per_g, size_t per_t,
-            size_t per_i, typename Row<DT>::T* __restrict__ out, float* __restrict__ lse) {
+k_bank_join(const P* __restrict__ sums, const f2v* __restrict__ stats, int T, int G, int H, int64_t C, int n, size_t per_bh,
+            size_t per_g, size_t per_t, size_t per_i, typename Row<DT>::T* __restrict__ out, float* __restrict__ lse) {
   const int lane = threadIdx.x & 63;
-  const int64_t c = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t c = (int64_t)blockIdx.x * 4 + wave_of(threadIdx.x);
   if (c >= C) return;
   const int h = blockIdx.y, b = blockIdx.z;
   const int64_t t = c / G;
   const int g = (int)(c - t * G), hq = h * G + g;
-  const float* p = part + ((size_t)(b * H + h) * per_bh + t * per_t + g * per_g) * (D + 2);
-  const size_t step = per_i * (D + 2);
+  const size_t at = (size_t)(b * H + h) * per_bh + t * per_t + g * per_g;
+  const P* p = sums + at * D;
+  const size_t step = per_i * D;
   float m = -__builtin_inff(), l = 0.f;
-  if (lane < n) { l = p[lane * step + D + 1]; m = p[lane * step + D]; }
+  if (lane < n) { const f2v x = stats[at + lane * per_i]; m = x.x; l = x.y; }
   const unsigned long long used = __ballot(l != 0.f);      // the others saw nothing, and their sums were not written
   float top = l != 0.f ? m : -__builtin_inff();
   for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
@@ -482,7 +480,7 @@ k_bank_join(const float* __restrict__ part, int T, int G, int H, int64_t C, int 
 #pragma unroll
     for (int j = 0; j < 8; ++j)
 #pragma unroll
-      for (int e = 0; e < E; ++e) y[j][e] = p[min(i0 + j, n - 1) * step + min(e * 64 + lane, D - 1)];
+      for (int e = 0; e < E; ++e) y[j][e] = (float)p[min(i0 + j, n - 1) * step + min(e * 64 + lane, D - 1)];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const bool use = used >> (i0 + j) & 1;
