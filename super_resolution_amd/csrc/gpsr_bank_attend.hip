@@ -5,10 +5,11 @@
 
 // ---------------------------------------------------------------- attention over the whole bank
 // Columns are the (query, head) pairs that share a bank head.  A workgroup of NW waves walks the rows of its split of the
-// bank, KT at a time: all threads decode the tile to LDS once, then each wave multiplies it with its own W columns, NB x W
-// rows at a time.
-//   WK = 1: each wave has columns of its own (many queries; bound by the exponentials and the matrix units)
-//   WK = NW: all have the same columns and a share of the tile's rows each (few queries; bound by reading the bank)
+// bank, KT at a time, NB x W of them in one step:
+//   WK = 1 (many queries; bound by the exponentials and the matrix units): all threads decode a tile to LDS once, then each
+//     wave multiplies it with W columns of its own;
+//   WK = NW (few queries; bound by reading the bank): all waves have the same columns, each walks every NW-th tile in LDS of its
+//     own, so that none waits for another, and the results are joined at the end.
 // AHEAD: tiles under way besides the one in LDS.
 template <int DT, int BITS, int D, int W, int NW, int WK, int KT, int NB, int AHEAD>
 __global__ void __launch_bounds__(64 * NW, WK > 1 ? 2 : tile_waves(D, Terms<DT>::N, NB))
@@ -17,15 +18,15 @@ k_bank_attend(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, 
               const int32_t* __restrict__ skip, typename Row<DT>::T* __restrict__ out, float* __restrict__ lse, int splits,
               float* __restrict__ sums, f2v* __restrict__ stats) {
   typedef Geo<W> X;
-  constexpr int NT = Terms<DT>::N, KW = KT / WK;                 // rows of one wave
-  constexpr int CW = (NW / WK) * W;                              // columns of the workgroup
-  __shared__ __attribute__((aligned(16))) char sm[tile_lds(D, KT)];
-  Tile<D, KT> tile(sm);
+  constexpr int NT = Terms<DT>::N, CW = (NW / WK) * W;           // columns of the workgroup
+  constexpr int TH = WK > 1 ? 64 : 64 * NW;                      // threads that share a tile
+  __shared__ __attribute__((aligned(16))) char sm[WK * tile_lds(D, KT)];
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_of(tid), part = lane / W, col = lane % W;
+  const int sid = WK > 1 ? lane : tid;
+  Tile<D, KT> tile(sm + (WK > 1 ? wave * tile_lds(D, KT) : 0));
   const int h = blockIdx.y, b = blockIdx.z, H = bk.heads;
   const int split = blockIdx.x % splits;
   const int64_t C = (int64_t)T * G, c = (int64_t)(blockIdx.x / splits) * CW + (WK == 1 ? wave * W : 0) + col;
-  const int wrow = WK == 1 ? 0 : wave * KW;                      // first row of this wave within a tile
 
   unsigned len = (unsigned)max(length[b], 0);
   const int64_t most = (int64_t)table_pages << pshift;
@@ -48,22 +49,24 @@ k_bank_attend(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, 
   Soft<D, W> st;
   const float c2 = scale * 1.4426950408889634f;
 
-  tile.clear_marks(tid, 64 * NW);
-  Fetch<BITS, D, KT, 64 * NW> f[AHEAD];
+  tile.clear_marks(sid, TH);
+  Fetch<BITS, D, KT, TH> f[AHEAD];
   const WholeBank rows = {table + (size_t)b * table_pages, bk.pages, pshift, len};
+  // between the accesses to a tile: LDS serves one wave in order, only the compiler has to be kept from moving them
+  const auto sync = [] { if constexpr (WK > 1) { asm volatile("" ::: "memory"); __builtin_amdgcn_wave_barrier(); } else __syncthreads(); };
   const auto step = [&](unsigned i, auto& f, auto move) {
-    __syncthreads();
-    f.template store<W>(tile, tid, i + 1);
-    __syncthreads();
-    f.codes(bk, h, pshift, (i + AHEAD) * KT, tid);
-    f.pages(rows, (i + 2 * AHEAD) * KT, tid);
-    const unsigned p0 = i * KT + wrow;
-    tile_marks<D, KT, KW>(tile, wrow, i + 1, st, [&](int r) { return !(p0 + r >= lo && p0 + r < hi); });
-    const bool skips = skip && __ballot(lo < p0 + KW && hi > p0 && lo < hi);
+    sync();
+    f.template store<W>(tile, sid, i + 1);
+    sync();
+    f.codes(bk, h, pshift, (i + WK * AHEAD) * KT, sid);
+    f.pages(rows, (i + 2 * WK * AHEAD) * KT, sid);
+    const unsigned p0 = i * KT;
+    tile_marks<D, KT, KT>(tile, 0, i + 1, st, [&](int r) { return !(p0 + r >= lo && p0 + r < hi); });
+    const bool skips = skip && __ballot(lo < p0 + KT && hi > p0 && lo < hi);
 #pragma unroll 1
-    for (int r = 0; r < KW; r += W * NB) {
+    for (int r = 0; r < KT; r += W * NB) {
       typename X::Acc s[NB];
-      tile_logits<D, KT, NT, NB, W>(tile, wrow + r, col, part, qf, s);
+      tile_logits<D, KT, NT, NB, W>(tile, r, col, part, qf, s);
       if (skips) {
         asm volatile("");        // not to be computed for the tiles that nobody skips
 #pragma unroll
@@ -74,22 +77,23 @@ k_bank_attend(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, 
             if (pos >= lo && pos < hi) s[kb][e] = -__builtin_inff();
           }
       }
-      tile_accumulate<D, KT, NT, NB, W, decltype(move)::value>(tile, wrow + r, col, part, c2, s, st);
+      tile_accumulate<D, KT, NT, NB, W, decltype(move)::value>(tile, r, col, part, c2, s, st);
     }
   };
   st.clear();
   for (bool safe = WK > 1; i0 < i1; safe = true) {
+    const unsigned first = i0 + (WK > 1 ? wave : 0);
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a) {
-      f[a].pages(rows, (i0 + a) * KT, tid);
-      f[a].codes(bk, h, pshift, (i0 + a) * KT, tid);
-      f[a].pages(rows, (i0 + AHEAD + a) * KT, tid);
+      f[a].pages(rows, (first + WK * a) * KT, sid);
+      f[a].codes(bk, h, pshift, (first + WK * a) * KT, sid);
+      f[a].pages(rows, (first + WK * (AHEAD + a)) * KT, sid);
     }
     if constexpr (WK > 1) {
-      for (unsigned i = i0; i < i1; i += AHEAD)
+      for (unsigned i = first; i < i1; i += WK * AHEAD)
 #pragma unroll
         for (int a = 0; a < AHEAD; ++a)
-          if (i + a < i1) step(i + a, f[a], std::true_type());
+          if (i + WK * a < i1) step(i + WK * a, f[a], std::true_type());
       break;
     } else {
       static_assert(AHEAD == 1, "one tile under way");
@@ -135,15 +139,17 @@ static Plan plan_of(const gpsr_bank* bk, int B, int table_pages, int T, int q_he
   const int nt = dtype == GPSR_BF16 ? 1 : dtype == GPSR_F16 ? 2 : 3, nw = many_nw(bk->dim, nt);
   p.few = C <= 32;
   p.cw = p.few ? 32 : 32 * nw;
-  p.kt = p.few ? 128 : many_kt(bk->dim, nt);
+  p.kt = p.few ? 32 : many_kt(bk->dim, nt);
   p.groups = (C + p.cw - 1) / p.cw;
   const int64_t tiles = (((int64_t)table_pages * bk->page_rows) + p.kt - 1) / p.kt;
-  // the splits that end soonest when `slots` workgroups run at a time, each paying for 2 tiles besides its own
+  // The splits that end soonest when `slots` workgroups run at a time, each paying for `own` tiles besides its share, and the join
+  // for some more.
   const int64_t slots = p.few ? 512 : 256 * 4 * tile_waves(bk->dim, nt, many_nb(bk->dim, nt)) / nw, wgs = p.groups * bk->heads * B;
+  const int step = p.few ? 4 : 1, own = p.few ? 4 : 2;           // tiles that a workgroup takes at once
   int64_t best = -1;
   p.splits = 1;
-  for (int s = 1; s <= 64 && s <= (tiles > 1 ? tiles : 1); ++s) {
-    const int64_t cost = ((wgs * s + slots - 1) / slots) * ((tiles + s - 1) / s + 2) + (s > 1 ? 2 + s / 4 : 0);
+  for (int s = 1; s <= 64 && s * step <= (tiles > step ? tiles + step - 1 : step); ++s) {
+    const int64_t cost = ((wgs * s + slots - 1) / slots) * ((tiles + s * step - 1) / (s * step) + own) + (s > 1 ? 2 + s / 4 : 0);
     if (best < 0 || cost < best) { best = cost; p.splits = s; }
   }
   return p;
@@ -167,8 +173,8 @@ static void launch_attend(const Plan& p, const gpsr_bank& bk, const int32_t* tab
   const dim3 grid((unsigned)(p.groups * p.splits), (unsigned)bk.heads, (unsigned)B);
 #define ATTEND(W, NW_, WK, KT, NB, AHEAD) hipLaunchKernelGGL((k_bank_attend<DT, BITS, D, W, NW_, WK, KT, NB, AHEAD>), grid, \
     dim3(64 * NW_), 0, st, bk, table, table_pages, pshift, length, (const E*)q, T, G, qs, qwide, scale, skip, (E*)out, lse, p.splits, sums, stats)
-  if (p.few && (int64_t)T * G <= 16) ATTEND(16, 4, 4, 128, 2, few_ahead(D, BITS, NT));
-  else if (p.few) ATTEND(32, 4, 4, 128, 1, 1);
+  if (p.few && (int64_t)T * G <= 16) ATTEND(16, 4, 4, 32, 2, few_ahead(D, BITS, NT));
+  else if (p.few) ATTEND(32, 4, 4, 32, 1, 1);
   else ATTEND(32, NW, 1, many_kt(D, NT), many_nb(D, NT), 1);
 #undef ATTEND
   if (p.splits > 1) {

@@ -205,14 +205,16 @@ template <int DT> struct Partial { typedef float T; };
 template <> struct Partial<GPSR_BF16> { typedef _Float16 T; };
 static constexpr int page_lds(int d, int kt) { return tile_lds(d, kt) > 256 * (d + 4) ? tile_lds(d, kt) : 256 * (d + 4); }
 
+// 32 rows at a time and three waves per SIMD: the workgroups are short and mostly wait (62 us; all 64 rows of a page at a time 66, two
+// waves 76 and 79, four waves with spills 90)
 template <int DT, int BITS, int D, int KT>
-__global__ void __launch_bounds__(256, tile_regs(D, Terms<DT>::N, KT / 32) <= 144 ? 3 : tile_waves(D, Terms<DT>::N, KT / 32))
+__global__ void __launch_bounds__(256, tile_waves(D, Terms<DT>::N, 1) > 3 ? 3 : tile_waves(D, Terms<DT>::N, 1))
 k_bank_pages_page(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, int pshift, const int32_t* __restrict__ length,
                   const typename Row<DT>::T* __restrict__ q, int T, int G, Strides qs, bool qwide, int n_sel, float scale,
                   const int32_t* __restrict__ skip, const int* __restrict__ start, const int* __restrict__ wgs, int buckets,
                   const int* __restrict__ owner, const int* __restrict__ list, typename Partial<DT>::T* __restrict__ sums,
                   f2v* __restrict__ stats) {
-  constexpr int NT = Terms<DT>::N, NB = KT / 32, CW = 128, W = 32;
+  constexpr int NT = Terms<DT>::N, NB = 1, CW = 128, W = 32;
   typedef Geo<W> X;
   __shared__ __attribute__((aligned(16))) char sm[page_lds(D, KT)];
   Tile<D, KT> tile(sm);
@@ -247,19 +249,20 @@ k_bank_pages_page(gpsr_bank bk, const int32_t* __restrict__ table, int table_pag
     f.pages(rows, v + KT, tid);
     f.codes(bk, h, pshift, v + KT, tid);
     tile_marks<D, KT, KT>(tile, 0, v / KT + 1, st, [&](int r) { return !(pos0 + v + r >= lo && pos0 + v + r < hi); });
-    typename X::Acc s[NB];
-    tile_logits<D, KT, NT, NB, W>(tile, 0, col, part, qf, s);
-    if (skip && __ballot(lo < pos0 + v + KT && hi > pos0 + v && lo < hi)) {
-      asm volatile("");
-#pragma unroll
-      for (int kb = 0; kb < NB; ++kb)
+#pragma unroll 1
+    for (int r = 0; r < KT; r += 32) {
+      typename X::Acc s[NB];
+      tile_logits<D, KT, NT, NB, W>(tile, r, col, part, qf, s);
+      if (skip && __ballot(lo < pos0 + v + KT && hi > pos0 + v && lo < hi)) {
+        asm volatile("");
 #pragma unroll
         for (int e = 0; e < X::E; ++e) {
-          const int64_t pos = pos0 + v + kb * W + X::row(part, e);
-          if (pos >= lo && pos < hi) s[kb][e] = -__builtin_inff();
+          const int64_t pos = pos0 + v + r + X::row(part, e);
+          if (pos >= lo && pos < hi) s[0][e] = -__builtin_inff();
         }
+      }
+      tile_accumulate<D, KT, NT, NB, W, true>(tile, r, col, part, c2, s, st);
     }
-    tile_accumulate<D, KT, NT, NB, W, true>(tile, 0, col, part, c2, s, st);
   }
   st.spoil();
   const size_t at = ((size_t)bh * T * n_sel + id) * G + g;

@@ -449,8 +449,8 @@ __device__ __forceinline__ void tile_accumulate(const Tile<D, KT>& tile, int r0,
 }
 
 // Joins the partial results of one column, at most 64: one wave per column.  First lane i weighs partial i, then the lanes
-// spread over the dim and eight partials are on their way at a time (with the weights formed along the way each load waited for
-// the one before it: 30 against 9 us for 64 partials of 96 columns).  Column (t, g) of bank head bh has its n partials at
+// spread over four partials or more of several rows at a time (with the weights formed along the way each load waited for the one
+// before it: 30 against 9 us for 64 partials of 96 columns).  Column (t, g) of bank head bh has its n partials at
 // numbers bh * per_bh + t * per_t + g * per_g + i * per_i.
 template <int DT, int D, class P>
 __global__ void __launch_bounds__(256)
@@ -473,26 +473,42 @@ k_bank_join(const P* __restrict__ sums, const f2v* __restrict__ stats, int T, in
   const float w = l != 0.f ? exp2f(m - (top == -__builtin_inff() ? 0.f : top)) : 0.f;
   l = l != 0.f ? l * w : 0.f;
   for (int o = 32; o; o >>= 1) l += __shfl_xor(l, o);
-  constexpr int E = (D + 63) / 64;
-  float acc[E] = {};
-  for (int i0 = 0; i0 < n; i0 += 8) {
-    float y[8][E];
+  // 4 columns a lane, R lanes a row, RP rows at a time
+  constexpr int R = D / 4, RP = 64 / R;
+  typedef P P4 __attribute__((ext_vector_type(4)));
+  const int row = lane / R, c4 = (lane - row * R) * 4;
+  float acc[4] = {0, 0, 0, 0};
+  for (int i0 = 0; i0 < n; i0 += 4 * RP) {
+    P4 y[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (int j = 0; j < 4; ++j) y[j] = *(const P4*)(p + min(i0 + j * RP + row, n - 1) * step + c4);
 #pragma unroll
-      for (int e = 0; e < E; ++e) y[j][e] = (float)p[min(i0 + j, n - 1) * step + min(e * 64 + lane, D - 1)];
+    for (int j = 0; j < 4; ++j) {
+      const int i = i0 + j * RP + row;
+      const bool use = row < RP && (used >> (i & 63) & 1) && i < n;
+      const float wj = __shfl(w, i & 63);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const bool use = used >> (i0 + j) & 1;
-      const float wj = __shfl(w, i0 + j);
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = use ? fmaf(wj, y[j][e], acc[e]) : acc[e];
+      for (int e = 0; e < 4; ++e) acc[e] = use ? fmaf(wj, (float)y[j][e], acc[e]) : acc[e];
     }
   }
-  typename Row<DT>::T* o = out + (((size_t)b * T + t) * (size_t)(H * G) + hq) * D;
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (e * 64 + lane < D) o[e * 64 + lane] = from_f32<DT>(l == 0.f ? 0.f : acc[e] / l);
+  for (int e = 0; e < 4; ++e) {
+    float all = acc[e];
+#pragma unroll
+    for (int k = 1; k < RP; ++k) all += __shfl(acc[e], (lane + k * R) & 63);
+    acc[e] = l == 0.f ? 0.f : all / l;
+  }
+  typename Row<DT>::T* o = out + (((size_t)b * T + t) * (size_t)(H * G) + hq) * D + c4;
+  if (lane < R) {
+    if constexpr (DT == GPSR_F32) *(f4v*)o = f4v{acc[0], acc[1], acc[2], acc[3]};
+    else {
+      unsigned x[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        x[j] = (unsigned)__builtin_bit_cast(uint16_t, from_f32<DT>(acc[2 * j])) | ((unsigned)__builtin_bit_cast(uint16_t, from_f32<DT>(acc[2 * j + 1])) << 16);
+      *(u2v*)o = u2v{x[0], x[1]};
+    }
+  }
   if (lse && lane == 0) lse[((size_t)b * (H * G) + hq) * T + t] = l == 0.f ? -__builtin_inff() : (log2f(l) + top) * 0.6931471805599453f;
 }
 
