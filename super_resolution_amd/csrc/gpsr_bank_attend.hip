@@ -1,8 +1,6 @@
 // gpsr_bank_attend.hip -- example bank: attention over all rows (include/gpsr.h).
 #include "gpsr_bank_tile.hpp"
 
-#include <type_traits>
-
 // ---------------------------------------------------------------- attention over the whole bank
 // Columns are the (query, head) pairs that share a bank head.  A workgroup of NW waves walks the rows of its split of the
 // bank, KT at a time, NB x W of them in one step:
@@ -50,16 +48,20 @@ k_bank_attend(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, 
   const float c2 = scale * 1.4426950408889634f;
 
   tile.clear_marks(sid, TH);
-  Fetch<BITS, D, KT, TH> f[AHEAD];
+  std::conditional_t<(WK > 1), WaveFetch<BITS, D>, Fetch<BITS, D, KT, TH>> f[AHEAD];
   const WholeBank rows = {table + (size_t)b * table_pages, bk.pages, pshift, len};
   // between the accesses to a tile: LDS serves one wave in order, only the compiler has to be kept from moving them
   const auto sync = [] { if constexpr (WK > 1) { asm volatile("" ::: "memory"); __builtin_amdgcn_wave_barrier(); } else __syncthreads(); };
+  const auto pages = [&](auto& f, unsigned i) { if constexpr (WK > 1) f.pages(rows, i * KT); else f.pages(rows, i * KT, sid); };
+  const auto codes = [&](auto& f, unsigned i) {
+    if constexpr (WK > 1) f.codes(bk, h, pshift, i * KT, len, sid); else f.codes(bk, h, pshift, i * KT, sid);
+  };
   const auto step = [&](unsigned i, auto& f, auto move) {
     sync();
     f.template store<W>(tile, sid, i + 1);
     sync();
-    f.codes(bk, h, pshift, (i + WK * AHEAD) * KT, sid);
-    f.pages(rows, (i + 2 * WK * AHEAD) * KT, sid);
+    codes(f, i + WK * AHEAD);
+    pages(f, i + 2 * WK * AHEAD);
     const unsigned p0 = i * KT;
     tile_marks<D, KT, KT>(tile, 0, i + 1, st, [&](int r) { return !(p0 + r >= lo && p0 + r < hi); });
     const bool skips = skip && __ballot(lo < p0 + KT && hi > p0 && lo < hi);
@@ -85,9 +87,9 @@ k_bank_attend(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, 
     const unsigned first = i0 + (WK > 1 ? wave : 0);
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a) {
-      f[a].pages(rows, (first + WK * a) * KT, sid);
-      f[a].codes(bk, h, pshift, (first + WK * a) * KT, sid);
-      f[a].pages(rows, (first + WK * (AHEAD + a)) * KT, sid);
+      pages(f[a], first + WK * a);
+      codes(f[a], first + WK * a);
+      pages(f[a], first + WK * (AHEAD + a));
     }
     if constexpr (WK > 1) {
       for (unsigned i = first; i < i1; i += WK * AHEAD)

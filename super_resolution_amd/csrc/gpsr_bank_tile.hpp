@@ -10,6 +10,8 @@
 #pragma once
 #include "gpsr_bank.hpp"
 
+#include <type_traits>
+
 // What an accumulator of W columns holds: lane = part * W + column, E values, value e of row row(part, e).  A product contracts
 // over STEP indices, 8 neighbouring ones for each part; slot(r) is where row r of a STEP goes for the second product.
 template <int W> struct Geo;
@@ -152,6 +154,44 @@ struct OnePage {
   __device__ __forceinline__ int left(unsigned v) const { return min(rows - (int)v, 4); }
 };
 
+// 32 columns of a row's key to LDS; MASKED: unless `there`, zeros and an offset of -inf instead
+template <int BITS, int D, int KT, bool MASKED>
+__device__ __forceinline__ void store_keys(const Tile<D, KT>& tile, int r, int g, const unsigned* w, const unsigned* sc, bool there) {
+  constexpr int CW = BITS / 4;
+  u4v* dst = (u4v*)(tile.k + r * Tile<D, KT>::KS + g * 32);
+  const float s = scale_of(!MASKED || there ? sc[0] : 127u);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const unsigned w0 = !MASKED || there ? w[CW * j] : 0u, w1 = !MASKED || there ? w[CW * j + CW - 1] : 0u;
+    dst[j] = u4v{pair<BITS, 0>(w0, w1, s), pair<BITS, 1>(w0, w1, s), pair<BITS, 2>(w0, w1, s), pair<BITS, 3>(w0, w1, s)};
+  }
+  if (g == 0) tile.off[r] = !MASKED || there ? __uint_as_float(sc[1]) : -__builtin_inff();
+}
+
+// 8 columns of 4 rows' values to LDS, transposed; MASKED: zeros for rows r + left and behind
+template <int BITS, int D, int KT, int W, bool MASKED>
+__device__ __forceinline__ void store_values(const Tile<D, KT>& tile, int r, int c, const unsigned* w, const unsigned* sc, int left,
+                                             unsigned number) {
+  constexpr int CW = BITS / 4;
+  unsigned y[4][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const bool here = !MASKED || j < left, nan = here && sc[j] == 255u, there = here && !nan;
+    if (nan) { tile.mark[(r + j) * (D / 32) + c / 4] = number; tile.mark[KT * (D / 32)] = number; }
+    const float s = scale_of(there ? sc[j] : 127u);
+    const unsigned w0 = there ? w[CW * j] : 0u, w1 = there ? w[CW * j + CW - 1] : 0u;
+    y[j][0] = pair<BITS, 0>(w0, w1, s); y[j][1] = pair<BITS, 1>(w0, w1, s);
+    y[j][2] = pair<BITS, 2>(w0, w1, s); y[j][3] = pair<BITS, 3>(w0, w1, s);
+  }
+  // rows r .. r + 3 of the tile are 4 neighbouring slots of a column
+  const int slot = (r & ~(Geo<W>::STEP - 1)) + Geo<W>::slot(r & (Geo<W>::STEP - 1));
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    *(u2v*)(tile.v + Tile<D, KT>::at(c * 8 + 2 * e, slot)) = u2v{pack_lo(y[0][e], y[1][e]), pack_lo(y[2][e], y[3][e])};
+    *(u2v*)(tile.v + Tile<D, KT>::at(c * 8 + 2 * e + 1, slot)) = u2v{pack_hi(y[0][e], y[1][e]), pack_hi(y[2][e], y[3][e])};
+  }
+}
+
 // ---- a tile on its way: codes are loaded a tile ahead of their use, page numbers two.  The tile is 2 U units, U of keys (32
 // columns of a row each) and U of values (8 columns of 4 rows each), dealt to the threads in that order: a thread has one kind or
 // the other at a time and holds both in the same registers.
@@ -225,38 +265,81 @@ struct Fetch {
       const int u = tid + NTH * i;
       if (!EVEN && u >= 2 * U) continue;
       const int r = row(i, tid);
-      if (keys(i, tid)) {
-        const int g = u % (D / 32);
-        const bool there = fpage[i] >= 0;
-        u4v* dst = (u4v*)(tile.k + r * Tile<D, KT>::KS + g * 32);
-        const float s = scale_of(there ? sc[i][0] : 127u);
+      if (keys(i, tid)) store_keys<BITS, D, KT, true>(tile, r, u % (D / 32), w[i], sc[i], fpage[i] >= 0);
+      else store_values<BITS, D, KT, W, true>(tile, r, (u - U) % (D / 8), w[i], sc[i], fleft[i], number);
+    }
+  }
+};
+
+// ---- the same for one wave with a tile of 32 rows of its own.  Its 16-row halves lie in one page each, so page numbers and
+// addresses are uniform, a lane's offsets stay the same from tile to tile, and only the bank's last tile has rows to be left out
+// (with Fetch, half of the instructions of a tile were addresses and masks).
+template <int BITS, int D>
+struct WaveFetch {
+  static constexpr int KT = 32, U = D, N = 2 * U / 64, CW = BITS / 4, RB = D * BITS / 8, G = D / 32;
+  int page[2];                       // of the halves of the next tile; -1: not there
+  int left;                          // rows of the tile under way that exist, if its pages do
+  bool there[2];
+  unsigned w[N][4 * CW], sc[N][4];
+
+  __device__ __forceinline__ static bool keys(int i, int lane) { return 64 * (i + 1) <= U ? true : 64 * i >= U ? false : lane + 64 * i < U; }
+  __device__ __forceinline__ static int row(int i, int lane) {
+    const int u = lane + 64 * i;
+    return keys(i, lane) ? u / G : (u - U) / (D / 8) * 4;
+  }
+  __device__ __forceinline__ void pages(const WholeBank& rows, unsigned p0) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const unsigned w0 = there ? w[i][CW * j] : 0u, w1 = there ? w[i][CW * j + CW - 1] : 0u;
-          dst[j] = u4v{pair<BITS, 0>(w0, w1, s), pair<BITS, 1>(w0, w1, s), pair<BITS, 2>(w0, w1, s), pair<BITS, 3>(w0, w1, s)};
+    for (int k = 0; k < 2; ++k) page[k] = __builtin_amdgcn_readfirstlane(rows.page(p0 + 16 * k));
+  }
+  __device__ __forceinline__ void codes(const gpsr_bank& bk, int h, int pshift, unsigned p0, unsigned len, int lane) {
+    const unsigned mask = (1u << pshift) - 1;
+    size_t at[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      there[k] = page[k] >= 0;
+      at[k] = (((size_t)max(page[k], 0) * bk.heads + h) << pshift) + ((p0 + 16 * k) & mask) - 16 * k;
+    }
+    left = len > p0 ? (int)min(len - p0, 32u) : 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int u = lane + 64 * i, r = row(i, lane);
+      const size_t base = r < 16 ? at[0] : at[1];
+      if (keys(i, lane)) {
+        const int g = u % G;
+        const u4v* src = (const u4v*)(bk.k_codes + base * RB + (r * RB + g * (4 * BITS)));
+#pragma unroll
+        for (int j = 0; j < CW; ++j) {
+          const u4v a = src[j];
+          w[i][4 * j] = a.x; w[i][4 * j + 1] = a.y; w[i][4 * j + 2] = a.z; w[i][4 * j + 3] = a.w;
         }
-        if (g == 0) tile.off[r] = there ? __uint_as_float(sc[i][1]) : -__builtin_inff();
+        sc[i][0] = (bk.k_scales + base * G)[r * G + g];
+        sc[i][1] = __float_as_uint((bk.offset + base)[r]);
       } else {
         const int c = (u - U) % (D / 8);
-        unsigned y[4][4];
+        const uint8_t* src = bk.v_codes + base * RB + (r * RB + c * BITS);
+        const uint8_t* scale = bk.v_scales + base * G + (r * G + c / 4);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const bool here = j < fleft[i], nan = here && sc[i][j] == 255u, there = here && !nan;
-          if (nan) { tile.mark[(r + j) * (D / 32) + c / 4] = number; tile.mark[KT * (D / 32)] = number; }
-          const float s = scale_of(there ? sc[i][j] : 127u);
-          const unsigned w0 = there ? w[i][CW * j] : 0u, w1 = there ? w[i][CW * j + CW - 1] : 0u;
-          y[j][0] = pair<BITS, 0>(w0, w1, s); y[j][1] = pair<BITS, 1>(w0, w1, s);
-          y[j][2] = pair<BITS, 2>(w0, w1, s); y[j][3] = pair<BITS, 3>(w0, w1, s);
-        }
-        // rows r .. r + 3 of the tile are 4 neighbouring slots of a column
-        const int slot = (r & ~(Geo<W>::STEP - 1)) + Geo<W>::slot(r & (Geo<W>::STEP - 1));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          *(u2v*)(tile.v + Tile<D, KT>::at(c * 8 + 2 * e, slot)) = u2v{pack_lo(y[0][e], y[1][e]), pack_lo(y[2][e], y[3][e])};
-          *(u2v*)(tile.v + Tile<D, KT>::at(c * 8 + 2 * e + 1, slot)) = u2v{pack_hi(y[0][e], y[1][e]), pack_hi(y[2][e], y[3][e])};
+          if constexpr (CW == 1) w[i][j] = *(const unsigned*)(src + j * RB);
+          else { const u2v a = *(const u2v*)(src + j * RB); w[i][2 * j] = a.x; w[i][2 * j + 1] = a.y; }
+          sc[i][j] = scale[j * G];
         }
       }
     }
+  }
+  template <int W>
+  __device__ __forceinline__ void store(const Tile<D, KT>& tile, int lane, unsigned number) {
+    const auto all = [&](auto masked) {
+      constexpr bool M = decltype(masked)::value;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int u = lane + 64 * i, r = row(i, lane);
+        const bool half = r < 16 ? there[0] : there[1];
+        if (keys(i, lane)) store_keys<BITS, D, KT, M>(tile, r, u % G, w[i], sc[i], half && r < left);
+        else store_values<BITS, D, KT, W, M>(tile, r, (u - U) % (D / 8), w[i], sc[i], half ? min(left - r, 4) : 0, number);
+      }
+    };
+    if (there[0] && there[1] && left == 32) all(std::false_type()); else all(std::true_type());
   }
 };
 
