@@ -443,6 +443,16 @@ int gpsr_bank_attend_pages(const gpsr_bank* bank, const int32_t* table, int B, i
                            size_t workspace_bytes, void* stream);
 
 /*
+ * Images to bank rows and back (the window loops of agpr.py:165-185 for a bank).  side odd, 3..15, side * side <= dim.
+ *   gpsr_bank_windows: the side x side window of every pixel that has a whole one, row by row: out [(H-side+1)*(W-side+1)][dim]
+ *     of dtype, columns behind side*side zero; centre != 0: less the window's own mean (taken in 64 bits).
+ *   gpsr_bank_blend: out[H][W] = img + the mean, over the windows that hold the pixel, of what they say about it (detail, laid out as
+ *     gpsr_bank_windows lays them out), summed in 64 bits in the windows' order.
+ */
+int gpsr_bank_windows(const double* img, int H, int W, int side, int centre, void* out, int dtype, int dim, void* stream);
+int gpsr_bank_blend(const double* img, int H, int W, int side, const void* detail, int dtype, int dim, double* out, void* stream);
+
+/*
  * Kernel timing for bench.py's roofline line: HIP-event brackets around the
  * tagged launches, on the stream they are launched on.  No counterpart in the
  * reference (its only instrumentation is time.time() per image, gprsr.py:49-72).

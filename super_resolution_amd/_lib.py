@@ -95,6 +95,8 @@ SIGNATURES = {
     "gpsr_bank_attend_pages_workspace_bytes": (c_size_t, [c_void_p] + [c_int] * 6),
     "gpsr_bank_attend_pages": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int,
                                        c_void_p, c_void_p, c_int, c_float] + [c_void_p] * 4 + [c_size_t, c_void_p]),
+    "gpsr_bank_windows": (c_int, [c_void_p] + [c_int] * 4 + [c_void_p, c_int, c_int, c_void_p]),
+    "gpsr_bank_blend": (c_int, [c_void_p] + [c_int] * 3 + [c_void_p, c_int, c_int, c_void_p, c_void_p]),
     "gpsr_sepfilter_u8": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p]),
     "gpsr_metrics_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
     "gpsr_metrics": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_size_t, c_void_p]),

@@ -49,8 +49,21 @@ class ColorSpace(Enum):
     GRAYSCALE = 2
 
 
+class Predictor(Enum):
+    GP = 1      # the reference's: the linear-kernel GP on the actively sampled tenth of the candidates
+    BANK = 2    # not in the reference: every candidate window in an example bank (bank.ExampleBank)
+
+
 DATASET = TrainingDataset.BSD100
 COLOR_SPACE = ColorSpace.YCRCB
+
+PREDICTOR = Predictor.GP
+#: Predictor.BANK: windows drawn from the training images, bits they are held in, pages of 64 windows looked at for each pixel
+#: (None: all), and the inverse squared bandwidths tried, as multiples of 1 / (mean squared norm of a window)
+BANK_ROWS = 100000
+BANK_BITS = 4
+BANK_PAGES = 16
+BANK_SCALES = (2, 4, 8, 16, 32)
 
 SCALE_COEFFICIENT_BANDWIDTH = 0.2
 CHARACTERISTIC_TRADEOFF = 0.2
@@ -97,6 +110,10 @@ class AGPRSuperResolution:
         self.srf = srf
         self.verbose = verbose
         self.start_time = time()
+        self.predictor = PREDICTOR
+        if self.predictor == Predictor.BANK:
+            self._set_bank(use_existing_model)
+            return
         if not os.path.exists(self.get_checkpoint_path('model')):
             use_existing_model = False
         if use_existing_model:
@@ -149,9 +166,18 @@ class AGPRSuperResolution:
     def upscale_channel_device(self, image):
         """device float64 LR image in [0,1] -> device float64 HR image * 255 (agpr.py:160-190)."""
         up = imgproc.resize_cubic(image, dsize=(image.shape[1] * self.srf, image.shape[0] * self.srf))
-        pred = ops.agpr_filter(up, L, self.filter_weights(), self.model.raw[0].contiguous())
+        if self.predictor == Predictor.BANK:
+            pred = self._bank_detail(up)
+        else:
+            pred = ops.agpr_filter(up, L, self.filter_weights(), self.model.raw[0].contiguous())
         pred = self.iterative_back_projection_device(pred, image)
         return torch.clamp(pred, 0.0, 1.0) * 255
+
+    def _bank_detail(self, up):
+        """up + the detail that the bank knows for its windows, each pixel's the mean over the windows that hold it."""
+        dim = self.bank.bank.centroid.shape[-1]
+        detail = self.bank.predict(ops.bank_windows(up, L, dim, centre=True), self.bank_scale, pages=BANK_PAGES)
+        return ops.bank_blend(up, detail, L)
 
     def iterative_back_projection(self, interpolated_image: np.ndarray, original_image: np.ndarray) -> np.ndarray:
         return self.iterative_back_projection_device(_to_dev(interpolated_image), _to_dev(original_image)).cpu().numpy()
@@ -201,6 +227,42 @@ class AGPRSuperResolution:
         torch.save(self.train_y, self.get_checkpoint_path("train_y"))
         if self.verbose:
             print("Training data set in {:.2f} seconds".format(time() - t0))
+
+    def _set_bank(self, use_existing):
+        """The example bank: from bank_x.pt / bank_y.pt of the checkpoint folder, or drawn from the training images (windows of the
+        bicubic image without their mean -> what the HR image has there besides) and saved there."""
+        names = [self.get_checkpoint_path(n) for n in ("bank_x", "bank_y")]
+        if use_existing and all(os.path.exists(n) for n in names):
+            x, y = (torch.load(n, weights_only=True, map_location=_device()) for n in names)
+        else:
+            x, y = self._draw_windows()
+            os.makedirs(self.get_checkpoint_folder(), exist_ok=True)
+            for n, t in zip(names, (x, y)):
+                torch.save(t.cpu(), n)
+        from .bank import ExampleBank
+        self.bank = ExampleBank(x.shape[0], L * L, bits=BANK_BITS).append(x, y)
+        unit = 1.0 / max(float(x.float().square().sum(-1).mean()), 1e-12)
+        self.bank_scale = self.bank.choose_scale([s * unit for s in BANK_SCALES], pages=BANK_PAGES)
+
+    def _draw_windows(self):
+        """BANK_ROWS windows and details [n,L*L] (bfloat16) at random places of the training images, ordered by the direction and
+        strength of the window's slope, so that a page holds windows that are alike."""
+        hr_images = self.get_training_images("HR")
+        per = -(-BANK_ROWS // len(hr_images))
+        xs, ys = [], []
+        for hr in hr_images:
+            hr = np.ascontiguousarray(hr[:hr.shape[0] // self.srf * self.srf, :hr.shape[1] // self.srf * self.srf])
+            high, low = _to_dev(hr), _to_dev(downscale(hr))
+            up = imgproc.resize_cubic(low, dsize=(hr.shape[1], hr.shape[0]))
+            n = (hr.shape[0] - L + 1) * (hr.shape[1] - L + 1)
+            at = torch.as_tensor(np.random.randint(0, n, per)).to(high.device)
+            xs.append(ops.bank_windows(up, L, L * L, centre=True)[0, at, 0])
+            ys.append(ops.bank_windows(ops.axpy(high, up, -1.0), L, L * L)[0, at, 0])
+        x, y = torch.cat(xs)[:BANK_ROWS], torch.cat(ys)[:BANK_ROWS]
+        w = x.float().view(-1, L, L)
+        dy, dx = w[:, padding + 1, padding] - w[:, padding - 1, padding], w[:, padding, padding + 1] - w[:, padding, padding - 1]
+        order = torch.argsort(torch.round(torch.atan2(dy, dx) * (8 / np.pi)) * 10 + torch.hypot(dy, dx))
+        return x[order].contiguous(), y[order].contiguous()
 
     def _active_sampling(self, data):
         """agpr.py:122-137 on the GPU (gpsr_active_sample): distances, representativeness scores and the greedy loop

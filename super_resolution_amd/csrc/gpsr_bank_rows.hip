@@ -251,3 +251,82 @@ extern "C" int gpsr_bank_read(const gpsr_bank* bank, const int32_t* table, int B
   CHECK_LAUNCH("k_bank_read");
   return 0;
 }
+
+// ---------------------------------------------------------------- images to rows and back
+// One wave per window, a column (or four) per lane: bound by writing the rows.
+template <int DT>
+__global__ void __launch_bounds__(256)
+k_bank_windows(const double* __restrict__ img, int W, int side, bool centre, int wide, int64_t n, typename Row<DT>::T* __restrict__ out, int dim) {
+  const int lane = threadIdx.x & 63;
+  const int64_t i = (int64_t)blockIdx.x * 4 + wave_of(threadIdx.x);
+  if (i >= n) return;
+  const double* p = img + (i / wide) * W + i % wide;
+  double y[4], sum = 0.0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int c = k * 64 + lane;
+    y[k] = c < side * side ? p[(size_t)(c / side) * W + c % side] : 0.0;
+    sum += y[k];
+  }
+  for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+  const double mean = centre ? sum / (side * side) : 0.0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int c = k * 64 + lane;
+    if (c < dim) {
+      const float x = c < side * side ? (float)(y[k] - mean) : 0.f;
+      if constexpr (DT == GPSR_BF16) out[i * dim + c] = bf16_rne(x); else out[i * dim + c] = (typename Row<DT>::T)x;
+    }
+  }
+}
+
+// One thread per pixel: up to side * side windows hold it.
+template <int DT>
+__global__ void __launch_bounds__(256)
+k_bank_blend(const double* __restrict__ img, int H, int W, int side, const typename Row<DT>::T* __restrict__ detail, int dim,
+             double* __restrict__ out) {
+  const int x = blockIdx.x * 256 + threadIdx.x, y = blockIdx.y;
+  if (x >= W) return;
+  const int wide = W - side + 1, high = H - side + 1;
+  double sum = 0.0;
+  int n = 0;
+  for (int wy = max(y - side + 1, 0); wy <= min(y, high - 1); ++wy)
+    for (int wx = max(x - side + 1, 0); wx <= min(x, wide - 1); ++wx) {
+      sum += (double)to_f32<DT>(detail[((size_t)wy * wide + wx) * dim + (y - wy) * side + (x - wx)]);
+      ++n;
+    }
+  out[(size_t)y * W + x] = img[(size_t)y * W + x] + sum / n;
+}
+
+static const char* windows_wrong(const double* img, int H, int W, int side, const void* rows, int dtype, int dim) {
+  if (!img || !rows) return "bank_windows: null pointer";
+  if (side < 3 || side > 15 || side % 2 == 0) return "bank_windows: side must be odd, 3..15";
+  if (H < side || W < side) return "bank_windows: image smaller than a window";
+  if (dim < side * side || dim > 256) return "bank_windows: dim must be in side * side .. 256";
+  if (!type_ok(dtype)) return "bank_windows: dtype";
+  if (H > 65535) return "bank_windows: more than 65535 rows";
+  return nullptr;
+}
+extern "C" int gpsr_bank_windows(const double* img, int H, int W, int side, int centre, void* out, int dtype, int dim, void* stream) {
+  if (const char* w = windows_wrong(img, H, W, side, out, dtype, dim)) return arg_fail(w);
+  const int wide = W - side + 1;
+  const int64_t n = (int64_t)wide * (H - side + 1);
+  const dim3 grid((unsigned)((n + 3) / 4));
+  hipStream_t st = (hipStream_t)stream;
+#define WINDOWS(DT) hipLaunchKernelGGL((k_bank_windows<DT>), grid, dim3(256), 0, st, img, W, side, centre != 0, wide, n, (Row<DT>::T*)out, dim)
+  if (dtype == GPSR_BF16) WINDOWS(GPSR_BF16); else if (dtype == GPSR_F16) WINDOWS(GPSR_F16); else WINDOWS(GPSR_F32);
+#undef WINDOWS
+  CHECK_LAUNCH("k_bank_windows");
+  return 0;
+}
+extern "C" int gpsr_bank_blend(const double* img, int H, int W, int side, const void* detail, int dtype, int dim, double* out, void* stream) {
+  if (const char* w = windows_wrong(img, H, W, side, detail, dtype, dim)) return arg_fail(w);
+  if (!out) return arg_fail("bank_blend: null pointer");
+  const dim3 grid((unsigned)((W + 255) / 256), (unsigned)H);
+  hipStream_t st = (hipStream_t)stream;
+#define BLEND(DT) hipLaunchKernelGGL((k_bank_blend<DT>), grid, dim3(256), 0, st, img, H, W, side, (const Row<DT>::T*)detail, dim, out)
+  if (dtype == GPSR_BF16) BLEND(GPSR_BF16); else if (dtype == GPSR_F16) BLEND(GPSR_F16); else BLEND(GPSR_F32);
+#undef BLEND
+  CHECK_LAUNCH("k_bank_blend");
+  return 0;
+}

@@ -598,6 +598,34 @@ def bank_attend_pages(bank, table, length, q, pages, scale, skip=None, want_lse=
     return (out, lse) if want_lse else out
 
 
+def bank_windows(img, side, dim, dtype=torch.bfloat16, centre=False):
+    """float64 [H,W] -> [1,(H-side+1)*(W-side+1),1,dim]: the side x side window of every pixel that has a whole one, zeros behind
+    its side*side columns; centre: less its own mean (gpsr_bank_windows)."""
+    lib = _lib.load()
+    H, W = img.shape
+    if dtype not in _BANK_TYPES:
+        raise _lib.GpsrError(f"bank_windows: expected bfloat16, float16 or float32, got {dtype}")
+    n = max(H - side + 1, 0) * max(W - side + 1, 0)
+    out = torch.empty((1, n, 1, dim), dtype=dtype, device=img.device)
+    _lib.check(lib.gpsr_bank_windows(_p(img, torch.float64), H, W, side, int(centre), out.data_ptr(), _BANK_TYPES[dtype], dim, _stream()),
+               "gpsr_bank_windows")
+    return out
+
+
+def bank_blend(img, detail, side):
+    """img [H,W] + the mean of what the windows that hold a pixel say about it; detail as bank_windows lays windows out (gpsr_bank_blend)."""
+    lib = _lib.load()
+    H, W = img.shape
+    n = max(H - side + 1, 0) * max(W - side + 1, 0)
+    dim = detail.shape[-1]
+    if detail.numel() != n * dim or detail.dtype not in _BANK_TYPES:
+        raise _lib.GpsrError(f"bank_blend: detail {tuple(detail.shape)} {detail.dtype} does not fit {H} x {W} and side {side}")
+    out = torch.empty_like(img)
+    _lib.check(lib.gpsr_bank_blend(_p(img, torch.float64), H, W, side, _p(detail), _BANK_TYPES[detail.dtype], dim, out.data_ptr(),
+                                   _stream()), "gpsr_bank_blend")
+    return out
+
+
 # ------------------------------------------------------------ kernel timing
 PROF_TAGS = ("update", "panel", "pivot", "build", "grad1", "grad2", "predict", "update_last", "update2", "update_sel", "fused")
 

@@ -81,3 +81,16 @@ def test_ops_refuse_host_tensors():
               lambda: ops.bank_attend_pages(bank, i32(1, 2), i32(1), f32(1, 1, 1, 64), i32(1, 1, 1, 2), 1.0)):
         with pytest.raises(_lib.GpsrError, match="device tensors"):
             f()
+
+
+def test_windows_and_blend_refuse():
+    from super_resolution_amd import _lib
+    lib = _lib.load()
+    ok = dict(img=4096, H=20, W=20, side=7, rows=4096, dtype=0, dim=64, out=4096)
+    for change in (dict(img=0), dict(rows=0), dict(side=4), dict(side=1), dict(side=17), dict(H=6), dict(W=6), dict(dim=48), dict(dim=257),
+                   dict(dtype=3), dict(H=65536)):
+        a = {**ok, **change}
+        assert lib.gpsr_bank_windows(a["img"], a["H"], a["W"], a["side"], 1, a["rows"], a["dtype"], a["dim"], None) == -1, change
+        assert lib.gpsr_bank_blend(a["img"], a["H"], a["W"], a["side"], a["rows"], a["dtype"], a["dim"], a["out"], None) == -1, change
+    a = {**ok, "out": 0}
+    assert lib.gpsr_bank_blend(a["img"], a["H"], a["W"], a["side"], a["rows"], a["dtype"], a["dim"], a["out"], None) == -1
