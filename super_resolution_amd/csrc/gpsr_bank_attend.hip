@@ -128,10 +128,14 @@ k_bank_attend(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, 
 }
 
 // How one call is cut: a plan of sizes alone, so that the workspace can be asked for beforehand.
-struct Plan { bool few; int cw, kt, splits; int64_t groups; };
+struct Plan { bool few, lone; int cw, kt, splits; int64_t groups; };
 static constexpr int many_nb(int d, int nt) { return tile_waves(d, nt, 2) == tile_waves(d, nt, 1) ? 2 : 1; }
 static constexpr int many_nw(int d, int nt) { return tile_waves(d, nt, many_nb(d, nt)) >= 2 ? 8 : 4; }
-static constexpr int many_kt(int d, int nt) { return many_nw(d, nt) == 8 && tile_lds(d, 128) <= 80 * 1024 ? 128 : 64; }
+// 128 rows a tile where one or two workgroups of it fit a CU; 64 where the query terms leave too few registers to have more under way
+// (96 columns in f16 862 against 892 us, in f32 95 against 105; 64 columns in f32 553 against 527)
+static constexpr int many_kt(int d, int nt) { return many_nw(d, nt) == 8 && tile_lds(d, 128) <= 80 * 1024 && (d < 96 || nt == 1) ? 128 : 64; }
+// whether there is a form with half the waves and twice the registers (plan_of says when it is taken)
+static constexpr bool lone_nb(int d, int nt) { return tile_waves(d, nt, 1) == 4 && tile_waves(d, nt, 2) == 2; }
 // tiles under way for up to 16 columns: two where the registers hold them (96 columns: a thread with keys and values by turns, which
 // the compiler keeps in memory)
 static constexpr int few_ahead(int d, int bits, int nt) { return d * bits <= 512 && d != 96 ? 2 : 1; }
@@ -140,19 +144,31 @@ static Plan plan_of(const gpsr_bank* bk, int B, int table_pages, int T, int q_he
   const int64_t C = (int64_t)T * (q_heads / bk->heads);
   const int nt = dtype == GPSR_BF16 ? 1 : dtype == GPSR_F16 ? 2 : 3, nw = many_nw(bk->dim, nt);
   p.few = C <= 32;
+  p.lone = false;
   p.cw = p.few ? 32 : 32 * nw;
   p.kt = p.few ? 32 : many_kt(bk->dim, nt);
   p.groups = (C + p.cw - 1) / p.cw;
   const int64_t tiles = (((int64_t)table_pages * bk->page_rows) + p.kt - 1) / p.kt;
   // The splits that end soonest when `slots` workgroups run at a time, each paying for `own` tiles besides its share, and the join
   // for some more.
-  const int64_t slots = p.few ? 512 : 256 * 4 * tile_waves(bk->dim, nt, many_nb(bk->dim, nt)) / nw, wgs = p.groups * bk->heads * B;
+  const int64_t wgs = p.groups * bk->heads * B;
+  const int64_t slots = p.few ? 512 : 256 * 4 * tile_waves(bk->dim, nt, many_nb(bk->dim, nt)) / nw;
   const int step = p.few ? 4 : 1, own = p.few ? 4 : 2;           // tiles that a workgroup takes at once
   int64_t best = -1;
   p.splits = 1;
   for (int s = 1; s <= 64 && s * step <= (tiles > step ? tiles + step - 1 : step); ++s) {
     const int64_t cost = ((wgs * s + slots - 1) / slots) * ((tiles + s * step - 1) / (s * step) + own) + (s > 1 ? 2 + s / 4 : 0);
     if (best < 0 || cost < best) { best = cost; p.splits = s; }
+  }
+  // Or one workgroup on each CU with 64 rows at a time in twice the registers.  At 64 columns a tile of 128 rows takes a CU's two
+  // workgroups of 4 waves a SIMD 4.4 us (and starting and ending one as much as 4 tiles), the lone one 2.95; partials cost 0.13 ns
+  // a column and split, and the join 10 us.  So it
+  // pays where the columns just fill the CUs and the bank is short: 65 025 queries of 5000 rows 124 us instead of 136 (but 40 000
+  // of 100 000 rows 1470 instead of 1150).
+  if (!p.few && lone_nb(bk->dim, nt) && p.splits > 1) {
+    const double split = ((wgs * p.splits + slots - 1) / slots) * ((tiles + p.splits - 1) / p.splits + 4) * 4.4 + 10 + 0.13e-3 * (double)C * bk->heads * B * p.splits;
+    const double lone = ((wgs + 255) / 256) * (tiles + own) * 2.95;
+    if (lone < split) { p.lone = true; p.splits = 1; }
   }
   return p;
 }
@@ -177,7 +193,8 @@ static void launch_attend(const Plan& p, const gpsr_bank& bk, const int32_t* tab
     dim3(64 * NW_), 0, st, bk, table, table_pages, pshift, length, (const E*)q, T, G, qs, qwide, scale, skip, (E*)out, lse, p.splits, sums, stats)
   if (p.few && (int64_t)T * G <= 16) ATTEND(16, 4, 4, 32, 2, few_ahead(D, BITS, NT));
   else if (p.few) ATTEND(32, 4, 4, 32, 1, 1);
-  else ATTEND(32, NW, 1, many_kt(D, NT), many_nb(D, NT), 1);
+  else if (!p.lone) ATTEND(32, NW, 1, many_kt(D, NT), many_nb(D, NT), 1);
+  else if constexpr (lone_nb(D, NT)) ATTEND(32, NW, 1, many_kt(D, NT), 2, 1);
 #undef ATTEND
   if (p.splits > 1) {
     const int64_t C = (int64_t)T * G;
