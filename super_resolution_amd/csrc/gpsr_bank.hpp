@@ -116,6 +116,8 @@ static inline const char* bank_wrong(const gpsr_bank* b) {
 }
 static inline size_t type_size(int dtype) { return dtype == GPSR_F32 ? 4 : 2; }
 static inline bool type_ok(int dtype) { return dtype == GPSR_BF16 || dtype == GPSR_F16 || dtype == GPSR_F32; }
+// a launch can have fewer than 2^32 threads along a dimension
+static inline bool grid_fits(int64_t groups, int threads) { return groups <= (int64_t)0xffffffffu / threads; }
 // whether every row starts at a multiple of 16 bytes
 static inline bool rows_wide(const void* p, const int64_t* st, int dtype) {
   const int64_t m = 16 / (int64_t)type_size(dtype);

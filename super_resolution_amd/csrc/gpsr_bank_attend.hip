@@ -56,6 +56,9 @@ k_bank_attend(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, 
   const auto codes = [&](auto& f, unsigned i) {
     if constexpr (WK > 1) f.codes(bk, h, pshift, i * KT, len, sid); else f.codes(bk, h, pshift, i * KT, sid);
   };
+  // 0, or 32 in a second walk (Soft::lost), which any 2^31 rows bear; not always 32, because products with values near 2^-100
+  // would leave the range at its other end
+  float above = 0.f;
   const auto step = [&](unsigned i, auto& f, auto move) {
     sync();
     f.template store<W>(tile, sid, i + 1);
@@ -79,11 +82,12 @@ k_bank_attend(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, 
             if (pos >= lo && pos < hi) s[kb][e] = -__builtin_inff();
           }
       }
-      tile_accumulate<D, KT, NT, NB, W, decltype(move)::value>(tile, r, col, part, c2, s, st);
+      tile_accumulate<D, KT, NT, NB, W, decltype(move)::value>(tile, r, col, part, c2, above, s, st);
     }
   };
   st.clear();
-  for (bool safe = WK > 1; i0 < i1; safe = true) {
+#pragma unroll 1
+  for (; i0 < i1; above = 32.f) {
     const unsigned first = i0 + (WK > 1 ? wave : 0);
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a) {
@@ -96,18 +100,18 @@ k_bank_attend(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, 
 #pragma unroll
         for (int a = 0; a < AHEAD; ++a)
           if (i + WK * a < i1) step(i + WK * a, f[a], std::true_type());
-      break;
+      if (above != 0.f || !__ballot(st.lost())) break;
     } else {
       static_assert(AHEAD == 1, "one tile under way");
       // The steps without a move are a loop of their own, in which the sums never leave their registers.  The waves of a
       // workgroup may be in different ones of the two; every step has the same barriers.
       for (unsigned i = i0; i < i1;) {
         step(i++, f[0], std::true_type());
-        while (i < i1 && !safe && !st.wants_move()) step(i++, f[0], std::false_type());
+        while (i < i1 && above == 0.f && !st.wants_move()) step(i++, f[0], std::false_type());
       }
-      if (safe || !__syncthreads_or(st.lost())) break;
-      st.clear();
+      if (above != 0.f || !__syncthreads_or(st.lost())) break;
     }
+    st.clear();
   }
   st.spoil();
 
@@ -210,7 +214,7 @@ extern "C" int gpsr_bank_attend(const gpsr_bank* bank, const int32_t* table, int
   if (B <= 0 || T <= 0) return 0;
   if (const char* w = attend_wrong(bank, table, B, table_pages, length, q, dtype, q_heads, qst, scale, out)) return arg_fail(w);
   const Plan p = plan_of(bank, B, table_pages, T, q_heads, dtype);
-  if (p.groups * p.splits > 0x7fffffff) return arg_fail("bank_attend: too many queries for one call");
+  if (!grid_fits(p.groups * p.splits, 512) || !grid_fits(((int64_t)T * (q_heads / bank->heads) + 3) / 4, 256)) return arg_fail("bank_attend: too many queries for one call");
   const size_t need = gpsr_bank_attend_workspace_bytes(bank, B, table_pages, T, q_heads, dtype);
   if (workspace_bytes < need || (need && !workspace)) return arg_fail("workspace too small");
   if (need && ((uintptr_t)workspace & 15)) return arg_fail("bank_attend: workspace must be 16-byte aligned");

@@ -10,6 +10,10 @@
 // on its place in a list, and the join runs in the order of the caller's numbers: results do not change.
 #include "gpsr_bank_tile.hpp"
 
+// A query's rows are at most 64 pages of 256, so with weights of at most 2^-15 sums of any values stay in float32's range, and
+// products of the smallest held values (2^-111 in 4 bits) with the largest weights as well.
+static constexpr float ABOVE = 15.f;
+
 // ---------------------------------------------------------------- by query
 template <int DT, int BITS, int D, int W>
 __global__ void __launch_bounds__(256, 2)
@@ -85,7 +89,7 @@ k_bank_pages_query(gpsr_bank bk, const int32_t* __restrict__ table, int table_pa
         for (int e = 0; e < X::E; ++e)
           if (skips(i * KT + wrow + kb * W + X::row(part, e))) s[kb][e] = -__builtin_inff();
     }
-    tile_accumulate<D, KT, NT, NB, W, true>(tile, wrow, col, part, c2, s, st);
+    tile_accumulate<D, KT, NT, NB, W, true>(tile, wrow, col, part, c2, ABOVE, s, st);
   }
   st.spoil();
   __syncthreads();
@@ -261,7 +265,7 @@ k_bank_pages_page(gpsr_bank bk, const int32_t* __restrict__ table, int table_pag
           if (pos >= lo && pos < hi) s[0][e] = -__builtin_inff();
         }
       }
-      tile_accumulate<D, KT, NT, NB, W, true>(tile, r, col, part, c2, s, st);
+      tile_accumulate<D, KT, NT, NB, W, true>(tile, r, col, part, c2, ABOVE, s, st);
     }
   }
   st.spoil();
@@ -395,7 +399,7 @@ extern "C" int gpsr_bank_attend_pages(const gpsr_bank* bank, const int32_t* tabl
   if (!sel) return arg_fail("bank_attend_pages: null pointer");
   if (n_sel < 1 || n_sel > 64) return arg_fail("bank_attend_pages: n_sel must be in 1..64");
   const PagesPlan p = plan_of(bank, B, table_pages, T, q_heads, n_sel, dtype);
-  if (p.by_page ? p.most_wgs > 0x7fffffff : (int64_t)T * p.groups * p.splits > 0x7fffffff)
+  if (!grid_fits(p.by_page ? p.most_wgs : (int64_t)T * p.groups * p.splits, 256) || !grid_fits(((int64_t)T * (q_heads / bank->heads) + 3) / 4, 256))
     return arg_fail("bank_attend_pages: too many queries for one call");
   if (workspace_bytes < p.bytes || (p.bytes && !workspace)) return arg_fail("workspace too small");
   if (p.bytes && ((uintptr_t)workspace & 15)) return arg_fail("bank_attend_pages: workspace must be 16-byte aligned");

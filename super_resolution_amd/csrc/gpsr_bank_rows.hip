@@ -177,6 +177,7 @@ extern "C" int gpsr_bank_write(const gpsr_bank* bank, const int32_t* table, int 
   // a run of T rows that starts anywhere in a page touches at most this many
   int64_t touched = (((int64_t)T + bank->page_rows - 2) >> pshift) + 1;
   if (touched > table_pages) touched = table_pages;
+  if (!grid_fits(touched, WR_THREADS)) return arg_fail("bank_write: too many rows for one call");
   const dim3 grid((unsigned)touched, (unsigned)bank->heads, (unsigned)B);
   const Strides ks = {kst[0], kst[1], kst[2]}, vs = {vst[0], vst[1], vst[2]};
   const bool kw = rows_wide(k, kst, dtype), vw = rows_wide(v, vst, dtype);
@@ -237,7 +238,7 @@ extern "C" int gpsr_bank_read(const gpsr_bank* bank, const int32_t* table, int B
   if (((uintptr_t)k | (uintptr_t)v) & 15) return arg_fail("bank_read: k and v must be 16-byte aligned");
   const int pshift = __builtin_ctz((unsigned)bank->page_rows);
   const int64_t blocks = ((int64_t)T * bank->heads * (bank->dim / 8) + 255) / 256;
-  if (blocks > 0x7fffffff) return arg_fail("bank_read: too many rows for one call");
+  if (!grid_fits(blocks, 256)) return arg_fail("bank_read: too many rows for one call");
   const dim3 grid((unsigned)blocks, (unsigned)B);
   hipStream_t st = (hipStream_t)stream;
 #define READ(DT, BITS) hipLaunchKernelGGL((k_bank_read<DT, BITS>), grid, dim3(256), 0, st, *bank, table, table_pages, pshift, \
@@ -256,11 +257,12 @@ extern "C" int gpsr_bank_read(const gpsr_bank* bank, const int32_t* table, int B
 // One wave per window, a column (or four) per lane: bound by writing the rows.
 template <int DT>
 __global__ void __launch_bounds__(256)
-k_bank_windows(const double* __restrict__ img, int W, int side, bool centre, int wide, int64_t n, typename Row<DT>::T* __restrict__ out, int dim) {
+k_bank_windows(const double* __restrict__ img, int W, int side, bool centre, int wide, typename Row<DT>::T* __restrict__ out, int dim) {
   const int lane = threadIdx.x & 63;
-  const int64_t i = (int64_t)blockIdx.x * 4 + wave_of(threadIdx.x);
-  if (i >= n) return;
-  const double* p = img + (i / wide) * W + i % wide;
+  const int x0 = blockIdx.x * 4 + wave_of(threadIdx.x);
+  if (x0 >= wide) return;
+  const size_t i = (size_t)blockIdx.y * wide + x0;
+  const double* p = img + (size_t)blockIdx.y * W + x0;
   double y[4], sum = 0.0;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -304,16 +306,16 @@ static const char* windows_wrong(const double* img, int H, int W, int side, cons
   if (H < side || W < side) return "bank_windows: image smaller than a window";
   if (dim < side * side || dim > 256) return "bank_windows: dim must be in side * side .. 256";
   if (!type_ok(dtype)) return "bank_windows: dtype";
+  if (W > (1 << 24)) return "bank_windows: more than 2^24 columns";
   if (H > 65535) return "bank_windows: more than 65535 rows";
   return nullptr;
 }
 extern "C" int gpsr_bank_windows(const double* img, int H, int W, int side, int centre, void* out, int dtype, int dim, void* stream) {
   if (const char* w = windows_wrong(img, H, W, side, out, dtype, dim)) return arg_fail(w);
   const int wide = W - side + 1;
-  const int64_t n = (int64_t)wide * (H - side + 1);
-  const dim3 grid((unsigned)((n + 3) / 4));
+  const dim3 grid((unsigned)((wide + 3) / 4), (unsigned)(H - side + 1));
   hipStream_t st = (hipStream_t)stream;
-#define WINDOWS(DT) hipLaunchKernelGGL((k_bank_windows<DT>), grid, dim3(256), 0, st, img, W, side, centre != 0, wide, n, (Row<DT>::T*)out, dim)
+#define WINDOWS(DT) hipLaunchKernelGGL((k_bank_windows<DT>), grid, dim3(256), 0, st, img, W, side, centre != 0, wide, (Row<DT>::T*)out, dim)
   if (dtype == GPSR_BF16) WINDOWS(GPSR_BF16); else if (dtype == GPSR_F16) WINDOWS(GPSR_F16); else WINDOWS(GPSR_F32);
 #undef WINDOWS
   CHECK_LAUNCH("k_bank_windows");

@@ -527,6 +527,7 @@ extern "C" int gpsr_bank_select(const gpsr_bank* bank, const int32_t* table, int
   if (table_pages < 0) return arg_fail("bank_select: table_pages");
   if (q_heads < 1 || q_heads > 65535 || q_heads % bank->heads) return arg_fail("bank_select: query heads must be a multiple of the bank's heads, up to 65535");
   if (n_sel < 1 || n_sel > SE_MAX) return arg_fail("bank_select: n_sel must be in 1..64");
+  if (!grid_fits(((int64_t)T + 3) / 4, 256)) return arg_fail("bank_select: too many queries for one call");
   const SelectPlan p = plan_of(bank, B, table_pages, T, n_sel);
   if (workspace_bytes < p.bytes || (p.bytes && !workspace)) return arg_fail("workspace too small");
   if (p.bytes && ((uintptr_t)workspace & 15)) return arg_fail("bank_select: workspace must be 16-byte aligned");

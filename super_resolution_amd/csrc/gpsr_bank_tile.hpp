@@ -382,8 +382,16 @@ struct Soft {
       for (int e = 0; e < X::E; ++e) o[d][e] = 0.f;
   }
   __device__ __forceinline__ bool wants_move() const { return __ballot(m == -__builtin_inff() || l > 0x1p40f) != 0; }
-  // whether a sum ran out of range (or met a NaN: then a second walk changes nothing)
-  __device__ __forceinline__ bool lost() const { return !(l < __builtin_inff()); }
+  // Whether a sum came near the end of its range, or went past it (or met a NaN: then a second walk changes nothing): a weight
+  // far above the reference, or values near the end of theirs.  A sum that passed it stays infinite or NaN.
+  __device__ __forceinline__ bool lost() const {
+    bool ok = l < 0x1p120f;
+#pragma unroll
+    for (int d = 0; d < D / W; ++d)
+#pragma unroll
+      for (int e = 0; e < X::E; ++e) ok = ok && fabsf(o[d][e]) < 0x1p120f;
+    return !ok;
+  }
   __device__ __forceinline__ void rescale(float a) {
     l *= a;
 #pragma unroll
@@ -479,12 +487,13 @@ __device__ __forceinline__ void tile_marks(const Tile<D, KT>& tile, int wrow, un
 }
 
 // One step of the running softmax: logits in, weights times values added to the state.
-//   MOVE: the reference becomes the maximum so far, as a power of two (weights are at most 1), and the state is rescaled.
+//   MOVE: the reference becomes the maximum so far, as a power of two, and the state is rescaled: weights are at most
+//     2^-above, so that fewer than 2^(above - 1) rows of any values stay in range.
 //   otherwise it stays, which saves the maximum of every tile and the wait for it: bf16 and the sums have range to spare, and
-//     their precision is relative.  Soft::wants_move says when it has to be moved (nothing seen yet, or a sum past 2^40); a
-//     weight past 2^127 makes the sum infinite, which the caller has to look for (Soft::lost) and walk again with MOVE only.
+//     their precision is relative.  Soft::wants_move says when it has to be moved (nothing seen yet, or a sum past 2^40); what
+//     a weight far above the reference does is for the caller to look for (Soft::lost), and to walk again with MOVE only.
 template <int D, int KT, int NT, int NB, int W, bool MOVE>
-__device__ __forceinline__ void tile_accumulate(const Tile<D, KT>& tile, int r0, int col, int part, float c2,
+__device__ __forceinline__ void tile_accumulate(const Tile<D, KT>& tile, int r0, int col, int part, float c2, float above,
                                                 typename Geo<W>::Acc (&s)[NB], Soft<D, W>& st) {
   typedef Geo<W> X;
   if constexpr (MOVE) {
@@ -493,7 +502,7 @@ __device__ __forceinline__ void tile_accumulate(const Tile<D, KT>& tile, int r0,
     for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
       for (int e = 0; e < X::E; ++e) mx = fmaxf(mx, s[kb][e]);
-    float mn = fmaxf(st.m, X::parts(mx, max2) * c2);
+    float mn = fmaxf(st.m, fmaf(X::parts(mx, max2), c2, above));
     if (X::parts(st.l, max2) > 0x1p40f) mn = fmaxf(mn, st.m + 40.f);
     st.rescale(mn == -__builtin_inff() ? 1.f : exp2f(st.m - mn));
     st.m = mn;
@@ -553,9 +562,10 @@ k_bank_join(const P* __restrict__ sums, const f2v* __restrict__ stats, int T, in
   const unsigned long long used = __ballot(l != 0.f);      // the others saw nothing, and their sums were not written
   float top = l != 0.f ? m : -__builtin_inff();
   for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-  const float w = l != 0.f ? exp2f(m - (top == -__builtin_inff() ? 0.f : top)) : 0.f;
+  float w = l != 0.f ? exp2f(m - (top == -__builtin_inff() ? 0.f : top)) : 0.f;
   l = l != 0.f ? l * w : 0.f;
   for (int o = 32; o; o >>= 1) l += __shfl_xor(l, o);
+  w = l != 0.f ? w / l : 0.f;          // before the sums: a mean of values near the end of their range stays in it
   // 4 columns a lane, R lanes a row, RP rows at a time
   constexpr int R = D / 4, RP = 64 / R;
   typedef P P4 __attribute__((ext_vector_type(4)));
@@ -579,7 +589,7 @@ k_bank_join(const P* __restrict__ sums, const f2v* __restrict__ stats, int T, in
     float all = acc[e];
 #pragma unroll
     for (int k = 1; k < RP; ++k) all += __shfl(acc[e], (lane + k * R) & 63);
-    acc[e] = l == 0.f ? 0.f : all / l;
+    acc[e] = all;
   }
   typename Row<DT>::T* o = out + (((size_t)b * T + t) * (size_t)(H * G) + hq) * D + c4;
   if (lane < R) {

@@ -94,3 +94,17 @@ def test_windows_and_blend_refuse():
         assert lib.gpsr_bank_blend(a["img"], a["H"], a["W"], a["side"], a["rows"], a["dtype"], a["dim"], a["out"], None) == -1, change
     a = {**ok, "out": 0}
     assert lib.gpsr_bank_blend(a["img"], a["H"], a["W"], a["side"], a["rows"], a["dtype"], a["dim"], a["out"], None) == -1
+
+
+def test_calls_too_large_for_a_launch_are_refused():
+    """A launch has fewer than 2^32 threads along a dimension: 256 for 4 queries, 8 columns a thread, or a page."""
+    most = (1 << 31) - 1
+    for change, which in ((dict(T=most), ("read", "attend", "select", "pages")), (dict(T=most, J=1 << 25), ("write",)),
+                          (dict(T=(1 << 26) + 1, J=1 << 20, n_sel=1), ("attend", "select", "pages")), (dict(T=1 << 24, J=0, n_sel=2), ("pages",))):
+        calls, lib = _calls(_struct(page_rows=16), **change)
+        for name in which:
+            assert calls[name]() == -1 and b"too many" in lib.gpsr_last_error(), (change, name)
+    for call in (lambda lib: lib.gpsr_bank_windows(4096, 9, (1 << 24) + 1, 3, 1, 4096, 0, 32, None),
+                 lambda lib: lib.gpsr_bank_blend(4096, 9, (1 << 24) + 1, 3, 4096, 0, 32, 4096, None)):
+        lib = _calls(_struct())[1]
+        assert call(lib) == -1 and b"columns" in lib.gpsr_last_error()

@@ -693,3 +693,41 @@ def test_refusals_on_the_device():
         with pytest.raises(_lib.GpsrError):
             f()
             pytest.fail(f"call {i} was not refused")
+
+
+# ------------------------------------------------------------ sums near the end of float32's range
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("D,T", [(32, 3), (32, 20), (32, 100), (64, 100), (256, 40)])
+def test_a_row_far_above_all_before_it(dtype, D, T):
+    """A weight of 2^126.5 against the rows before it, times a value of 6, is past float32's range, the weight and the mean are not."""
+    ops = _ops()
+    c = Case([900], 1, D, 32, 4, "LINEAR", dtype, seed=D + T)
+    c.k.zero_()
+    c.k[0, 555, 0, 0] = 96.0
+    c.v[0, 555, 0, :] = 6.0
+    ops.bank_write(c.bank, c.table, torch.zeros_like(c.length), c.length, c.k.to(c.dev), c.v.to(c.dev))
+    c.hk, c.hv, c.o = held(c.k.double().numpy(), 4), held(c.v.double().numpy(), 4), np.zeros((1, 900, 1))
+    q = torch.zeros(1, T, 1, D, dtype=dtype)
+    q[..., 0] = 1.0
+    s = float(np.float32(126.5 * math.log(2) / 96))
+    out, lse = ops.bank_attend(c.bank, c.table, c.length, q.to(c.dev), s, want_lse=True)
+    c.check(q, out, lse, s, lambda b, t, h: np.ones(900, bool))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("size", [2.5e38, 2.0 ** -108])
+@pytest.mark.parametrize("T", [3, 20, 100, 700])
+def test_values_of_the_ends_of_the_range(dtype, size, T):
+    """Means of 900 values of up to 6 * 2^125, whose sum is past float32's range; and of the smallest ones."""
+    ops = _ops()
+    c = Case([900], 1, 64, 32, 4, "RBF", dtype, seed=T)
+    c.v = (torch.as_tensor(c.rng.integers(-1, 2, size=(1, 900, 1, 64))).double() * size + size).to(dtype)     # 0, size, 2 size
+    c.v.clamp_(max=2.5e38)
+    ops.bank_write(c.bank, c.table, torch.zeros_like(c.length), c.length, c.k.to(c.dev), c.v.to(c.dev))
+    c.hv = held(c.v.double().numpy(), 4)
+    q, qd = c.queries(T, 1, dtype)
+    out, lse = ops.bank_attend(c.bank, c.table, c.length, qd, 0.25, want_lse=True)
+    c.check(q, out, lse, 0.25, lambda b, t, h: np.ones(900, bool))
+    sel = torch.as_tensor(c.rng.integers(0, 29, (1, T, 1, 16)).astype(np.int32))
+    out, lse = ops.bank_attend_pages(c.bank, c.table, c.length, qd, sel.to(c.dev), 0.25, want_lse=True)
+    c.check(q, out, lse, 0.25, lambda b, t, h: np.isin(np.arange(900) // 32, sel[b, t, h].numpy()))
