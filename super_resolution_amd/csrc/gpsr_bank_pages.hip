@@ -1,11 +1,12 @@
 // gpsr_bank_pages.hip -- example bank: attention over chosen pages (include/gpsr.h).
 //
 // Two ways through the same mathematics:
-//   by query: a workgroup per query walks that query's pages, its four waves 32 rows each against the query's heads.  Nothing
+//   by query (7 us for one query and 16 pages): a workgroup per query walks that query's pages, its four waves 32 rows each against the query's heads.  Nothing
 //     is shared, 31 of 32 columns of the matrix instructions idle (one head), but it takes one or two launches.
 //   by page: the choices are turned over (for each page the list of queries that chose it), a workgroup takes one page and
 //     128 of its queries, writes each query's partial result for that page, and a last kernel joins each query's partials.
-//     Pages are decoded once per 128 queries and all columns work, at the price of writing and reading the partials.
+//     Pages are decoded once per 128 queries and all columns work, at the price of writing and reading the partials: 40 000
+//     queries with 16 pages each 109 us (count 14, shares 10, scan 5, fill 7, products 59, join 19), by query 4380.
 // Within a chunk of choices the lists' order comes from counters in LDS and may differ from run to run; a partial does not depend
 // on its place in a list, and the join runs in the order of the caller's numbers: results do not change.
 #include "gpsr_bank_tile.hpp"
@@ -109,7 +110,7 @@ k_bank_pages_query(gpsr_bank bk, const int32_t* __restrict__ table, int table_pa
 // ---------------------------------------------------------------- by page
 // The choices of one entry are cut into chunks of PG_CHUNK.  A chunk counts its own in LDS (bucket: bank head and logical page)
 // and writes its histogram; a choice keeps its place within its chunk's share of the list, -1 if it is passed over.  Counting
-// through global atomics instead took 59 us for 640 000 choices of 1563 pages, this 9.
+// through global atomics instead took 59 us for 640 000 choices of 1563 pages; counts 14 and shares 10 us this way.
 #define PG_CHUNK 4096
 #define PG_BUCKETS 16384      // of one entry: 64 KB of LDS
 __global__ void __launch_bounds__(512)
@@ -161,7 +162,7 @@ k_bank_pages_shares(int* __restrict__ hist, int buckets, int chunks, int* __rest
 }
 
 // exclusive sums of the counts and of the workgroups that each bucket needs, and each workgroup's bucket (found by bisection
-// over the sums instead, it was a third of the 66 us of the product kernel); one workgroup
+// over the sums instead, it was a third of the product kernel's time); one workgroup
 __global__ void __launch_bounds__(1024)
 k_bank_pages_scan(const int* __restrict__ count, int buckets, int G, int cw, int* __restrict__ start, int* __restrict__ wgs,
                   int* __restrict__ owner) {
@@ -209,8 +210,8 @@ template <int DT> struct Partial { typedef float T; };
 template <> struct Partial<GPSR_BF16> { typedef _Float16 T; };
 static constexpr int page_lds(int d, int kt) { return tile_lds(d, kt) > 256 * (d + 4) ? tile_lds(d, kt) : 256 * (d + 4); }
 
-// 32 rows at a time and three waves per SIMD: the workgroups are short and mostly wait (62 us; all 64 rows of a page at a time 66, two
-// waves 76 and 79, four waves with spills 90)
+// 32 rows at a time and three waves per SIMD: the workgroups are short and mostly wait (59 us for 40 000 queries x 16 pages of
+// 64 rows of 64 columns, 178 TFLOP/s; all 64 rows of a page at a time 4 us more, two waves 15 more, four with spills 30 more)
 template <int DT, int BITS, int D, int KT>
 __global__ void __launch_bounds__(256, tile_waves(D, Terms<DT>::N, 1) > 3 ? 3 : tile_waves(D, Terms<DT>::N, 1))
 k_bank_pages_page(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, int pshift, const int32_t* __restrict__ length,
@@ -281,7 +282,7 @@ k_bank_pages_page(gpsr_bank bk, const int32_t* __restrict__ table, int table_pag
     big = X::parts(big, max2);
     const int ex = big > 0.f && big < __builtin_inff() ? __builtin_amdgcn_frexp_expf(big) - 1 : 0;
     // through LDS, so that a row leaves in whole cache lines: stored from the accumulators, 32 bytes of 32 rows at a time, the
-    // stores were a third of the kernel
+    // stores were a third of the kernel's time
     typedef _Float16 h4 __attribute__((ext_vector_type(4)));
     _Float16* mine = (_Float16*)sm + wave * (32 * (D + 4));
     __syncthreads();
