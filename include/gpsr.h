@@ -385,8 +385,12 @@ int gpsr_active_sample(const double* data, int N, int D, int K, int n_pick, doub
  * Queries and outputs: [B][T][q_heads][dim] of `dtype`, q_heads a multiple of heads (query head h reads bank head
  * h / (q_heads / heads)).  skip (or NULL): [B][T][2] int32, query t of entry b does not see positions skip[0] <= r <
  * skip[1] (leave-one-image-out).  A query that sees no row gets zeros (lse -inf).  Rows that a query does not see have no
- * influence, whatever they hold.  Sums, maxima and exponentials are kept in 32 bits; queries and weights enter the matrix
- * units as one (bf16), two (f16) or three (f32) bf16 terms, so that each type keeps its own precision.
+ * influence, whatever they hold; of the rows that it does see, one whose key is NaN makes its output and lse NaN, one whose value
+ * is NaN in a group of 32 columns makes its output NaN in those columns.  Sums, maxima and exponentials are kept in 32 bits, for
+ * values of any held size; queries and weights enter the matrix units as one (bf16), two (f16) or three (f32) bf16 terms, so that
+ * each type keeps its own precision.  Logits too are 32-bit numbers: a key so large that |k|^2 / 2 leaves their range has no weight.
+ * All entry points run on the given stream and wait for nothing; they may be captured into a graph.  Overlapping calls may read one
+ * bank, each with a workspace of its own.  There are no gradients: a bank is filled and asked.
  */
 enum { GPSR_BF16 = 0, GPSR_F16 = 1, GPSR_F32 = 2 };
 typedef struct {
@@ -426,7 +430,7 @@ int gpsr_bank_attend(const gpsr_bank* bank, const int32_t* table, int B, int tab
  * The n_sel (1..64) best pages for each query and bank head: sel [B][T][heads][n_sel], logical page numbers (table
  * columns) in ascending order, -1 behind the last one.  Score of a page with centroid c: the sum over the query heads of
  * the bank head of q.c (- |c|^2 / 2 for RBF), in 64 bits; equal scores: the lower page first.  A page can be chosen if
- * its table entry exists and it has a row below length[b] that the query does not skip.
+ * its table entry exists, it has a row below length[b] that the query does not skip, and its centroid is a number.
  */
 size_t gpsr_bank_select_workspace_bytes(const gpsr_bank* bank, int B, int table_pages, int T, int q_heads, int n_sel, int dtype);
 int gpsr_bank_select(const gpsr_bank* bank, const int32_t* table, int B, int table_pages, const int32_t* length,
@@ -434,7 +438,9 @@ int gpsr_bank_select(const gpsr_bank* bank, const int32_t* table, int B, int tab
                      int32_t* sel, void* workspace, size_t workspace_bytes, void* stream);
 /*
  * Attention over chosen pages: sel [B][T][heads][n_sel] as gpsr_bank_select gives it.  Entries outside [0, table_pages)
- * and repeats of an earlier entry are passed over; the order is free.
+ * and repeats of an earlier entry are passed over; the order is free.  Where many queries share the pages, their pages' partial
+ * results are kept in the workspace in 32 bits; for bf16 outputs in f16 (11 bits) with a power of two for each row, so that a
+ * column 2^-14 times the row's largest loses bits.
  */
 size_t gpsr_bank_attend_pages_workspace_bytes(const gpsr_bank* bank, int B, int table_pages, int T, int q_heads, int n_sel, int dtype);
 int gpsr_bank_attend_pages(const gpsr_bank* bank, const int32_t* table, int B, int table_pages, const int32_t* length,

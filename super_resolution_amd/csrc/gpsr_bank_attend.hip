@@ -4,12 +4,12 @@
 // ---------------------------------------------------------------- attention over the whole bank
 // Columns are the (query, head) pairs that share a bank head.  A workgroup of NW waves walks the rows of its split of the
 // bank, KT at a time, NB x W of them in one step:
-//   WK = 1 (many queries; bound by the exponentials and the matrix units): all threads decode a tile to LDS once, then each
-//     wave multiplies it with W columns of its own;
-//     40 000 queries of 100 000 rows x 64 columns 1130 us, 900 TFLOP/s, where a library's product of 8192^3 reaches 1120;
-//   WK = NW (few queries; bound by reading the bank, and waiting for it: 12 queries to each of 8 banks of up to 180 000
-//     rows x 128 columns in 4 bits, 154 MB, 61 us, 2.5 TB/s): all waves have the same columns, each walks every NW-th tile in LDS of its
-//     own, so that none waits for another, and the results are joined at the end.
+//   WK = 1 (many queries): all threads decode a tile to LDS once, then each wave multiplies it with W columns of its own.
+//     Bound by the exponentials and the matrix units together: 40 000 queries of 100 000 rows x 64 columns 1130 to 1180 us, 870 to
+//     910 TFLOP/s, where a library's product of 8192^3 reaches 1120.
+//   WK = NW (few queries): all waves have the same columns, each walks every NW-th tile in LDS of its own, so that none waits
+//     for another, and the results are joined at the end.  Bound by reading the bank and waiting for it: 12 queries to each of 8
+//     banks of up to 180 000 rows x 128 columns in 4 bits, 154 MB, 61 us, 2.5 TB/s.
 // AHEAD: tiles under way besides the one in LDS.
 template <int DT, int BITS, int D, int W, int NW, int WK, int KT, int NB, int AHEAD>
 __global__ void __launch_bounds__(64 * NW, WK > 1 ? 2 : tile_waves(D, Terms<DT>::N, NB))

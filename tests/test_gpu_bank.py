@@ -731,3 +731,35 @@ def test_values_of_the_ends_of_the_range(dtype, size, T):
     sel = torch.as_tensor(c.rng.integers(0, 29, (1, T, 1, 16)).astype(np.int32))
     out, lse = ops.bank_attend_pages(c.bank, c.table, c.length, qd, sel.to(c.dev), 0.25, want_lse=True)
     c.check(q, out, lse, 0.25, lambda b, t, h: np.isin(np.arange(900) // 32, sel[b, t, h].numpy()))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("T", [2, 20, 100, 700])
+def test_a_value_group_that_is_not_a_number(dtype, T):
+    """NaN in columns 32 .. 63 of one row's value: those columns of the queries that see the row, and nothing else; T = 700 goes page by page."""
+    ops = _ops()
+    c = Case([900], 1, 96, 32, 4, "RBF", dtype, seed=T)
+    c.v[0, 333, 0, 40] = math.nan
+    ops.bank_write(c.bank, c.table, torch.zeros_like(c.length), c.length, c.k.to(c.dev), c.v.to(c.dev))
+    q, qd = c.queries(T, 1, dtype)
+    skip = torch.zeros(1, T, 2, dtype=torch.int32)
+    skip[:, ::2] = torch.tensor([333, 334])
+    sel = torch.as_tensor(c.rng.permuted(np.tile(np.arange(29), (T, 1)), axis=1)[None, :, None, :16].astype(np.int32)).contiguous()
+    every = lambda b, t, h: np.ones(900, bool)
+    chosen = lambda b, t, h: np.isin(np.arange(900) // 32, sel[b, t, h].numpy())
+    for see, f in ((every, lambda: ops.bank_attend(c.bank, c.table, c.length, qd, 0.25, skip=skip.to(c.dev), want_lse=True)),
+                   (chosen, lambda: ops.bank_attend_pages(c.bank, c.table, c.length, qd, sel.to(c.dev), 0.25, skip=skip.to(c.dev), want_lse=True))):
+        out, lse = f()
+        seen = torch.tensor([bool(see(0, t, 0)[333]) and t % 2 == 1 for t in range(T)])
+        gone = torch.isnan(out[0, :, 0]).cpu()
+        assert torch.equal(gone[:, 32:64], seen[:, None].expand(T, 32)) and not gone[:, :32].any() and not gone[:, 64:].any()
+        # the rest as if the row's value were zero there
+        c.hv = held(torch.nan_to_num(c.v).double().numpy(), 4)
+        c.hv[0, 333, 0, 32:64] = 0
+        fixed = out.clone()
+        for t in range(T):
+            if seen[t]:
+                e = softmax_mean(q[0, t, 0].double().numpy(), c.hk[0, :, 0], c.o[0, :, 0], c.hv[0, :, 0], see(0, t, 0), 0.25)[0]
+                fixed[0, t, 0, 32:64] = torch.as_tensor(e[32:64]).to(dtype)
+        r = np.arange(900)
+        c.check(q, fixed, lse, 0.25, lambda b, t, h: see(b, t, h) & ~((r >= int(skip[b, t, 0])) & (r < int(skip[b, t, 1]))))
