@@ -98,6 +98,16 @@ __device__ __forceinline__ void store8(typename Row<DT>::T* __restrict__ p, cons
   }
 }
 
+// over all lanes of a wave, by moves between neighbouring lanes, rows of 16 and halves
+template <class F>
+__device__ __forceinline__ float wave_all(float x, float none, const F& f) {
+#define STEP(ctrl) x = f(x, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(none), __float_as_int(x), ctrl, 0xf, 0xf, false)))
+  STEP(0x111); STEP(0x112); STEP(0x114); STEP(0x118);   // row_shr 1, 2, 4, 8
+  STEP(0x142); STEP(0x143);                             // row_bcast 15, 31
+#undef STEP
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+
 // ---- host side
 // every bank that the kernels accept; text for arg_fail, or NULL
 static inline const char* bank_wrong(const gpsr_bank* b) {

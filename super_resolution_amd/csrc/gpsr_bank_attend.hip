@@ -156,14 +156,16 @@ static Plan plan_of(const gpsr_bank* bk, int B, int table_pages, int T, int q_he
   p.groups = (C + p.cw - 1) / p.cw;
   const int64_t tiles = (((int64_t)table_pages * bk->page_rows) + p.kt - 1) / p.kt;
   // The splits that end soonest when `slots` workgroups run at a time, each paying for `own` tiles besides its share, and the join
-  // for some more.
+  // for some more; behind 64 of them, which one wave joins, four waves do, and the partials' way to memory and back counts (some
+  // 4 MB for a tile's time): 1 query of 100 000 rows 21 us instead of 30, 256 queries 43 instead of 63.
   const int64_t wgs = p.groups * bk->heads * B;
   const int64_t slots = p.few ? 512 : 256 * 4 * tile_waves(bk->dim, nt, many_nb(bk->dim, nt)) / nw;
   const int step = p.few ? 4 : 1, own = p.few ? 4 : 2;           // tiles that a workgroup takes at once
   int64_t best = -1;
   p.splits = 1;
-  for (int s = 1; s <= 64 && s * step <= (tiles > step ? tiles + step - 1 : step); ++s) {
-    const int64_t cost = ((wgs * s + slots - 1) / slots) * ((tiles + s * step - 1) / (s * step) + own) + (s > 1 ? 2 + s / 4 : 0);
+  for (int s = 1; s <= 256 && s * step <= (tiles > step ? tiles + step - 1 : step); s += s < 64 ? 1 : 32) {
+    const int64_t join = s == 1 ? 0 : s <= 64 ? 2 + s / 4 : 5 + s / 16 + C * bk->heads * B * (s - 64) * bk->dim / 500000;
+    const int64_t cost = ((wgs * s + slots - 1) / slots) * ((tiles + s * step - 1) / (s * step) + own) + join;
     if (best < 0 || cost < best) { best = cost; p.splits = s; }
   }
   // Or one workgroup on each CU with 64 rows at a time in twice the registers.  At 64 columns a tile of 128 rows takes a CU's two
@@ -203,9 +205,10 @@ static void launch_attend(const Plan& p, const gpsr_bank& bk, const int32_t* tab
 #undef ATTEND
   if (p.splits > 1) {
     const int64_t C = (int64_t)T * G;
-    hipLaunchKernelGGL((k_bank_join<DT, D, float>), dim3((unsigned)((C + 3) / 4), (unsigned)bk.heads, (unsigned)B), dim3(256), 0, st, sums,
-                       stats, T, G, bk.heads, C, p.splits, (size_t)p.splits * C, (size_t)1, (size_t)G, (size_t)C,
-                       (E*)out, lse);
+#define JOIN(WJ, wgs) hipLaunchKernelGGL((k_bank_join<DT, D, float, WJ>), dim3((unsigned)(wgs), (unsigned)bk.heads, (unsigned)B), dim3(256), \
+    0, st, sums, stats, T, G, bk.heads, C, p.splits, (size_t)p.splits * C, (size_t)1, (size_t)G, (size_t)C, (E*)out, lse)
+    if (p.splits <= 64) JOIN(1, (C + 3) / 4); else JOIN(4, C);
+#undef JOIN
   }
 }
 

@@ -11,6 +11,8 @@
 // on its place in a list, and the join runs in the order of the caller's numbers: results do not change.
 #include "gpsr_bank_tile.hpp"
 
+#include <cmath>
+
 // A query's rows are at most 64 pages of 256, so with weights of at most 2^-15 sums of any values stay in float32's range, and
 // products of the smallest held values (2^-111 in 4 bits) with the largest weights as well.
 static constexpr float ABOVE = 15.f;
@@ -315,9 +317,17 @@ static PagesPlan plan_of(const gpsr_bank* bk, int B, int table_pages, int T, int
   const int H = bk->heads, G = q_heads / H;
   p.entries = (int64_t)B * T * H * n_sel;
   p.buckets = (int64_t)B * H * table_pages;
-  // by page where a page serves 8 choices or more on average
-  p.by_page = p.buckets > 0 && p.entries * G >= 8 * p.buckets && p.entries * G >= 4096 && p.entries <= 0x7fffffff &&
-              (int64_t)H * table_pages <= PG_BUCKETS && p.buckets <= (1 << 24);
+  // By page where that is sooner.  A query (and 16 or 32 of its heads) costs 4 ns and 15 ps a row at 64 columns; by page, six
+  // launches 25 us more, a page 6.5 ns and a choice 0.08 ns; more columns cost (dim / 64)^1.5 times as much.  Both sides measured for
+  // 256 to 8192 queries of 4 or 16 pages, 16 or 64 rows, 32 to 6250 pages, 64 and 256 columns: 2048 queries of 16 x 64 rows
+  // 49 us by query, 45 by page (1563 pages); 512 queries 20 and 44; 512 queries of 256 columns 95 and 121, 1024 190 and 125; 8192
+  // queries of 16 x 16 rows of 6250 pages 72 and 86.
+  const int width = G <= 16 ? 16 : 32;
+  p.groups = (G + width - 1) / width;
+  const double wide = bk->dim / 64.0 * sqrt(bk->dim / 64.0);
+  const double by_query = wide * (double)B * T * H * p.groups * (4e-3 + 15e-6 * n_sel * bk->page_rows);
+  const double by_page = 25 + wide * (6.5e-3 * (double)(p.buckets < p.entries ? p.buckets : p.entries) + 0.08e-3 * (double)p.entries * G);
+  p.by_page = by_query > by_page && p.buckets > 0 && p.entries <= 0x7fffffff && (int64_t)H * table_pages <= PG_BUCKETS && p.buckets <= (1 << 24);
   if (p.by_page) {
     p.most_wgs = p.entries * G / 128 + (p.buckets < p.entries ? p.buckets : p.entries);
     p.chunks = (int)(((int64_t)T * H * n_sel + PG_CHUNK - 1) / PG_CHUNK);
@@ -332,8 +342,6 @@ static PagesPlan plan_of(const gpsr_bank* bk, int B, int table_pages, int T, int
     p.sums = at; at += (size_t)p.entries * G * bk->dim * (dtype == GPSR_BF16 ? 2 : 4);
     p.bytes = at;
   } else {
-    const int width = G <= 16 ? 16 : 32;
-    p.groups = (G + width - 1) / width;
     const int64_t wgs = (int64_t)B * T * H * p.groups, tiles = ((int64_t)n_sel * bk->page_rows + 127) / 128;
     int64_t s = 512 / wgs;
     if (s < 1) s = 1;

@@ -473,7 +473,11 @@ static SelectPlan plan_of(const gpsr_bank* bk, int B, int table_pages, int T, in
   SelectPlan p = {};
   const int64_t queries = (int64_t)B * T * bk->heads;
   p.J = table_pages;
-  p.screen = table_pages > 64 && queries >= 512;
+  // Exact scores for all pages take a round for each 256 queries, of 9 us and 0.8 for each 10 000 of pages x columns; the screen 55
+  // and 1.2, however many they are up to some thousands (measured: 1563 pages of 64 columns 22 us a round and 82, 100 pages 9 and
+  // 44, 1906 of 128 columns 30 and 95, 6000 of 256 columns 110 and 229).
+  const double work = (double)table_pages * bk->dim / 10000;
+  p.screen = table_pages > 64 && (double)((queries + 255) / 256) * (9 + 0.8 * work) > 55 + 1.2 * work;
   p.waves = !p.screen && table_pages > 64 ? 16 : 1;
   if (p.screen) {
     p.blocks = (table_pages + 31) / 32;

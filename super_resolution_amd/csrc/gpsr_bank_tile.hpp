@@ -540,32 +540,51 @@ __device__ __forceinline__ void tile_accumulate(const Tile<D, KT>& tile, int r0,
   }
 }
 
-// Joins the partial results of one column, at most 64: one wave per column.  First lane i weighs partial i, then the lanes
-// spread over four partials or more of several rows at a time (with the weights formed along the way each load waited for the one
-// before it: 30 against 9 us for 64 partials of 96 columns).  Column (t, g) of bank head bh has its n partials at
-// numbers bh * per_bh + t * per_t + g * per_g + i * per_i.
-template <int DT, int D, class P>
+// Joins the partial results of one column, at most 64 for each of its WJ waves (1: four columns a workgroup; 4).  First lane i weighs
+// partial i, then the lanes spread over four partials or more of several rows at a time (with the weights formed along the way
+// each load waited for the one before it: 30 against 9 us for 64 partials of 96 columns).  Column (t, g) of bank head bh has its n
+// partials at numbers bh * per_bh + t * per_t + g * per_g + i * per_i.
+template <int DT, int D, class P, int WJ = 1>
 __global__ void __launch_bounds__(256)
 k_bank_join(const P* __restrict__ sums, const f2v* __restrict__ stats, int T, int G, int H, int64_t C, int n, size_t per_bh,
             size_t per_g, size_t per_t, size_t per_i, typename Row<DT>::T* __restrict__ out, float* __restrict__ lse) {
-  const int lane = threadIdx.x & 63;
-  const int64_t c = (int64_t)blockIdx.x * 4 + wave_of(threadIdx.x);
-  if (c >= C) return;
+  // Weights and sums go from lane to lane through LDS, a wave's own part of it; reading other lanes' registers by
+  // permutes, 28 of them under way at a time, has given other lanes' values now and then in the f32 form of this kernel.
+  __shared__ float tops[4], ls[4], weight[4][64];
+  __shared__ __attribute__((aligned(16))) float part[4][64][4];
+  const auto sync = [] { asm volatile("" ::: "memory"); __builtin_amdgcn_wave_barrier(); };
+  const int lane = threadIdx.x & 63, wave = wave_of(threadIdx.x);
+  const int64_t c = WJ > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+  if (c >= C) return;            // WJ > 1: never
   const int h = blockIdx.y, b = blockIdx.z;
   const int64_t t = c / G;
   const int g = (int)(c - t * G), hq = h * G + g;
-  const size_t at = (size_t)(b * H + h) * per_bh + t * per_t + g * per_g;
+  if (WJ > 1) n = (n - wave + 3) / 4;               // this wave's: wave, wave + 4, ..
+  const size_t at = (size_t)(b * H + h) * per_bh + t * per_t + g * per_g + (WJ > 1 ? wave * per_i : 0);
+  if (WJ > 1) per_i *= 4;
   const P* p = sums + at * D;
   const size_t step = per_i * D;
   float m = -__builtin_inff(), l = 0.f;
   if (lane < n) { const f2v x = stats[at + lane * per_i]; m = x.x; l = x.y; }
   const unsigned long long used = __ballot(l != 0.f);      // the others saw nothing, and their sums were not written
   float top = l != 0.f ? m : -__builtin_inff();
-  for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  top = wave_all(top, -__builtin_inff(), max2);
+  if constexpr (WJ > 1) {
+    if (lane == 0) tops[wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  }
   float w = l != 0.f ? exp2f(m - (top == -__builtin_inff() ? 0.f : top)) : 0.f;
   l = l != 0.f ? l * w : 0.f;
-  for (int o = 32; o; o >>= 1) l += __shfl_xor(l, o);
+  l = wave_all(l, 0.f, add2);
+  if constexpr (WJ > 1) {
+    if (lane == 0) ls[wave] = l;
+    __syncthreads();
+    l = (ls[0] + ls[1]) + (ls[2] + ls[3]);
+  }
   w = l != 0.f ? w / l : 0.f;          // before the sums: a mean of values near the end of their range stays in it
+  weight[wave][lane] = w;
+  sync();
   // 4 columns a lane, R lanes a row, RP rows at a time
   constexpr int R = D / 4, RP = 64 / R;
   typedef P P4 __attribute__((ext_vector_type(4)));
@@ -579,18 +598,21 @@ k_bank_join(const P* __restrict__ sums, const f2v* __restrict__ stats, int T, in
     for (int j = 0; j < 4; ++j) {
       const int i = i0 + j * RP + row;
       const bool use = row < RP && (used >> (i & 63) & 1) && i < n;
-      const float wj = __shfl(w, i & 63);
+      const float wj = weight[wave][i & 63];
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[e] = use ? fmaf(wj, (float)y[j][e], acc[e]) : acc[e];
     }
   }
+  *(f4v*)part[wave][lane] = f4v{acc[0], acc[1], acc[2], acc[3]};
+  if constexpr (WJ > 1) __syncthreads(); else sync();
+  if (WJ > 1 && wave) return;
+  if (lane < R)
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    float all = acc[e];
+    for (int k = 1; k < WJ * RP; ++k) {
+      const f4v y = *(const f4v*)part[WJ > 1 ? k / RP : wave][lane + k % RP * R];
 #pragma unroll
-    for (int k = 1; k < RP; ++k) all += __shfl(acc[e], (lane + k * R) & 63);
-    acc[e] = all;
-  }
+      for (int e = 0; e < 4; ++e) acc[e] += y[e];
+    }
   typename Row<DT>::T* o = out + (((size_t)b * T + t) * (size_t)(H * G) + hq) * D + c4;
   if (lane < R) {
     if constexpr (DT == GPSR_F32) *(f4v*)o = f4v{acc[0], acc[1], acc[2], acc[3]};

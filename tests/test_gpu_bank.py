@@ -441,7 +441,9 @@ def _select_exact_many(c, q, n_sel, skip=None, rbf=True):
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("D,P,H,G,T,n_sel,lengths", [
     (64, 16, 1, 1, 700, 16, [16 * 400 - 3]), (32, 16, 2, 1, 301, 4, [1100, 16 * 70]), (128, 32, 1, 3, 513, 64, [32 * 300]),
-    (96, 16, 1, 2, 600, 33, [16 * 3000]), (192, 64, 1, 1, 520, 1, [64 * 80]), (256, 16, 1, 1, 550, 9, [16 * 99 + 1])])
+    (96, 16, 1, 2, 600, 33, [16 * 3000]), (192, 64, 1, 1, 520, 1, [64 * 80]), (256, 16, 1, 1, 550, 9, [16 * 99 + 1]),
+    (64, 16, 1, 1, 1700, 16, [16 * 400 - 3]), (32, 16, 2, 1, 430, 4, [1100, 16 * 70]), (128, 32, 1, 3, 1301, 64, [32 * 300]),
+    (192, 64, 1, 1, 1600, 1, [64 * 80]), (256, 16, 1, 1, 1550, 9, [16 * 99 + 1])])
 def test_select_for_many_queries(dtype, D, P, H, G, T, n_sel, lengths):
     """Enough queries and pages for the screen in fewer bits: the choice has to stay the one in 64."""
     ops = _ops()
@@ -455,11 +457,12 @@ def test_select_for_many_queries(dtype, D, P, H, G, T, n_sel, lengths):
         assert np.array_equal(got.cpu().numpy(), _select_exact_many(c, q, n_sel, skip, kernel == "RBF"))
 
 
-def test_select_for_many_queries_where_few_bits_do_not_tell():
+@pytest.mark.parametrize("T", [600, 1300])
+def test_select_for_many_queries_where_few_bits_do_not_tell(T):
     """Runs of equal pages (more candidates than the screen holds), scores one 32-bit step apart, pages of huge and of tiny norm,
     pages that are not numbers (never chosen), queries of zeros and of huge values."""
     ops = _ops()
-    P, n, T = 16, 700, 600
+    P, n = 16, 700
     for kernel in ("RBF", "LINEAR"):
         for dtype in (BF16, F32):
             c = Case([P * n], 1, 64, P, 4, kernel, dtype, seed=77)
@@ -518,7 +521,8 @@ def test_attend_pages(dtype, bits, D, P, H, G, T, S, lengths):
 @pytest.mark.parametrize("dtype,bits", [(BF16, 4), (F16, 8), (F32, 4)])
 @pytest.mark.parametrize("D,P,H,G,T,S,lengths", [
     (64, 64, 1, 1, 600, 8, [900]), (32, 16, 2, 2, 150, 8, [200, 77]), (128, 128, 1, 1, 700, 6, [1500]), (96, 32, 1, 3, 100, 16, [333]),
-    (256, 256, 1, 1, 1100, 4, [700]), (192, 16, 3, 1, 100, 16, [160])])
+    (256, 256, 1, 1, 1100, 4, [700]), (192, 16, 3, 1, 100, 16, [160]), (64, 64, 1, 1, 3100, 8, [900]), (32, 16, 2, 2, 4500, 8, [200, 77]),
+    (128, 128, 1, 1, 1400, 6, [1500]), (96, 32, 1, 3, 2300, 16, [333]), (192, 16, 3, 1, 400, 16, [160])])
 def test_attend_pages_of_many_queries(dtype, bits, D, P, H, G, T, S, lengths):
     """Enough queries for each page to be taken page by page; repeats, numbers outside the table and skipped rows among them."""
     ops = _ops()
@@ -596,7 +600,7 @@ def test_broadcast_queries_empty_batches_and_no_rows():
     assert (ops.bank_select(c.bank, c.table[:, :0].contiguous(), c.length, qd, 3) == -1).all()
 
 
-@pytest.mark.parametrize("T,n", [(1, 6000), (400, 900)])
+@pytest.mark.parametrize("T,n", [(1, 6000), (400, 900), (4500, 12000)])
 def test_captured_and_replayed_beside_eager_calls(T, n):
     """One graph of the whole set, replayed with new queries and rows, another graph of the same calls between, eager calls beside."""
     ops = _ops()
@@ -716,7 +720,7 @@ def test_a_row_far_above_all_before_it(dtype, D, T):
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("size", [2.5e38, 2.0 ** -108])
-@pytest.mark.parametrize("T", [3, 20, 100, 700])
+@pytest.mark.parametrize("T", [3, 20, 100, 700, 2900])
 def test_values_of_the_ends_of_the_range(dtype, size, T):
     """Means of 900 values of up to 6 * 2^125, whose sum is past float32's range; and of the smallest ones."""
     ops = _ops()
@@ -734,9 +738,9 @@ def test_values_of_the_ends_of_the_range(dtype, size, T):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-@pytest.mark.parametrize("T", [2, 20, 100, 700])
+@pytest.mark.parametrize("T", [2, 20, 100, 700, 1600])
 def test_a_value_group_that_is_not_a_number(dtype, T):
-    """NaN in columns 32 .. 63 of one row's value: those columns of the queries that see the row, and nothing else; T = 700 goes page by page."""
+    """NaN in columns 32 .. 63 of one row's value: those columns of the queries that see the row, and nothing else; T = 1600 goes page by page."""
     ops = _ops()
     c = Case([900], 1, 96, 32, 4, "RBF", dtype, seed=T)
     c.v[0, 333, 0, 40] = math.nan
@@ -763,3 +767,46 @@ def test_a_value_group_that_is_not_a_number(dtype, T):
                 fixed[0, t, 0, 32:64] = torch.as_tensor(e[32:64]).to(dtype)
         r = np.arange(900)
         c.check(q, fixed, lse, 0.25, lambda b, t, h: see(b, t, h) & ~((r >= int(skip[b, t, 0])) & (r < int(skip[b, t, 1]))))
+
+
+def test_which_way_the_pages_go():
+    """The calls above that are to go page by page do: only that way has a workspace where there are this many queries."""
+    from super_resolution_amd import _lib
+    ops, lib = _ops(), _lib.load()
+    for D, P, H, G, T, S, pages in ((64, 64, 1, 1, 3100, 8, 15), (32, 16, 2, 2, 4500, 8, 14), (128, 128, 1, 1, 1400, 6, 13), (96, 32, 1, 3, 2300, 16, 12),
+                                    (192, 16, 3, 1, 400, 16, 11), (256, 256, 1, 1, 1100, 4, 4), (64, 32, 1, 1, 2900, 16, 30), (96, 32, 1, 1, 1600, 16, 30)):
+        bank = ops.bank_alloc(pages, H, D, P, 4, ops.RBF)
+        ref, _, _ = ops._bank(bank, bank.offset.get_device())
+        B = 2 if T == 4500 else 1
+        assert lib.gpsr_bank_attend_pages_workspace_bytes(ref, B, pages, T, H * G, S, 0) > 0, (D, T)
+
+
+@pytest.mark.parametrize("dtype,D,bits", [(BF16, 64, 4), (F16, 96, 8), (F32, 32, 4), (BF16, 256, 4), (F32, 192, 8)])
+@pytest.mark.parametrize("T,G", [(1, 1), (3, 10), (70, 1)])
+def test_attend_of_few_queries_to_a_long_bank(dtype, D, bits, T, G):
+    """More partial results of a column than one wave joins."""
+    ops = _ops()
+    c = Case([70001], 1, D, 64, bits, "RBF", dtype, seed=D + T)
+    q, qd = c.queries(T, G, dtype)
+    skip = torch.zeros(1, T, 2, dtype=torch.int32)
+    skip[0, 0] = torch.tensor([0, 69000])         # most partials saw nothing
+    out, lse = ops.bank_attend(c.bank, c.table, c.length, qd, 0.25, skip=skip.to(c.dev), want_lse=True)
+    r = np.arange(70001)
+    c.check(q, out, lse, 0.25, lambda b, t, h: ~((r >= int(skip[b, t, 0])) & (r < int(skip[b, t, 1]))))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("D", [32, 64, 96])
+def test_many_joined_columns_are_the_same_every_time(dtype, D):
+    """Tens of thousands of columns joined from their partials, several times: every bit the same."""
+    ops = _ops()
+    c = Case([200, 77], 2, D, 16, 4, "RBF", dtype, seed=D)
+    q, qd = c.queries(9000, 2, dtype)
+    sel = torch.as_tensor(c.rng.integers(-2, 14, (2, 9000, 2, 4)).astype(np.int32)).to(c.dev)
+    first = ops.bank_attend_pages(c.bank, c.table, c.length, qd, sel, 0.2, want_lse=True)
+    for _ in range(4):
+        assert all(torch.equal(a, b) for a, b in zip(first, ops.bank_attend_pages(c.bank, c.table, c.length, qd, sel, 0.2, want_lse=True)))
+    part = [ops.bank_attend_pages(c.bank, c.table, c.length, qd[:, t:t + 50].contiguous(), sel[:, t:t + 50].contiguous(), 0.2) for t in range(0, 9000, 50)]
+    u, uw = torch.finfo(dtype).eps / 2, U_W[dtype]
+    # the same rows taken query by query: two roundings of each kind, of means of values of at most 5
+    assert (torch.cat(part, 1).double() - first[0].double()).abs().max() <= 5 * 2 * (u + uw + 2.0 ** -12)
