@@ -439,8 +439,7 @@ int gpsr_bank_select(const gpsr_bank* bank, const int32_t* table, int B, int tab
 /*
  * Attention over chosen pages: sel [B][T][heads][n_sel] as gpsr_bank_select gives it.  Entries outside [0, table_pages)
  * and repeats of an earlier entry are passed over; the order is free.  Where many queries share the pages, their pages' partial
- * results are kept in the workspace in 32 bits; for bf16 outputs in f16 (11 bits) with a power of two for each row, so that a
- * column 2^-14 times the row's largest loses bits.
+ * results are kept in the workspace in 32 bits.
  */
 size_t gpsr_bank_attend_pages_workspace_bytes(const gpsr_bank* bank, int B, int table_pages, int T, int q_heads, int n_sel, int dtype);
 int gpsr_bank_attend_pages(const gpsr_bank* bank, const int32_t* table, int B, int table_pages, const int32_t* length,

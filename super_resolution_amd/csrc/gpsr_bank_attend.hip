@@ -205,7 +205,7 @@ static void launch_attend(const Plan& p, const gpsr_bank& bk, const int32_t* tab
 #undef ATTEND
   if (p.splits > 1) {
     const int64_t C = (int64_t)T * G;
-#define JOIN(WJ, wgs) hipLaunchKernelGGL((k_bank_join<DT, D, float, WJ>), dim3((unsigned)(wgs), (unsigned)bk.heads, (unsigned)B), dim3(256), \
+#define JOIN(WJ, wgs) hipLaunchKernelGGL((k_bank_join<DT, D, WJ>), dim3((unsigned)(wgs), (unsigned)bk.heads, (unsigned)B), dim3(256), \
     0, st, sums, stats, T, G, bk.heads, C, p.splits, (size_t)p.splits * C, (size_t)1, (size_t)G, (size_t)C, (E*)out, lse)
     if (p.splits <= 64) JOIN(1, (C + 3) / 4); else JOIN(4, C);
 #undef JOIN

@@ -6,7 +6,10 @@
 //   by page: the choices are turned over (for each page the list of queries that chose it), a workgroup takes one page and
 //     128 of its queries, writes each query's partial result for that page, and a last kernel joins each query's partials.
 //     Pages are decoded once per 128 queries and all columns work, at the price of writing and reading the partials: 40 000
-//     queries with 16 pages each 109 us (count 14, shares 10, scan 5, fill 7, products 59, join 19), by query 4380.
+//     queries with 16 pages each 125 us (count 15, shares 10, scan 5, fill 8, products 68, join 25), by query 4380.  Partials are
+//     f32 whatever the caller's type: their sums are weighed against each other by their keys alone, and a column may be any
+//     number of powers of two under its neighbours (in f16 with a power of two a row, products took 59 and the join 19 us, but
+//     columns 2^-25 under the row's largest became zero).
 // Within a chunk of choices the lists' order comes from counters in LDS and may differ from run to run; a partial does not depend
 // on its place in a list, and the join runs in the order of the caller's numbers: results do not change.
 #include "gpsr_bank_tile.hpp"
@@ -206,24 +209,18 @@ k_bank_pages_fill(const int32_t* __restrict__ sel, int n_sel, int table_pages, i
   list[start[(size_t)b * buckets + bucket] + share + r] = (int)(th / H * n_sel + (e - th * n_sel));
 }
 
-// What a partial is kept in: bf16 outputs take f16 (11 bits against the 8 that the result has), scaled by a power of two so
-// that the largest of its columns is between 1 and 2, which goes into its reference; half the bytes to write and read again.
-template <int DT> struct Partial { typedef float T; };
-template <> struct Partial<GPSR_BF16> { typedef _Float16 T; };
-static constexpr int page_lds(int d, int kt) { return tile_lds(d, kt) > 256 * (d + 4) ? tile_lds(d, kt) : 256 * (d + 4); }
-
-// 32 rows at a time and three waves per SIMD: the workgroups are short and mostly wait (59 us for 40 000 queries x 16 pages of
-// 64 rows of 64 columns, 178 TFLOP/s; all 64 rows of a page at a time 4 us more, two waves 15 more, four with spills 30 more)
+// 32 rows at a time and three waves per SIMD: the workgroups are short and mostly wait (68 us for 40 000 queries x 16 pages of
+// 64 rows of 64 columns, 154 TFLOP/s; measured with f16 partials, at 59 us, all 64 rows of a page at a time took 4 us more, two
+// waves 15 more, four with spills 30 more)
 template <int DT, int BITS, int D, int KT>
 __global__ void __launch_bounds__(256, tile_waves(D, Terms<DT>::N, 1) > 3 ? 3 : tile_waves(D, Terms<DT>::N, 1))
 k_bank_pages_page(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, int pshift, const int32_t* __restrict__ length,
                   const typename Row<DT>::T* __restrict__ q, int T, int G, Strides qs, bool qwide, int n_sel, float scale,
                   const int32_t* __restrict__ skip, const int* __restrict__ start, const int* __restrict__ wgs, int buckets,
-                  const int* __restrict__ owner, const int* __restrict__ list, typename Partial<DT>::T* __restrict__ sums,
-                  f2v* __restrict__ stats) {
+                  const int* __restrict__ owner, const int* __restrict__ list, float* __restrict__ sums, f2v* __restrict__ stats) {
   constexpr int NT = Terms<DT>::N, NB = 1, CW = 128, W = 32;
   typedef Geo<W> X;
-  __shared__ __attribute__((aligned(16))) char sm[page_lds(D, KT)];
+  __shared__ __attribute__((aligned(16))) char sm[tile_lds(D, KT)];
   Tile<D, KT> tile(sm);
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_of(tid), part = lane / W, col = lane % W;
   const int w = blockIdx.x;
@@ -273,46 +270,12 @@ k_bank_pages_page(gpsr_bank bk, const int32_t* __restrict__ table, int table_pag
   }
   st.spoil();
   const size_t at = ((size_t)bh * T * n_sel + id) * G + g;
-  if constexpr (DT != GPSR_BF16) {
-    if (there) st.store_partial(sums + at * D, stats + at, part);
-  } else {
-    float big = 0.f;
-#pragma unroll
-    for (int d = 0; d < D / W; ++d)
-#pragma unroll
-      for (int e = 0; e < X::E; ++e) big = fmaxf(big, fabsf(st.o[d][e]));
-    big = X::parts(big, max2);
-    const int ex = big > 0.f && big < __builtin_inff() ? __builtin_amdgcn_frexp_expf(big) - 1 : 0;
-    // through LDS, so that a row leaves in whole cache lines: stored from the accumulators, 32 bytes of 32 rows at a time, the
-    // stores were a third of the kernel's time
-    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-    _Float16* mine = (_Float16*)sm + wave * (32 * (D + 4));
-    __syncthreads();
-#pragma unroll
-    for (int d = 0; d < D / W; ++d)
-#pragma unroll
-      for (int e = 0; e < X::E; e += 4) {
-        h4 y;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = (_Float16)ldexpf(st.o[d][e + j], -ex);
-        *(h4*)(mine + col * (D + 4) + d * W + X::row(part, e)) = y;
-      }
-    const float all = X::parts(st.l, add2);
-    if (there && part == 0) stats[at] = f2v{st.m + (float)ex, ldexpf(all, -ex)};
-    __syncthreads();
-    constexpr int PER = D / 4;             // lanes for a row
-#pragma unroll 4
-    for (int i = lane; i < 32 * PER; i += 64) {
-      const int r = i / PER;
-      const size_t to = __shfl(at, r);
-      if (__shfl((int)there, r)) *(h4*)(sums + to * D + i % PER * 4) = *(const h4*)(mine + r * (D + 4) + i % PER * 4);
-    }
-  }
+  if (there) st.store_partial(sums + at * D, stats + at, part);
 }
 
 // ---------------------------------------------------------------- host
 struct PagesPlan { bool by_page; int groups, splits, chunks; int64_t entries, buckets, most_wgs; size_t hist, rank, start, wgs, owner, list, stats, sums, bytes; };
-static PagesPlan plan_of(const gpsr_bank* bk, int B, int table_pages, int T, int q_heads, int n_sel, int dtype) {
+static PagesPlan plan_of(const gpsr_bank* bk, int B, int table_pages, int T, int q_heads, int n_sel) {
   PagesPlan p = {};
   const int H = bk->heads, G = q_heads / H;
   p.entries = (int64_t)B * T * H * n_sel;
@@ -339,7 +302,7 @@ static PagesPlan plan_of(const gpsr_bank* bk, int B, int table_pages, int T, int
     p.owner = at; at += align256((size_t)p.most_wgs * 4);
     p.list = at; at += align256((size_t)p.entries * 4);
     p.stats = at; at += align256((size_t)p.entries * G * sizeof(f2v));
-    p.sums = at; at += (size_t)p.entries * G * bk->dim * (dtype == GPSR_BF16 ? 2 : 4);
+    p.sums = at; at += (size_t)p.entries * G * bk->dim * sizeof(float);
     p.bytes = at;
   } else {
     const int64_t wgs = (int64_t)B * T * H * p.groups, tiles = ((int64_t)n_sel * bk->page_rows + 127) / 128;
@@ -353,7 +316,7 @@ static PagesPlan plan_of(const gpsr_bank* bk, int B, int table_pages, int T, int
 
 extern "C" size_t gpsr_bank_attend_pages_workspace_bytes(const gpsr_bank* bank, int B, int table_pages, int T, int q_heads, int n_sel, int dtype) {
   if (bank_wrong(bank) || B <= 0 || T <= 0 || table_pages < 0 || q_heads < 1 || q_heads % bank->heads || n_sel < 1 || n_sel > 64 || !type_ok(dtype)) return 0;
-  return plan_of(bank, B, table_pages, T, q_heads, n_sel, dtype).bytes;
+  return plan_of(bank, B, table_pages, T, q_heads, n_sel).bytes;
 }
 
 template <int DT, int BITS, int D>
@@ -373,13 +336,12 @@ static void launch_pages(const PagesPlan& p, const gpsr_bank& bk, const int32_t*
     if (G <= 16) QUERY(16); else QUERY(32);
 #undef QUERY
     if (p.splits > 1)
-      hipLaunchKernelGGL((k_bank_join<DT, D, float>), join, dim3(256), 0, st, sums, stats, T, G, H, C, p.splits, (size_t)p.splits * C, (size_t)1,
+      hipLaunchKernelGGL((k_bank_join<DT, D>), join, dim3(256), 0, st, sums, stats, T, G, H, C, p.splits, (size_t)p.splits * C, (size_t)1,
                          (size_t)p.splits * G, (size_t)G, (E*)out, lse);
     return;
   }
   int *count = (int*)ws, *rank = (int*)(ws + p.rank), *start = (int*)(ws + p.start), *wgs = (int*)(ws + p.wgs), *list = (int*)(ws + p.list);
-  typedef typename Partial<DT>::T P;
-  P* sums = (P*)(ws + p.sums);
+  float* sums = (float*)(ws + p.sums);
   f2v* stats = (f2v*)(ws + p.stats);
   int* owner = (int*)(ws + p.owner);
   const int64_t per = (int64_t)T * H * n_sel;
@@ -395,7 +357,7 @@ static void launch_pages(const PagesPlan& p, const gpsr_bank& bk, const int32_t*
     table_pages, pshift, length, (const E*)q, T, G, qs, qwide, n_sel, scale, skip, start, wgs, (int)p.buckets, owner, list, sums, stats)
   if (bk.page_rows <= 32) PAGE(32); else PAGE(64);
 #undef PAGE
-  hipLaunchKernelGGL((k_bank_join<DT, D, P>), join, dim3(256), 0, st, sums, stats, T, G, H, C, n_sel, (size_t)n_sel * C, (size_t)1,
+  hipLaunchKernelGGL((k_bank_join<DT, D>), join, dim3(256), 0, st, sums, stats, T, G, H, C, n_sel, (size_t)n_sel * C, (size_t)1,
                      (size_t)n_sel * G, (size_t)G, (E*)out, lse);
 }
 
@@ -407,7 +369,7 @@ extern "C" int gpsr_bank_attend_pages(const gpsr_bank* bank, const int32_t* tabl
   if (const char* w = attend_wrong(bank, table, B, table_pages, length, q, dtype, q_heads, qst, scale, out)) return arg_fail(w);
   if (!sel) return arg_fail("bank_attend_pages: null pointer");
   if (n_sel < 1 || n_sel > 64) return arg_fail("bank_attend_pages: n_sel must be in 1..64");
-  const PagesPlan p = plan_of(bank, B, table_pages, T, q_heads, n_sel, dtype);
+  const PagesPlan p = plan_of(bank, B, table_pages, T, q_heads, n_sel);
   if (!grid_fits(p.by_page ? p.most_wgs : (int64_t)T * p.groups * p.splits, 256) || !grid_fits(((int64_t)T * (q_heads / bank->heads) + 3) / 4, 256))
     return arg_fail("bank_attend_pages: too many queries for one call");
   if (workspace_bytes < p.bytes || (p.bytes && !workspace)) return arg_fail("workspace too small");

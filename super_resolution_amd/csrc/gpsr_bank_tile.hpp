@@ -544,9 +544,9 @@ __device__ __forceinline__ void tile_accumulate(const Tile<D, KT>& tile, int r0,
 // partial i, then the lanes spread over four partials or more of several rows at a time (with the weights formed along the way
 // each load waited for the one before it: 30 against 9 us for 64 partials of 96 columns).  Column (t, g) of bank head bh has its n
 // partials at numbers bh * per_bh + t * per_t + g * per_g + i * per_i.
-template <int DT, int D, class P, int WJ = 1>
+template <int DT, int D, int WJ = 1>
 __global__ void __launch_bounds__(256)
-k_bank_join(const P* __restrict__ sums, const f2v* __restrict__ stats, int T, int G, int H, int64_t C, int n, size_t per_bh,
+k_bank_join(const float* __restrict__ sums, const f2v* __restrict__ stats, int T, int G, int H, int64_t C, int n, size_t per_bh,
             size_t per_g, size_t per_t, size_t per_i, typename Row<DT>::T* __restrict__ out, float* __restrict__ lse) {
   // Weights and sums go from lane to lane through LDS, a wave's own part of it; reading other lanes' registers by
   // permutes, 28 of them under way at a time, has given other lanes' values now and then in the f32 form of this kernel.
@@ -562,7 +562,7 @@ k_bank_join(const P* __restrict__ sums, const f2v* __restrict__ stats, int T, in
   if (WJ > 1) n = (n - wave + 3) / 4;               // this wave's: wave, wave + 4, ..
   const size_t at = (size_t)(b * H + h) * per_bh + t * per_t + g * per_g + (WJ > 1 ? wave * per_i : 0);
   if (WJ > 1) per_i *= 4;
-  const P* p = sums + at * D;
+  const float* p = sums + at * D;
   const size_t step = per_i * D;
   float m = -__builtin_inff(), l = 0.f;
   if (lane < n) { const f2v x = stats[at + lane * per_i]; m = x.x; l = x.y; }
@@ -587,20 +587,19 @@ k_bank_join(const P* __restrict__ sums, const f2v* __restrict__ stats, int T, in
   sync();
   // 4 columns a lane, R lanes a row, RP rows at a time
   constexpr int R = D / 4, RP = 64 / R;
-  typedef P P4 __attribute__((ext_vector_type(4)));
   const int row = lane / R, c4 = (lane - row * R) * 4;
   float acc[4] = {0, 0, 0, 0};
   for (int i0 = 0; i0 < n; i0 += 4 * RP) {
-    P4 y[4];
+    f4v y[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = *(const P4*)(p + min(i0 + j * RP + row, n - 1) * step + c4);
+    for (int j = 0; j < 4; ++j) y[j] = *(const f4v*)(p + min(i0 + j * RP + row, n - 1) * step + c4);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int i = i0 + j * RP + row;
       const bool use = row < RP && (used >> (i & 63) & 1) && i < n;
       const float wj = weight[wave][i & 63];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] = use ? fmaf(wj, (float)y[j][e], acc[e]) : acc[e];
+      for (int e = 0; e < 4; ++e) acc[e] = use ? fmaf(wj, y[j][e], acc[e]) : acc[e];
     }
   }
   *(f4v*)part[wave][lane] = f4v{acc[0], acc[1], acc[2], acc[3]};
