@@ -11,8 +11,8 @@
 //            fit), sorted across a wave by (score, page).
 // With Cauchy-Schwarz, and u = 2^-8 the half step of bf16: two terms of q and of c and their three larger products leave out
 // at most 3 u^2 |q||c| (one exact term of q: u^2 |q||c|); the 32-bit sum of n products and the offset o adds (n + 2) 2^-23
-// (|q||c| + |o|), n = 3 dim (2 dim); 1e-35 (1 + |q| + |c|) covers subnormal terms.  Norms above 1e18 or not finite are not
-// screened: their pages are all candidates.
+// (|q||c| + |o|), n = 3 dim (2 dim); 1e-35 (1 + |q| + |c|) covers subnormal terms.  Norms above 1e18 are not screened: their pages
+// are all candidates.  A page whose centroid is not a number is passed over, as one that does not exist: it is never chosen.
 // 40 000 queries of 64 columns, 1563 pages, 16 of them: prepare 5, screen 104, pick 25 us, one product after the other 127 us
 // at its rate in 32 bf16 terms 14; exact scores for all pages took 14 900 us.
 #include "gpsr_bank_tile.hpp"
@@ -34,28 +34,35 @@ k_bank_select_prepare(gpsr_bank bk, const int32_t* __restrict__ table, int J, in
   const int64_t lp = (int64_t)r * blocks + k;
   int64_t page = -1;
   if (lp < J && (lp << pshift) < length[b]) page = table[(size_t)b * J + lp];
-  const bool there = page >= 0 && page < bk.pages;
+  bool there = page >= 0 && page < bk.pages;
   __bf16* to = hl + ((size_t)(b * H + h) * blocks + k) * 32 * (2 * D) + r * 8;
+  f4v y[D / 32];        // 4 columns at a time
   double sq = 0.0;
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) {    // 4 columns at a time
+  for (int i = 0; i < D / 32; ++i) {
+    y[i] = f4v{0, 0, 0, 0};
+    if (there) y[i] = *(const f4v*)(bk.centroid + ((size_t)page * H + h) * D + (i * 8 + part) * 4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sq = fma((double)y[i][j], (double)y[i][j], sq);
+  }
+  sq += __shfl_xor(sq, 1); sq += __shfl_xor(sq, 2); sq += __shfl_xor(sq, 4);
+  there = there && sq == sq;      // a page that is not a number is never chosen: here as if it were not there
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
     const int c = (i * 8 + part) * 4;
-    f4v y = {0, 0, 0, 0};
-    if (there) y = *(const f4v*)(bk.centroid + ((size_t)page * H + h) * D + c);
     bf2 hi[2], lo[2];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const __bf16 t = (__bf16)y[j];
-      hi[j / 2][j % 2] = t; lo[j / 2][j % 2] = (__bf16)(y[j] - (float)t);
-      sq = fma((double)y[j], (double)y[j], sq);
+      const float x = there ? y[i][j] : 0.f;
+      const __bf16 t = (__bf16)x;
+      hi[j / 2][j % 2] = t; lo[j / 2][j % 2] = (__bf16)(x - (float)t);
     }
     const int at = (c / 16) * 1024 + (c / 8 % 2) * 256 + c % 8;
     *(u2v*)(to + at) = u2v{__builtin_bit_cast(unsigned, hi[0]), __builtin_bit_cast(unsigned, hi[1])};
     *(u2v*)(to + at + 512) = u2v{__builtin_bit_cast(unsigned, lo[0]), __builtin_bit_cast(unsigned, lo[1])};
   }
-  sq += __shfl_xor(sq, 1); sq += __shfl_xor(sq, 2); sq += __shfl_xor(sq, 4);
   const float o = bk.kernel_id == GPSR_KERNEL_RBF ? (float)(-0.5 * G * sq) : 0.f;
-  // a norm that is too large (or NaN) makes the block's bound infinite
+  // a norm that is too large makes the block's bound infinite
   float norm = !there ? 0.f : sq * (double)G < 1e36 ? (float)sqrt(sq) : __builtin_inff();
   float big = there && norm < __builtin_inff() ? fabsf(o) : 0.f;
   if (part == 0) off[((size_t)(b * H + h) * blocks + k) * 32 + r] = there && norm < __builtin_inff() ? o : -__builtin_inff();

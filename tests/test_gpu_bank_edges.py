@@ -90,3 +90,48 @@ def test_columns_at_both_ends_of_the_range(dtype, T):
     q, qd = c.queries(T, 1, dtype)
     out, lse = ops.bank_attend(c.bank, c.table, c.length, qd, 0.25, want_lse=True)
     c.check(q, out, lse, 0.25, lambda b, t, h: np.ones(900, bool))
+
+
+# ------------------------------------------------------------ the screen of bank_select
+def _screened(c, qd, n_sel):
+    """bank_select through the library with a workspace of our own: the choice, and how many candidates the screen left each query
+    (-1: more than it keeps, -2: the choice was clear)."""
+    import ctypes
+    from super_resolution_amd import _lib
+    ops, lib = _ops(), _lib.load()
+    ref, H, D = ops._bank(c.bank, c.dev.index)
+    B, T, Hq, _ = qd.shape
+    J, code = c.table.shape[1], {BF16: 0, F16: 1, F32: 2}[qd.dtype]
+    n = lib.gpsr_bank_select_workspace_bytes(ref, B, J, T, Hq, n_sel, code)
+    assert n > 0, "not screened"
+    ws = torch.zeros(n, dtype=torch.uint8, device=c.dev)
+    sel = torch.empty(B, T, H, n_sel, dtype=torch.int32, device=c.dev)
+    st = (ctypes.c_int64 * 3)(*qd.stride()[:3])
+    _lib.check(lib.gpsr_bank_select(ref, c.table.data_ptr(), B, J, c.length.data_ptr(), qd.data_ptr(), code, T, Hq, st, n_sel, None,
+                                    sel.data_ptr(), ws.data_ptr(), n, ops._stream()), "gpsr_bank_select")
+    # the workspace ends with a count for each query and, aligned to 256 bytes, the candidates: 64 for n_sel <= 16
+    up = lambda x: -(-x // 256) * 256
+    at = n - up(B * T * H * 64 * 4) - up(B * T * H * 4)
+    return sel, ws[at:at + B * T * H * 4].view(torch.int32)
+
+
+@pytest.mark.parametrize("kernel", ["RBF", "LINEAR"])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_pages_that_are_not_numbers_do_not_blind_the_screen(dtype, kernel):
+    """A NaN in the keys of a few pages: they are not chosen, and the others are told apart as without them."""
+    ops = _ops()
+    c = Case([16 * 700], 1, 64, 16, 4, kernel, dtype, seed=12)
+    q, qd = c.queries(1300, 1, dtype)
+    bad = c.rng.choice(700, 6, replace=False)
+    for j in bad:
+        c.k[0, j * 16 + 5, 0, 3] = math.nan
+    ops.bank_write(c.bank, c.table, torch.zeros_like(c.length), c.length, c.k.to(c.dev), c.v.to(c.dev))
+    sel, count = _screened(c, qd, 16)
+    assert not np.isin(sel.cpu().numpy(), bad).any() and (sel >= 0).all()
+    assert float((count == -1).float().mean()) < 0.01
+    far = c.bank.centroid.clone()
+    gone = torch.as_tensor(c.table_np[0, bad].astype(np.int64)).to(c.dev)
+    # the same choice as from a table without these pages
+    table = c.table.clone()
+    table[0, torch.as_tensor(bad.astype(np.int64)).to(c.dev)] = -1
+    assert torch.equal(sel, ops.bank_select(c.bank, table, c.length, qd, 16)) and torch.isnan(far[gone]).any()
