@@ -69,11 +69,12 @@ k_bank_attend(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, 
     pages(f, i + 2 * WK * AHEAD);
     const unsigned p0 = i * KT;
     tile_marks<D, KT, KT>(tile, 0, i + 1, st, [&](int r) { return !(p0 + r >= lo && p0 + r < hi); });
+    const bool weightless = tile.weightless(i + 1);
     const bool skips = skip && __ballot(lo < p0 + KT && hi > p0 && lo < hi);
 #pragma unroll 1
     for (int r = 0; r < KT; r += W * NB) {
       typename X::Acc s[NB];
-      tile_logits<D, KT, NT, NB, W>(tile, r, col, part, qf, s);
+      tile_logits<D, KT, NT, NB, W>(tile, r, col, part, weightless, qf, s);
       if (skips) {
         asm volatile("");        // not to be computed for the tiles that nobody skips
 #pragma unroll

@@ -86,7 +86,7 @@ k_bank_pages_query(gpsr_bank bk, const int32_t* __restrict__ table, int table_pa
     };
     tile_marks<D, KT, 32>(tile, wrow, i + 1, st, [&](int r) { return !skips(i * KT + wrow + r); });
     typename X::Acc s[NB];
-    tile_logits<D, KT, NT, NB, W>(tile, wrow, col, part, qf, s);
+    tile_logits<D, KT, NT, NB, W>(tile, wrow, col, part, tile.weightless(i + 1), qf, s);
     if (lo < hi) {
       asm volatile("");
 #pragma unroll
@@ -253,10 +253,11 @@ k_bank_pages_page(gpsr_bank bk, const int32_t* __restrict__ table, int table_pag
     f.pages(rows, v + KT, tid);
     f.codes(bk, h, pshift, v + KT, tid);
     tile_marks<D, KT, KT>(tile, 0, v / KT + 1, st, [&](int r) { return !(pos0 + v + r >= lo && pos0 + v + r < hi); });
+    const bool weightless = tile.weightless(v / KT + 1);
 #pragma unroll 1
     for (int r = 0; r < KT; r += 32) {
       typename X::Acc s[NB];
-      tile_logits<D, KT, NT, NB, W>(tile, r, col, part, qf, s);
+      tile_logits<D, KT, NT, NB, W>(tile, r, col, part, weightless, qf, s);
       if (skip && __ballot(lo < pos0 + v + KT && hi > pos0 + v && lo < hi)) {
         asm volatile("");
 #pragma unroll

@@ -96,7 +96,8 @@ struct Tile {
   float* off;
   // A value group that is NaN is held as zeros, so that it cannot reach queries that do not see its row (0 * NaN); who does
   // see it is told by its mark: mark[row][group] = the number of the tile in which it is NaN, mark[KT][0] = of the last such
-  // tile.  Numbers of earlier tiles need no clearing.
+  // tile.  Numbers of earlier tiles need no clearing.  mark[KT][1] = the last tile with a row that has no weight (offset -inf:
+  // it does not exist, or its key is past the range): its product with a query may still be infinite or NaN.
   unsigned* mark;
   __device__ Tile(char* sm) {
     k = (uint16_t*)sm; v = k + KT * KS; off = (float*)(v + D * VS); mark = (unsigned*)(off + KT);
@@ -104,7 +105,10 @@ struct Tile {
   // where slot s of column c lies
   __device__ __forceinline__ static int at(int c, int s) { return c * VS + (s ^ (((c ^ (c >> 3)) & SWZ) << 3)); }
   __device__ void clear_marks(int tid, int threads) {
-    for (int i = tid; i < KT * (D / 32) + 1; i += threads) mark[i] = 0;
+    for (int i = tid; i < KT * (D / 32) + 2; i += threads) mark[i] = 0;
+  }
+  __device__ __forceinline__ bool weightless(unsigned number) const {
+    return __builtin_amdgcn_readfirstlane(mark[KT * (D / 32) + 1]) == (int)number;
   }
 };
 
@@ -156,7 +160,8 @@ struct OnePage {
 
 // 32 columns of a row's key to LDS; MASKED: unless `there`, zeros and an offset of -inf instead
 template <int BITS, int D, int KT, bool MASKED>
-__device__ __forceinline__ void store_keys(const Tile<D, KT>& tile, int r, int g, const unsigned* w, const unsigned* sc, bool there) {
+__device__ __forceinline__ void store_keys(const Tile<D, KT>& tile, int r, int g, const unsigned* w, const unsigned* sc, bool there,
+                                           unsigned number) {
   constexpr int CW = BITS / 4;
   u4v* dst = (u4v*)(tile.k + r * Tile<D, KT>::KS + g * 32);
   const float s = scale_of(!MASKED || there ? sc[0] : 127u);
@@ -165,7 +170,11 @@ __device__ __forceinline__ void store_keys(const Tile<D, KT>& tile, int r, int g
     const unsigned w0 = !MASKED || there ? w[CW * j] : 0u, w1 = !MASKED || there ? w[CW * j + CW - 1] : 0u;
     dst[j] = u4v{pair<BITS, 0>(w0, w1, s), pair<BITS, 1>(w0, w1, s), pair<BITS, 2>(w0, w1, s), pair<BITS, 3>(w0, w1, s)};
   }
-  if (g == 0) tile.off[r] = !MASKED || there ? __uint_as_float(sc[1]) : -__builtin_inff();
+  if (g == 0) {
+    const float o = !MASKED || there ? __uint_as_float(sc[1]) : -__builtin_inff();
+    tile.off[r] = o;
+    if (o == -__builtin_inff()) tile.mark[KT * (D / 32) + 1] = number;
+  }
 }
 
 // 8 columns of 4 rows' values to LDS, transposed; MASKED: zeros for rows r + left and behind
@@ -265,7 +274,7 @@ struct Fetch {
       const int u = tid + NTH * i;
       if (!EVEN && u >= 2 * U) continue;
       const int r = row(i, tid);
-      if (keys(i, tid)) store_keys<BITS, D, KT, true>(tile, r, u % (D / 32), w[i], sc[i], fpage[i] >= 0);
+      if (keys(i, tid)) store_keys<BITS, D, KT, true>(tile, r, u % (D / 32), w[i], sc[i], fpage[i] >= 0, number);
       else store_values<BITS, D, KT, W, true>(tile, r, (u - U) % (D / 8), w[i], sc[i], fleft[i], number);
     }
   }
@@ -335,7 +344,7 @@ struct WaveFetch {
       for (int i = 0; i < N; ++i) {
         const int u = lane + 64 * i, r = row(i, lane);
         const bool half = r < 16 ? there[0] : there[1];
-        if (keys(i, lane)) store_keys<BITS, D, KT, M>(tile, r, u % G, w[i], sc[i], half && r < left);
+        if (keys(i, lane)) store_keys<BITS, D, KT, M>(tile, r, u % G, w[i], sc[i], half && r < left, number);
         else store_values<BITS, D, KT, W, M>(tile, r, (u - U) % (D / 8), w[i], sc[i], half ? min(left - r, 4) : 0, number);
       }
     };
@@ -343,10 +352,11 @@ struct WaveFetch {
   }
 };
 
-// raw logits q.k + offset of NB x W rows (from r0 on) for a wave's W columns
+// raw logits q.k + offset of NB x W rows (from r0 on) for a wave's W columns; weightless: rows with an offset of -inf are among the
+// tile's, and their logits are -inf whatever the query holds
 template <int D, int KT, int NT, int NB, int W>
-__device__ __forceinline__ void tile_logits(const Tile<D, KT>& tile, int r0, int col, int part, const bf8 (&qf)[NT][D / Geo<W>::STEP],
-                                            typename Geo<W>::Acc (&s)[NB]) {
+__device__ __forceinline__ void tile_logits(const Tile<D, KT>& tile, int r0, int col, int part, bool weightless,
+                                            const bf8 (&qf)[NT][D / Geo<W>::STEP], typename Geo<W>::Acc (&s)[NB]) {
   typedef Geo<W> X;
 #pragma unroll
   for (int kb = 0; kb < NB; ++kb) {
@@ -363,6 +373,17 @@ __device__ __forceinline__ void tile_logits(const Tile<D, KT>& tile, int r0, int
 #pragma unroll
       for (int t = 0; t < NT; ++t) s[kb] = X::mul(a, qf[t][d], s[kb]);
     }
+  }
+  if (weightless) {
+    asm volatile("");        // not to be computed for the other tiles
+#pragma unroll
+    for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+      for (int e = 0; e < X::E; e += 4) {
+        const f4v a = *(const f4v*)(tile.off + r0 + kb * W + X::row(part, e));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[kb][e + j] = a[j] == -__builtin_inff() ? a[j] : s[kb][e + j];
+      }
   }
 }
 

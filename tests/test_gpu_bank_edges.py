@@ -135,3 +135,56 @@ def test_pages_that_are_not_numbers_do_not_blind_the_screen(dtype, kernel):
     table = c.table.clone()
     table[0, torch.as_tensor(bad.astype(np.int64)).to(c.dev)] = -1
     assert torch.equal(sel, ops.bank_select(c.bank, table, c.length, qd, 16)) and torch.isnan(far[gone]).any()
+
+
+# ------------------------------------------------------------ keys past the range, queries that are not numbers
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_keys_past_the_range_have_no_weight(dtype, bits):
+    """RBF keys whose |k|^2 / 2 is past float32's range, and queries for which q.k is as well."""
+    ops = _ops()
+    for T in (3, 20, 100, 2900):
+        c = Case([900], 1, 64, 32, bits, "RBF", F32, seed=T)
+        huge = np.zeros(900, bool)
+        huge[[0, 17, 33, 34, 500, 899]] = True
+        sign = torch.as_tensor(c.rng.choice([-1.0, 1.0], size=(1, 6, 1, 64))).float()
+        sign[:, ::2] = 1.0
+        c.k[:, huge] = sign * 2.9e38
+        ops.bank_write(c.bank, c.table, torch.zeros_like(c.length), c.length, c.k.to(c.dev), c.v.to(c.dev))
+        assert int(torch.isinf(c.bank.offset).sum()) == 6
+        c.k[:, huge] = 0
+        c.hk, c.hv = held(c.k.double().numpy(), bits), held(c.v.double().numpy(), bits)
+        c.o = -0.5 * (c.hk ** 2).sum(-1)
+        q, _ = c.queries(T, 1, dtype)
+        q[0, 0], q[0, 1], q[0, 2] = 0, 1, 4
+        qd = q.to(c.dev)
+        out, lse = ops.bank_attend(c.bank, c.table, c.length, qd, 0.25, want_lse=True)
+        c.check(q[:, :100], out[:, :100], lse[..., :100], 0.25, lambda b, t, h: ~huge)
+        sel, seen = _choices(c, T, 16)
+        out, lse = ops.bank_attend_pages(c.bank, c.table, c.length, qd, sel, 0.25, want_lse=True)
+        c.check(q[:, :100], out[:, :100], lse[..., :100], 0.25, lambda b, t, h: seen(b, t, h) & ~huge)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("T", [2, 20, 100, 6000])
+def test_queries_that_are_not_numbers_and_see_no_row(dtype, T):
+    """Zeros and -inf for whoever sees no row, whatever the query holds; NaN for such a query that does see one; nothing for others."""
+    ops = _ops()
+    c = Case([75], 1, 64, 16, 4, "RBF", dtype, seed=3)
+    q, _ = c.queries(T, 1, dtype)
+    q[0, 0], q[0, 1, 0, ::2] = math.nan, math.inf
+    qd = q.to(c.dev)
+    skip = torch.zeros(1, T, 2, dtype=torch.int32, device=c.dev)
+    skip[0, :2, 1] = 75                                    # all rows, and none behind them
+    pages = torch.arange(5, dtype=torch.int32, device=c.dev).expand(1, T, 1, 5).repeat(1, 1, 1, 3)
+    gone = torch.full_like(c.table, -1)
+    gone[0, 0] = c.table[0, 0]
+    first = torch.tensor([[[0, 16]]], dtype=torch.int32, device=c.dev).expand(1, T, 2).contiguous()
+    for table, sk, none in ((c.table, skip, 2), (torch.full_like(c.table, -1), None, T), (gone, first, T)):
+        for out, lse in (ops.bank_attend(c.bank, table, c.length, qd, 0.25, skip=sk, want_lse=True),
+                         ops.bank_attend_pages(c.bank, table, c.length, qd, pages, 0.25, skip=sk, want_lse=True)):
+            assert not out[:, :none].any() and (lse[..., :none] == -math.inf).all()
+            assert torch.isfinite(out).all() and torch.isfinite(lse[..., none:]).all()
+    for out, lse in (ops.bank_attend(c.bank, c.table, c.length, qd, 0.25, want_lse=True),
+                     ops.bank_attend_pages(c.bank, c.table, c.length, qd, pages, 0.25, want_lse=True)):
+        assert torch.isnan(out[:, :2]).all() and torch.isnan(lse[..., :2]).all() and torch.isfinite(out[:, 2:]).all()
