@@ -52,8 +52,9 @@ __device__ __forceinline__ typename Row<DT>::T from_f32(float y) {
   if constexpr (DT == GPSR_BF16) return bf16_rne(y); else return (typename Row<DT>::T)y;
 }
 
-// y[8] as NT bf16 terms, each the rounding of what the terms before left over
-template <int NT>
+// y[8] as NT bf16 terms, each the rounding of what the terms before left over.  LARGE: y may be finite and beyond the largest bf16
+// number, to which its first term then stops short.
+template <int NT, bool LARGE = false>
 __device__ __forceinline__ void split_terms(const float* y, bf8* t) {
   float r[8];
 #pragma unroll
@@ -62,7 +63,7 @@ __device__ __forceinline__ void split_terms(const float* y, bf8* t) {
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      t[n][i] = (__bf16)r[i];
+      t[n][i] = (__bf16)(LARGE && n == 0 && fabsf(r[i]) < __builtin_inff() ? __builtin_amdgcn_fmed3f(r[i], -0x1.fep127f, 0x1.fep127f) : r[i]);
       if (n + 1 < NT) r[i] -= (float)t[n][i];
     }
 }
@@ -76,7 +77,7 @@ __device__ __forceinline__ void load_query(const typename Row<DT>::T* __restrict
     float y[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (there) load8<DT>(p + s * Geo<W>::STEP + part * 8, wide, y);
     bf8 t[NT];
-    split_terms<NT>(y, t);
+    split_terms<NT, DT == GPSR_F32>(y, t);
 #pragma unroll
     for (int n = 0; n < NT; ++n) qf[n][s] = t[n];
   }

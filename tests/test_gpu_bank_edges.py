@@ -188,3 +188,15 @@ def test_queries_that_are_not_numbers_and_see_no_row(dtype, T):
     for out, lse in (ops.bank_attend(c.bank, c.table, c.length, qd, 0.25, want_lse=True),
                      ops.bank_attend_pages(c.bank, c.table, c.length, qd, pages, 0.25, want_lse=True)):
         assert torch.isnan(out[:, :2]).all() and torch.isnan(lse[..., :2]).all() and torch.isfinite(out[:, 2:]).all()
+
+
+def test_float32_queries_at_the_end_of_their_range():
+    """A query that a bf16 term does not reach (above 2^128 - 2^119): keys of 2^-100 bring its logits back."""
+    ops = _ops()
+    c = Case([300], 1, 64, 16, 8, "LINEAR", F32, seed=6)
+    c.k *= 2.0 ** -100
+    _rewrite(c, "LINEAR")
+    q = torch.full((1, 40, 1, 64), torch.finfo(F32).max)
+    q[0, ::2] *= -1
+    out, lse = ops.bank_attend(c.bank, c.table, c.length, q.to(c.dev), 2.0 ** -27, want_lse=True)
+    c.check(q, out, lse, 2.0 ** -27, lambda b, t, h: np.ones(300, bool))
