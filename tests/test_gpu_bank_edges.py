@@ -26,6 +26,13 @@ def _choices(c, T, S):
     return torch.as_tensor(np.ascontiguousarray(sel)).to(c.dev), seen
 
 
+def _pages_workspace(c, T, Hq, S, dtype):
+    from super_resolution_amd import _lib
+    ref, _, _ = _ops()._bank(c.bank, c.dev.index)
+    code = {BF16: 0, F16: 1, F32: 2}[dtype]
+    return _lib.load().gpsr_bank_attend_pages_workspace_bytes(ref, 1, c.table.shape[1], T, Hq, S, code)
+
+
 # 40 queries go by query, 2900 by page (test_which_way_the_pages_go in test_gpu_bank.py)
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("T", [40, 2900])
@@ -200,3 +207,54 @@ def test_float32_queries_at_the_end_of_their_range():
     q[0, ::2] *= -1
     out, lse = ops.bank_attend(c.bank, c.table, c.length, q.to(c.dev), 2.0 ** -27, want_lse=True)
     c.check(q, out, lse, 2.0 ** -27, lambda b, t, h: np.ones(300, bool))
+
+
+# ------------------------------------------------------------ many calls at once and again
+def test_two_streams_at_once_with_many_queries():
+    """Enough queries for the screen and for the way by page, whose lists and partials lie in a workspace."""
+    ops = _ops()
+    T = 4500
+    cs = [Case([12000], 1, 64, 64, 4, "RBF", BF16, seed=40 + i) for i in range(2)]
+    qs = [c.queries(T, 1, BF16)[1] for c in cs]
+    for c, q in zip(cs, qs):
+        _screened(c, q, 8)
+        assert _pages_workspace(c, T, 1, 8, BF16) > 0
+
+    def run(c, q):
+        sel = ops.bank_select(c.bank, c.table, c.length, q, 8)
+        return (sel, *ops.bank_attend_pages(c.bank, c.table, c.length, q, sel, 0.2, want_lse=True))
+    want = [run(c, q) for c, q in zip(cs, qs)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cs]
+    got = [[], []]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(run(cs[i], qs[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_many_columns_are_the_same_every_time_in_the_other_ways_too(dtype):
+    """Banks shared out and joined, pages by query, and the choice by the screen and without it: every bit the same."""
+    ops = _ops()
+    c = Case([5003], 1, 32, 16, 4, "RBF", dtype, seed=9)
+    q, qd = c.queries(20000, 1, dtype)
+
+    def calls():
+        yield ops.bank_attend(c.bank, c.table, c.length, qd, 0.2, want_lse=True)
+        sel = ops.bank_select(c.bank, c.table, c.length, qd, 8)
+        yield (sel,)
+        yield (torch.cat([ops.bank_select(c.bank, c.table, c.length, qd[:, t:t + 500], 8) for t in range(0, 20000, 500)], 1),)
+        for t in range(0, 2000, 200):
+            yield ops.bank_attend_pages(c.bank, c.table, c.length, qd[:, t:t + 200], sel[:, t:t + 200].contiguous(), 0.2, want_lse=True)
+        for t in range(0, 3000, 20):
+            yield ops.bank_attend(c.bank, c.table, c.length, qd[:, t:t + 20], 0.2, want_lse=True)
+    first = list(calls())
+    assert torch.equal(first[1][0], first[2][0])
+    for _ in range(3):
+        for a, b in zip(first, calls()):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
