@@ -104,15 +104,21 @@ SIGNATURES = {
 
 
 def build(force=False):
-    """Compile csrc/*.hip for gfx950 (one object per file, side by side) into libgpsr.so (in-tree)."""
+    """Compile csrc/*.hip for gfx950 (one object per file, side by side) into libgpsr.so (in-tree); what was built by another
+    compiler or with other flags (build/command) is built again."""
     from concurrent.futures import ThreadPoolExecutor
     heads = glob.glob(os.path.join(_CSRC, "*.hpp")) + [os.path.join(os.path.dirname(_HERE), "include", "gpsr.h")]
     srcs = sorted(glob.glob(os.path.join(_CSRC, "*.hip")))
     newer = lambda path, than: os.path.exists(path) and all(os.path.getmtime(path) >= os.path.getmtime(t) for t in than)
+    objdir = os.path.join(_HERE, "build")
+    stamp, command = os.path.join(objdir, "command"), " ".join([HIPCC] + HIPCC_FLAGS)
+    if not os.path.exists(stamp) or open(stamp).read() != command:
+        force = True
     if not force and newer(LIB_PATH, srcs + heads):
         return LIB_PATH
-    objdir = os.path.join(_HERE, "build")
     os.makedirs(objdir, exist_ok=True)
+    if os.path.exists(stamp):
+        os.remove(stamp)            # until everything is built by it
     flags = [f for f in HIPCC_FLAGS if f != "-shared"]
 
     def compile_one(src):
@@ -124,6 +130,8 @@ def build(force=False):
     with ThreadPoolExecutor(max_workers=min(8, len(srcs))) as pool:
         objs = list(pool.map(compile_one, srcs))
     subprocess.run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB_PATH] + objs, check=True, cwd=_HERE)
+    with open(stamp, "w") as f:
+        f.write(command)
     return LIB_PATH
 
 

@@ -1,6 +1,6 @@
 // chol16_inv (the 16x16 factor + inverse on the serial chain of k_pivot) in isolation: one wave, ITER dependent calls,
 // cycles per call, and a check of the result against a host Cholesky + inverse.
-//   hipcc -O3 --offload-arch=gfx950 -ffp-contract=off -I super_resolution_amd/csrc -o /tmp/chol16_bench tools/chol16_bench.hip
+//   hipcc -O3 --offload-arch=gfx950 -ffp-contract=off -Xclang -target-feature -Xclang -packed-fp32-ops -I super_resolution_amd/csrc -o /tmp/chol16_bench tools/chol16_bench.hip
 #include "gpsr_kernels.hpp"
 #include <cstdio>
 #include <cmath>

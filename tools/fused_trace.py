@@ -1,5 +1,6 @@
 """Where the cycles of a k_fit_fused workgroup go, by role.  Needs the instrumented build:
     hipcc -O3 --offload-arch=gfx950 -shared -fPIC -ffp-contract=off -DGPSR_FUSED_TRACE=1 \
+          -Xclang -target-feature -Xclang -packed-fp32-ops \
           -o tools/bin/libgpsr_ftrace.so super_resolution_amd/csrc/*.hip
     GPSR_LIB=$PWD/tools/bin/libgpsr_ftrace.so python tools/fused_trace.py [B n kernel_id iters]
 """

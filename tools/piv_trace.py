@@ -1,5 +1,6 @@
 """Where the cycles of a k_pivot workgroup go, by phase.  Needs the instrumented build:
     hipcc -O3 --offload-arch=gfx950 -shared -fPIC -ffp-contract=off -DGPSR_PIV_TRACE=1 \
+          -Xclang -target-feature -Xclang -packed-fp32-ops \
           -o super_resolution_amd/libgpsr_trace.so super_resolution_amd/csrc/*.hip
     GPSR_LIB=$PWD/super_resolution_amd/libgpsr_trace.so python tools/piv_trace.py [B N]
 """

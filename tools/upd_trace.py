@@ -1,6 +1,7 @@
 """Where the cycles of a k_update2 compute wave go (off-diagonal trailing tiles, the bulk of the launch).
 Needs the instrumented build:
     hipcc -O3 --offload-arch=gfx950 -shared -fPIC -ffp-contract=off -DGPSR_UPD_TRACE=<1|2|3> \
+          -Xclang -target-feature -Xclang -packed-fp32-ops \
           -o super_resolution_amd/libgpsr_trace.so super_resolution_amd/csrc/*.hip
     GPSR_LIB=$PWD/super_resolution_amd/libgpsr_trace.so python tools/upd_trace.py [B N]
 """

@@ -1,6 +1,6 @@
 // f64 VALU issue rate of a lone wave on gfx950 (dependent / independent chains, full / partial EXEC) and v_rsq_f64.
 // Measured: 7.5 cycles per v_fma_f64 dependent or not, no gain from 16 active lanes, rsq ~17.
-//   hipcc -O3 --offload-arch=gfx950 -o tools/bin/valu_lat tools/valu_lat.hip
+//   hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -o tools/bin/valu_lat tools/valu_lat.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 __global__ void __launch_bounds__(64) k(double* out, unsigned long long* cyc, int mode) {
