@@ -411,7 +411,8 @@ _I64x3 = ctypes.c_int64 * 3
 class Bank(NamedTuple):
     """Example windows in 4 or 8 bits (gpsr_bank of include/gpsr.h): the arrays of a bank, which bank_write fills and the
     other bank_* functions read.  codes [pages,H,P,D*bits/8] uint8, scales [pages,H,P,D/32] uint8, offset [pages,H,P]
-    and centroid [pages,H,D] float32; kernel_id RBF or LINEAR.  bank_alloc makes an empty one."""
+    and centroid [pages,H,D] float32; kernel_id RBF or LINEAR.  bank_alloc makes an empty one.
+    There are no gradients through a bank: rows and queries that ask for one are refused."""
     k_codes: torch.Tensor
     k_scales: torch.Tensor
     v_codes: torch.Tensor
@@ -443,6 +444,11 @@ def _ptr(t, dtype, dev):
     if t.get_device() != dev or t.dtype is not dtype or not t.is_contiguous():
         return _p(t, dtype)
     return t.data_ptr()
+
+
+def _no_grad(t, what):
+    if t.requires_grad and torch.is_grad_enabled():
+        raise _lib.GpsrError(f"{what}: there are no gradients through an example bank (detach it, or call under torch.no_grad())")
 
 
 def _bank_device(t):
@@ -480,6 +486,7 @@ def _strided(t, B, H, D, dev, what):
         raise _lib.GpsrError(f"{what}: the columns must be contiguous")
     if t.get_device() != dev:
         _p(t.as_strided((0,), (1,)))     # says what is wrong
+    _no_grad(t, what)
     return t.data_ptr(), code, _I64x3(sb, st, sh)
 
 
@@ -605,6 +612,7 @@ def bank_windows(img, side, dim, dtype=torch.bfloat16, centre=False):
     H, W = img.shape
     if dtype not in _BANK_TYPES:
         raise _lib.GpsrError(f"bank_windows: expected bfloat16, float16 or float32, got {dtype}")
+    _no_grad(img, "bank_windows: img")
     n = max(H - side + 1, 0) * max(W - side + 1, 0)
     out = torch.empty((1, n, 1, dim), dtype=dtype, device=img.device)
     _lib.check(lib.gpsr_bank_windows(_p(img, torch.float64), H, W, side, int(centre), out.data_ptr(), _BANK_TYPES[dtype], dim, _stream()),
@@ -620,6 +628,8 @@ def bank_blend(img, detail, side):
     dim = detail.shape[-1]
     if detail.numel() != n * dim or detail.dtype not in _BANK_TYPES:
         raise _lib.GpsrError(f"bank_blend: detail {tuple(detail.shape)} {detail.dtype} does not fit {H} x {W} and side {side}")
+    _no_grad(img, "bank_blend: img")
+    _no_grad(detail, "bank_blend: detail")
     out = torch.empty_like(img)
     _lib.check(lib.gpsr_bank_blend(_p(img, torch.float64), H, W, side, _p(detail), _BANK_TYPES[detail.dtype], dim, out.data_ptr(),
                                    _stream()), "gpsr_bank_blend")

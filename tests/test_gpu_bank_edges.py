@@ -258,3 +258,29 @@ def test_many_columns_are_the_same_every_time_in_the_other_ways_too(dtype):
     for _ in range(3):
         for a, b in zip(first, calls()):
             assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+# ------------------------------------------------------------ refusals
+def test_rows_and_queries_that_ask_for_gradients_are_refused():
+    from super_resolution_amd import _lib
+    from super_resolution_amd.bank import ExampleBank
+    ops = _ops()
+    c = Case([100], 1, 64, 16, 4, "RBF", F32, seed=1)
+    q = c.queries(3, 1, F32)[1].requires_grad_()
+    k, v = c.k.to(c.dev), c.v.to(c.dev)
+    sel = torch.zeros(1, 3, 1, 4, dtype=torch.int32, device=c.dev)
+    img = torch.zeros(9, 9, dtype=torch.float64, device=c.dev)
+    rows = torch.zeros(1, 9, 1, 64, device=c.dev)
+    b = ExampleBank(100, 49).append(k[0, :, 0, :49], v[0, :, 0, :49])
+    calls = [lambda: ops.bank_attend(c.bank, c.table, c.length, q, 1.0), lambda: ops.bank_select(c.bank, c.table, c.length, q, 2),
+             lambda: ops.bank_attend_pages(c.bank, c.table, c.length, q, sel, 1.0), lambda: b.predict(q[0, :, 0, :49], 1.0),
+             lambda: ops.bank_write(c.bank, c.table, torch.zeros_like(c.length), c.length, k.clone().requires_grad_(), v),
+             lambda: ops.bank_write(c.bank, c.table, torch.zeros_like(c.length), c.length, k, v.clone().requires_grad_()),
+             lambda: ops.bank_windows(img.clone().requires_grad_(), 7, 64), lambda: ops.bank_blend(img.clone().requires_grad_(), rows, 7),
+             lambda: ops.bank_blend(img, rows.clone().requires_grad_(), 7)]
+    for i, f in enumerate(calls):
+        with pytest.raises(_lib.GpsrError, match="gradients"):
+            f()
+            pytest.fail(f"call {i} was not refused")
+        with torch.no_grad():
+            f()
