@@ -420,7 +420,7 @@ int gpsr_bank_read(const gpsr_bank* bank, const int32_t* table, int B, int table
                    const int32_t* count, void* k, void* v, int dtype, int T, void* stream);
 /*
  * Attention over the whole bank.  q strides qst = {batch, row, head} in elements; out contiguous; lse [B][q_heads][T] f32
- * or NULL: log sum_r exp(scale * (q.k_r + offset_r)).  length[b]: rows of entry b.  scale > 0.
+ * or NULL: log sum_r exp(scale * (q.k_r + offset_r)).  length[b]: rows of entry b.  0 < scale <= 2.35e38.
  * Two banks' answers are joined by their lse.
  */
 size_t gpsr_bank_attend_workspace_bytes(const gpsr_bank* bank, int B, int table_pages, int T, int q_heads, int dtype);

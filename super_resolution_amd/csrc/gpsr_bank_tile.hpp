@@ -657,7 +657,8 @@ static inline const char* attend_wrong(const gpsr_bank* bank, const int32_t* tab
   if (B > 65535) return "bank_attend: more than 65535 entries";
   if (table_pages < 0) return "bank_attend: table_pages";
   if (q_heads < 1 || q_heads > 65535 || q_heads % bank->heads) return "bank_attend: query heads must be a multiple of the bank's heads, up to 65535";
-  if (!(scale > 0.f) || scale > 3.0e38f) return "bank_attend: scale must be positive and finite";
+  // the kernels take powers of two: scale * log2 e has to be finite too
+  if (!(scale > 0.f) || scale > 2.35e38f) return "bank_attend: scale must be positive and at most 2.35e38";
   if ((uintptr_t)out & 15) return "bank_attend: out must be 16-byte aligned";
   return nullptr;
 }
