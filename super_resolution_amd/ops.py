@@ -473,6 +473,11 @@ def _bank(bank, dev):
                                   _ptr(cent, f32, dev), pages, H, P, D, bits, kernel_id)), H, D
 
 
+def _rows_fit(n, what):
+    if not 0 <= n < 2 ** 31:      # ctypes would pass the low 32 bits on
+        raise _lib.GpsrError(f"{what}: from 0 to 2^31 - 1 rows in one call, got {n}")
+
+
 def _strided(t, B, H, D, dev, what):
     """Pointer, dtype code and (first three) element strides of a [B,T,H,D] tensor whose columns are contiguous (H None: any)."""
     shape = t.shape
@@ -481,6 +486,7 @@ def _strided(t, B, H, D, dev, what):
     code = _BANK_TYPES.get(t.dtype)
     if code is None:
         raise _lib.GpsrError(f"{what}: expected bfloat16, float16 or float32, got {t.dtype}")
+    _rows_fit(shape[1], what)
     sb, st, sh, sd = t.stride()
     if sd != 1:
         raise _lib.GpsrError(f"{what}: the columns must be contiguous")
@@ -501,6 +507,8 @@ def _bank_index(table, per_entry, dev, what):
     if len(shape) != 2 or not fits:
         raise _lib.GpsrError(f"{what}: expected a [B,J] table and [B] integers, got {tuple(table.shape)}, "
                              f"{[tuple(t.shape) for t in per_entry]}")
+    if shape[1] >= 2 ** 31:
+        raise _lib.GpsrError(f"{what}: a table of at most 2^31 - 1 pages an entry, got {shape[1]}")
     i32 = torch.int32
     return (_ptr(table, i32, dev), *[_ptr(t, i32, dev) for t in per_entry])
 
@@ -528,6 +536,7 @@ def bank_read(bank, table, start, count, rows, dtype=torch.float32):
     code = _BANK_TYPES.get(dtype)
     if code is None:
         raise _lib.GpsrError(f"bank_read: expected bfloat16, float16 or float32, got {dtype}")
+    _rows_fit(rows, "bank_read")
     B, J = table.shape
     k = table.new_empty((B, rows, H, D), dtype=dtype)
     v = torch.empty_like(k)

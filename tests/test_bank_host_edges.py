@@ -1,5 +1,6 @@
 """Example bank, without a GPU: arguments at the ends of what the kernels take."""
 import pytest
+import torch
 
 from test_bank_host import _calls, _struct
 
@@ -10,3 +11,16 @@ def test_scales_whose_power_of_two_form_is_not_finite_are_refused(scale):
     calls, lib = _calls(_struct(), scale=scale)
     for name in ("attend", "pages"):
         assert calls[name]() == -1 and b"scale" in lib.gpsr_last_error()
+
+
+@pytest.mark.parametrize("rows", [2 ** 31, 2 ** 32 + 5])
+def test_more_rows_than_a_call_can_count_are_refused(rows):
+    """The library counts rows in 32 bits: 2^32 + 5 of them would have been 5.  One row repeated, so that they need no memory."""
+    from super_resolution_amd import _lib, ops
+    q = torch.zeros(64).expand(1, rows, 1, 64)
+    with pytest.raises(_lib.GpsrError, match="rows"):
+        ops._strided(q, 1, None, 64, q.get_device(), "bank_attend: q")
+    assert ops._strided(q[:, :7], 1, None, 64, q.get_device(), "bank_attend: q")[1] == 2
+    table = torch.empty(1, rows, dtype=torch.int32, device="meta")
+    with pytest.raises(_lib.GpsrError, match="pages"):
+        ops._bank_index(table, (torch.zeros(1, dtype=torch.int32),), -1, "bank_attend")

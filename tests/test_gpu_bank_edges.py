@@ -284,3 +284,12 @@ def test_rows_and_queries_that_ask_for_gradients_are_refused():
             pytest.fail(f"call {i} was not refused")
         with torch.no_grad():
             f()
+
+
+def test_numbers_of_rows_that_a_read_cannot_have_are_refused():
+    from super_resolution_amd import _lib
+    ops = _ops()
+    c = Case([100], 1, 32, 16, 4, "RBF", F32, seed=1)
+    for rows in (-1, 2 ** 31, 2 ** 32 + 5):
+        with pytest.raises(_lib.GpsrError, match="rows"):
+            ops.bank_read(c.bank, c.table, torch.zeros_like(c.length), c.length, rows, BF16)
