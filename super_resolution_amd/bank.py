@@ -72,9 +72,12 @@ class ExampleBank:
 
     def choose_scale(self, scales, sample=4096, pages=None):
         """The scale of `scales` whose predictions of the bank's own values are best when a row, and what lies within a page of it,
-        is left out (mean squared error over `sample` rows spread over the bank)."""
+        is left out (mean squared error over `sample` rows spread over the bank; what is not a number is passed over, and refused if
+        nothing else is there)."""
         at = torch.arange(0, self.rows, max(1, self.rows // sample), device=self.length.device)
         keys, values = (x[at] for x in self.read(0, self.rows))
         skip = torch.stack([at - self.page_rows, at + self.page_rows + 1], -1).to(torch.int32)
-        errors = [float((self.predict(keys, s, pages, skip) - values).square().mean()) for s in scales]
+        errors = [float((self.predict(keys, s, pages, skip) - values).square().nanmean()) for s in scales]
+        if any(e != e for e in errors):
+            raise _lib.GpsrError(f"ExampleBank: none of its {self.rows} rows has a prediction and a value that are numbers")
         return scales[min(range(len(errors)), key=errors.__getitem__)]

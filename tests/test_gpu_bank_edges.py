@@ -293,3 +293,19 @@ def test_numbers_of_rows_that_a_read_cannot_have_are_refused():
     for rows in (-1, 2 ** 31, 2 ** 32 + 5):
         with pytest.raises(_lib.GpsrError, match="rows"):
             ops.bank_read(c.bank, c.table, torch.zeros_like(c.length), c.length, rows, BF16)
+
+
+def test_choose_scale_passes_over_what_is_not_a_number_and_refuses_an_empty_bank():
+    """One example whose value is NaN, seen by every query in 32 columns: the others decide, as without it."""
+    from super_resolution_amd import _lib
+    from super_resolution_amd.bank import ExampleBank
+    rng = np.random.default_rng(4)
+    dev = torch.device("cuda", torch.cuda.current_device())
+    k = torch.as_tensor(rng.normal(size=(700, 49)).astype(np.float32)).to(dev) * 0.2
+    v = torch.tanh(k @ torch.as_tensor(rng.normal(size=(49, 49)).astype(np.float32) * 0.25).to(dev))
+    assert ExampleBank(700, 49, bits=8).append(k, v).choose_scale([1e-6, 5.0], sample=300) == 5.0
+    v[333, 40] = math.nan
+    assert ExampleBank(700, 49, bits=8).append(k, v).choose_scale([1e-6, 5.0], sample=300) == 5.0
+    for b in (ExampleBank(10, 49), ExampleBank(700, 49).append(k, torch.full_like(v, math.nan))):
+        with pytest.raises(_lib.GpsrError, match="numbers"):
+            b.choose_scale([1.0, 2.0])
