@@ -49,7 +49,9 @@ class ExampleBank:
         return self
 
     def read(self, start, count, dtype=torch.float32):
-        """The keys and values that rows start .. start + count - 1 hold, [count,heads,dim] each."""
+        """The keys and values that rows start .. start + count - 1 hold, [count,heads,dim] each; zeros behind the last row."""
+        if start < 0:
+            raise _lib.GpsrError(f"ExampleBank: rows are counted from 0, got {start}")
         k, v = ops.bank_read(self.bank, self.table, self._one(start), self._one(min(count, self.rows - start)), count, dtype)
         return k[0, ..., :self.dim], v[0, ..., :self.dim]
 

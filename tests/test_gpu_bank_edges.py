@@ -309,3 +309,16 @@ def test_choose_scale_passes_over_what_is_not_a_number_and_refuses_an_empty_bank
     for b in (ExampleBank(10, 49), ExampleBank(700, 49).append(k, torch.full_like(v, math.nan))):
         with pytest.raises(_lib.GpsrError, match="numbers"):
             b.choose_scale([1.0, 2.0])
+
+
+def test_example_bank_reads_from_its_first_row_on():
+    from super_resolution_amd import _lib
+    from super_resolution_amd.bank import ExampleBank
+    dev = torch.device("cuda", torch.cuda.current_device())
+    k = torch.ones(10, 49, device=dev)
+    b = ExampleBank(20, 49).append(k, k)
+    with pytest.raises(_lib.GpsrError, match="from 0"):
+        b.read(-5, 10)
+    for start, rows in ((4, 6), (9, 1), (10, 0), (25, 0)):
+        got = b.read(start, 8)
+        assert all((x[:rows] == 1).all() and not x[rows:].any() and len(x) == 8 for x in got)
