@@ -464,6 +464,8 @@ def _bank(bank, dev):
     if kc.dim() != 4 or bits not in (4, 8):
         raise _lib.GpsrError(f"bank: bits must be 4 or 8 and codes [pages,H,P,width], got {bits}, {tuple(kc.shape)}")
     pages, H, P, width = shape = kc.shape
+    if H < 1:
+        raise _lib.GpsrError("bank: no heads")
     D = width * 8 // bits
     groups = (pages, H, P, D // BANK_GROUP)
     if vc.shape != shape or ks.shape != groups or vs.shape != groups or off.shape != (pages, H, P) or cent.shape != (pages, H, D):

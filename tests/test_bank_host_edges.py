@@ -24,3 +24,16 @@ def test_more_rows_than_a_call_can_count_are_refused(rows):
     table = torch.empty(1, rows, dtype=torch.int32, device="meta")
     with pytest.raises(_lib.GpsrError, match="pages"):
         ops._bank_index(table, (torch.zeros(1, dtype=torch.int32),), -1, "bank_attend")
+
+
+def test_a_bank_without_heads_is_refused():
+    """Before the query heads are divided by its number of heads."""
+    from super_resolution_amd import _lib, ops
+    u8, f32 = (lambda *s: torch.zeros(s, dtype=torch.uint8)), (lambda *s: torch.zeros(s))
+    for heads in (0, 1):
+        bank = ops.Bank(u8(2, heads, 16, 32), u8(2, heads, 16, 2), u8(2, heads, 16, 32), u8(2, heads, 16, 2), f32(2, heads, 16), f32(2, heads, 64))
+        if heads:
+            assert ops._bank(bank, -1)[1:] == (1, 64)
+        else:
+            with pytest.raises(_lib.GpsrError, match="heads"):
+                ops._bank(bank, -1)
