@@ -387,8 +387,9 @@ int gpsr_active_sample(const double* data, int N, int D, int K, int n_pick, doub
  * skip[1] (leave-one-image-out).  A query that sees no row gets zeros (lse -inf).  Rows that a query does not see have no
  * influence, whatever they hold; of the rows that it does see, one whose key is NaN makes its output and lse NaN, one whose value
  * is NaN in a group of 32 columns makes its output NaN in those columns.  Sums, maxima and exponentials are kept in 32 bits, for
- * values of any held size; queries and weights enter the matrix units as one (bf16), two (f16) or three (f32) bf16 terms, so that
- * each type keeps its own precision.  Logits too are 32-bit numbers: a key so large that |k|^2 / 2 leaves their range has no weight,
+ * values of any held size.  Queries enter the matrix units as one (bf16), two (f16) or three (f32) bf16 terms, so that each type keeps
+ * its own precision; weights with 16 bits (f32: 24), but with 8 where more than 32 bf16 columns (queries x query heads of a bank
+ * head) attend to the whole bank, which adds up to 2^-8 of the mean of |value| to an output that is rounded by 2^-8 of itself.  Logits too are 32-bit numbers: a key so large that |k|^2 / 2 leaves their range has no weight,
  * whatever the query.  A query that is not a number gets NaN if it sees a row that has weight.
  * All entry points run on the given stream and wait for nothing; they may be captured into a graph.  Overlapping calls may read one
  * bank, each with a workspace of its own.  There are no gradients: a bank is filled and asked.

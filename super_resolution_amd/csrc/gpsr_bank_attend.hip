@@ -85,7 +85,7 @@ k_bank_attend(gpsr_bank bk, const int32_t* __restrict__ table, int table_pages, 
             if (pos >= lo && pos < hi) s[kb][e] = -__builtin_inff();
           }
       }
-      tile_accumulate<D, KT, NT, NB, W, decltype(move)::value>(tile, r, col, part, c2, above, s, st);
+      tile_accumulate<D, KT, (WK > 1 ? weight_terms(NT) : NT), NB, W, decltype(move)::value>(tile, r, col, part, c2, above, s, st);
     }
   };
   st.clear();

@@ -95,7 +95,7 @@ k_bank_pages_query(gpsr_bank bk, const int32_t* __restrict__ table, int table_pa
         for (int e = 0; e < X::E; ++e)
           if (skips(i * KT + wrow + kb * W + X::row(part, e))) s[kb][e] = -__builtin_inff();
     }
-    tile_accumulate<D, KT, NT, NB, W, true>(tile, wrow, col, part, c2, ABOVE, s, st);
+    tile_accumulate<D, KT, weight_terms(NT), NB, W, true>(tile, wrow, col, part, c2, ABOVE, s, st);
   }
   st.spoil();
   __syncthreads();
@@ -266,7 +266,7 @@ k_bank_pages_page(gpsr_bank bk, const int32_t* __restrict__ table, int table_pag
           if (pos >= lo && pos < hi) s[0][e] = -__builtin_inff();
         }
       }
-      tile_accumulate<D, KT, NT, NB, W, true>(tile, r, col, part, c2, ABOVE, s, st);
+      tile_accumulate<D, KT, weight_terms(NT), NB, W, true>(tile, r, col, part, c2, ABOVE, s, st);
     }
   }
   st.spoil();

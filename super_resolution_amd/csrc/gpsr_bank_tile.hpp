@@ -5,8 +5,12 @@
 // the softmax statistics are lane-local but for an exchange between the wave's parts, and the accumulator registers, rounded
 // to bf16, are the second product's operand as they are: O^T = V^T P^T contracts over rows, and the order of a contraction is
 // free as long as both operands agree, so V^T is laid out in LDS in the order in which the accumulators hold the rows.
-// Held values have at most 4 significant bits: bf16 holds them exactly.  Queries and weights are split into Terms<DT>::N bf16
-// terms (8 bits each: bf16 queries 1, f16 2, f32 3), so that the products lose nothing that the caller's type can hold.
+// Held values have at most 4 significant bits: bf16 holds them exactly.  Queries are split into Terms<DT>::N bf16 terms
+// (8 bits each: bf16 queries 1, f16 2, f32 3), so that the products lose nothing that the caller's type can hold.  Weights are
+// not the caller's; they enter with at least twice the bits of a bf16 output (16; f32 24) wherever that costs little: few queries and
+// chosen pages wait for memory (a second term took pages_image of 40 000 queries from 125 to 129 us, others not measurably
+// longer).  Many bf16 queries over the whole bank keep one term of 8 bits, which adds up to 2^-8 of the mean |value| to an
+// output that is rounded by 2^-8 of itself: two took 65 025 queries of 5000 rows from 127 to 164 us, 40 000 of 100 000 from 1190 to 1700.
 #pragma once
 #include "gpsr_bank.hpp"
 
@@ -41,6 +45,9 @@ template <int DT> struct Terms;
 template <> struct Terms<GPSR_BF16> { static constexpr int N = 1; };
 template <> struct Terms<GPSR_F16> { static constexpr int N = 2; };
 template <> struct Terms<GPSR_F32> { static constexpr int N = 3; };
+
+// terms of the weights where the matrix units are not what a call waits for
+static constexpr int weight_terms(int nt) { return nt < 2 ? 2 : nt; }
 
 // registers that a wave of 32 columns and NB x 32 rows at a time needs, roughly: sums, logits, query terms, the rest
 static constexpr int tile_regs(int d, int nt, int nb) { return d / 2 + 16 * nb + nt * d / 4 + 64; }
@@ -514,7 +521,8 @@ __device__ __forceinline__ void tile_marks(const Tile<D, KT>& tile, int wrow, un
 //   otherwise it stays, which saves the maximum of every tile and the wait for it: bf16 and the sums have range to spare, and
 //     their precision is relative.  Soft::wants_move says when it has to be moved (nothing seen yet, or a sum past 2^40); what
 //     a weight far above the reference does is for the caller to look for (Soft::lost), and to walk again with MOVE only.
-template <int D, int KT, int NT, int NB, int W, bool MOVE>
+// WT: bf16 terms of the weights.
+template <int D, int KT, int WT, int NB, int W, bool MOVE>
 __device__ __forceinline__ void tile_accumulate(const Tile<D, KT>& tile, int r0, int col, int part, float c2, float above,
                                                 typename Geo<W>::Acc (&s)[NB], Soft<D, W>& st) {
   typedef Geo<W> X;
@@ -551,13 +559,13 @@ __device__ __forceinline__ void tile_accumulate(const Tile<D, KT>& tile, int r0,
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] = s[2 * k + e / 4][e % 4];
     }
-    bf8 p[NT];
-    split_terms<NT>(y, p);
+    bf8 p[WT];
+    split_terms<WT>(y, p);
 #pragma unroll
     for (int d = 0; d < D / W; ++d) {
       const bf8 a = *(const bf8*)(tile.v + Tile<D, KT>::at(d * W + col, r0 + k * X::STEP + part * 8));
 #pragma unroll
-      for (int t = 0; t < NT; ++t) st.o[d] = X::mul(a, p[t], st.o[d]);
+      for (int t = 0; t < WT; ++t) st.o[d] = X::mul(a, p[t], st.o[d]);
     }
   }
 }

@@ -99,6 +99,22 @@ def test_columns_at_both_ends_of_the_range(dtype, T):
     c.check(q, out, lse, 0.25, lambda b, t, h: np.ones(900, bool))
 
 
+@pytest.mark.parametrize("T,whole", [(1, True), (3, True), (30, True), (40, False), (2900, False)])
+def test_weights_of_bf16_callers_keep_16_bits_where_few_ask_or_pages_are_chosen(T, whole, monkeypatch):
+    """The general bound with 2^-16 in place of 2^-8 for the weights; means of signed values, so that they are smaller than A."""
+    import test_gpu_bank
+    monkeypatch.setitem(test_gpu_bank.U_W, BF16, 2.0 ** -16)
+    ops = _ops()
+    c = Case([900], 1, 64, 32, 4, "RBF", BF16, seed=T + 2)
+    q, qd = c.queries(T, 1, BF16)
+    if whole:
+        out, lse = ops.bank_attend(c.bank, c.table, c.length, qd, 0.25, want_lse=True)
+        c.check(q, out, lse, 0.25, lambda b, t, h: np.ones(900, bool))
+    sel, seen = _choices(c, T, 4 if T < 40 else 16)
+    out, lse = ops.bank_attend_pages(c.bank, c.table, c.length, qd, sel, 0.25, want_lse=True)
+    c.check(q, out, lse, 0.25, seen)
+
+
 # ------------------------------------------------------------ the screen of bank_select
 def _screened(c, qd, n_sel):
     """bank_select through the library with a workspace of our own: the choice, and how many candidates the screen left each query
