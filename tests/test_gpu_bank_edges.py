@@ -253,6 +253,16 @@ def test_two_streams_at_once_with_many_queries():
             assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
 
 
+def test_agpr_with_a_bank_by_page(tmp_path, golden_dir, monkeypatch):
+    """1564 windows with 16 pages of 64 rows each go by page; fewer pages would go by query."""
+    import test_gpu_agpr_bank
+    from super_resolution_amd import _lib, ops
+    ref, _, _ = ops._bank(ops.bank_alloc(47, 1, 64), torch.cuda.current_device())
+    size = _lib.load().gpsr_bank_attend_pages_workspace_bytes
+    assert size(ref, 1, 47, 1564, 1, 16, 0) > 0 and size(ref, 1, 47, 1564, 1, 4, 0) == 0
+    test_gpu_agpr_bank.test_agpr_with_a_bank_runs_as_its_definition(tmp_path, golden_dir, monkeypatch, 16)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 def test_many_columns_are_the_same_every_time_in_the_other_ways_too(dtype):
     """Banks shared out and joined, pages by query, and the choice by the screen and without it: every bit the same."""
