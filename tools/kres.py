@@ -7,8 +7,8 @@ import sys
 import tempfile
 
 src = sys.argv[1] if len(sys.argv) > 1 else "super_resolution_amd/csrc/gpsr_api.hip"
-with tempfile.NamedTemporaryFile(suffix=".so") as tmp:
-    out = subprocess.run(["/opt/rocm/bin/hipcc", "-O3", "--offload-arch=gfx950", "-ffp-contract=off", "-fPIC", "-shared",
+with tempfile.NamedTemporaryFile(suffix=".o") as tmp:
+    out = subprocess.run(["/opt/rocm/bin/hipcc", "-O3", "--offload-arch=gfx950", "-ffp-contract=off", "-c", "--offload-device-only",
                           "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
                           "-Rpass-analysis=kernel-resource-usage", "-o", tmp.name, src] + sys.argv[2:],
                          capture_output=True, text=True).stderr
