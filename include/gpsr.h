@@ -432,7 +432,7 @@ int gpsr_bank_attend(const gpsr_bank* bank, const int32_t* table, int B, int tab
  * The n_sel (1..64) best pages for each query and bank head: sel [B][T][heads][n_sel], logical page numbers (table
  * columns) in ascending order, -1 behind the last one.  Score of a page with centroid c: the sum over the query heads of
  * the bank head of q.c (- |c|^2 / 2 for RBF), in 64 bits; equal scores: the lower page first.  A page can be chosen if
- * its table entry exists, it has a row below length[b] that the query does not skip, and its centroid is a number.
+ * its table entry exists, it has a row below length[b] that the query does not skip, and its score is a number.
  */
 size_t gpsr_bank_select_workspace_bytes(const gpsr_bank* bank, int B, int table_pages, int T, int q_heads, int n_sel, int dtype);
 int gpsr_bank_select(const gpsr_bank* bank, const int32_t* table, int B, int table_pages, const int32_t* length,
@@ -452,7 +452,8 @@ int gpsr_bank_attend_pages(const gpsr_bank* bank, const int32_t* table, int B, i
 /*
  * Images to bank rows and back (the window loops of agpr.py:165-185 for a bank).  side odd, 3..15, side * side <= dim.
  *   gpsr_bank_windows: the side x side window of every pixel that has a whole one, row by row: out [(H-side+1)*(W-side+1)][dim]
- *     of dtype, columns behind side*side zero; centre != 0: less the window's own mean (taken in 64 bits).
+ *     of dtype, columns behind side*side zero; centre != 0: less the window's own mean (taken in 64 bits);
+ *     rounded to 32 bits, then to dtype.
  *   gpsr_bank_blend: out[H][W] = img + the mean, over the windows that hold the pixel, of what they say about it (detail, laid out as
  *     gpsr_bank_windows lays them out), summed in 64 bits in the windows' order.
  */

@@ -5,11 +5,12 @@
 // Columns are the (query, head) pairs that share a bank head.  A workgroup of NW waves walks the rows of its split of the
 // bank, KT at a time, NB x W of them in one step:
 //   WK = 1 (many queries): all threads decode a tile to LDS once, then each wave multiplies it with W columns of its own.
-//     Bound by the exponentials and the matrix units together: 40 000 queries of 100 000 rows x 64 columns 1130 to 1180 us, 870 to
-//     910 TFLOP/s, where a library's product of 8192^3 reaches 1120.
+//     Bound by the exponentials and the matrix units together: 40 000 queries of 100 000 rows x 64 columns 1140 to 1200 us, 855 to
+//     900 TFLOP/s, where a library's product of 8192^3 reaches 1120.
 //   WK = NW (few queries): all waves have the same columns, each walks every NW-th tile in LDS of its own, so that none waits
 //     for another, and the results are joined at the end.  Bound by reading the bank and waiting for it: 12 queries to each of 8
-//     banks of up to 180 000 rows x 128 columns in 4 bits, 154 MB, 61 us, 2.5 TB/s.
+//     banks of up to 180 000 rows x 128 columns in 4 bits, 154 MB, 62 us, 2.5 TB/s; the
+//     longest bank's waves walk 22 tiles where the mean is 17, since all entries of a call share one number of splits.
 // AHEAD: tiles under way besides the one in LDS.
 template <int DT, int BITS, int D, int W, int NW, int WK, int KT, int NB, int AHEAD>
 __global__ void __launch_bounds__(64 * NW, WK > 1 ? 2 : tile_waves(D, Terms<DT>::N, NB))
@@ -172,7 +173,9 @@ static Plan plan_of(const gpsr_bank* bk, int B, int table_pages, int T, int q_he
   // Or one workgroup on each CU with 64 rows at a time in twice the registers.  At 64 columns a tile of 128 rows takes a CU's two
   // workgroups of 4 waves a SIMD 4.4 us (and starting and ending one as much as 4 tiles), the lone one 2.95; partials cost 0.13 ns
   // a column and split, and the join 10 us.  So it pays where the columns just fill the CUs and the bank is short: 65 025 queries
-  // of 5000 rows 124 us instead of 136 (but 40 000 of 100 000 rows 1470 instead of 1150).
+  // of 5000 rows 137 us instead of 150, of 1000 rows 37 instead of 68 (but 40 000 of 100 000 rows 1470 instead of 1150).  The other form
+  // that has both, 32 columns in f32, keeps their ratio: 40 000 to 131 072 queries of 1000 to 20 000 rows up to 35 % sooner at 1000 and
+  // 2500 rows and within 4 % elsewhere, but for 40 000 of 2500 (98 instead of 91) and 50 000 of 5000 (189 instead of 171).
   if (!p.few && lone_nb(bk->dim, nt) && p.splits > 1) {
     const double split = ((wgs * p.splits + slots - 1) / slots) * ((tiles + p.splits - 1) / p.splits + 4) * 4.4 + 10 + 0.13e-3 * (double)C * bk->heads * B * p.splits;
     const double lone = ((wgs + 255) / 256) * (tiles + own) * 2.95;

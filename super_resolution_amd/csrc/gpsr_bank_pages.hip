@@ -6,7 +6,7 @@
 //   by page: the choices are turned over (for each page the list of queries that chose it), a workgroup takes one page and
 //     128 of its queries, writes each query's partial result for that page, and a last kernel joins each query's partials.
 //     Pages are decoded once per 128 queries and all columns work, at the price of writing and reading the partials: 40 000
-//     queries with 16 pages each 125 us (count 15, shares 10, scan 5, fill 8, products 68, join 25), by query 4380.  Partials are
+//     queries with 16 pages each 129 us (count 14, shares 10, scan 5, fill 8, products 73, join 26), by query 4380.  Partials are
 //     f32 whatever the caller's type: their sums are weighed against each other by their keys alone, and a column may be any
 //     number of powers of two under its neighbours (in f16 with a power of two a row, products took 59 and the join 19 us, but
 //     columns 2^-25 under the row's largest became zero).
@@ -209,8 +209,8 @@ k_bank_pages_fill(const int32_t* __restrict__ sel, int n_sel, int table_pages, i
   list[start[(size_t)b * buckets + bucket] + share + r] = (int)(th / H * n_sel + (e - th * n_sel));
 }
 
-// 32 rows at a time and three waves per SIMD: the workgroups are short and mostly wait (68 us for 40 000 queries x 16 pages of
-// 64 rows of 64 columns, 154 TFLOP/s; measured with f16 partials, at 59 us, all 64 rows of a page at a time took 4 us more, two
+// 32 rows at a time and three waves per SIMD: the workgroups are short and mostly wait (73 us for 40 000 queries x 16 pages of
+// 64 rows of 64 columns, 144 TFLOP/s; measured with f16 partials, at 59 us, all 64 rows of a page at a time took 4 us more, two
 // waves 15 more, four with spills 30 more)
 template <int DT, int BITS, int D, int KT>
 __global__ void __launch_bounds__(256, tile_waves(D, Terms<DT>::N, 1) > 3 ? 3 : tile_waves(D, Terms<DT>::N, 1))
@@ -284,7 +284,7 @@ static PagesPlan plan_of(const gpsr_bank* bk, int B, int table_pages, int T, int
   // By page where that is sooner.  A query (and 16 or 32 of its heads) costs 4 ns and 15 ps a row at 64 columns; by page, six
   // launches 25 us more, a page 6.5 ns and a choice 0.08 ns; more columns cost (dim / 64)^1.5 times as much.  Both sides measured for
   // 256 to 8192 queries of 4 or 16 pages, 16 or 64 rows, 32 to 6250 pages, 64 and 256 columns: 2048 queries of 16 x 64 rows
-  // 49 us by query, 45 by page (1563 pages); 512 queries 20 and 44; 512 queries of 256 columns 95 and 121, 1024 190 and 125; 8192
+  // 49 us by query, 50 by page (1563 pages); 512 queries 20 and 44; 512 queries of 256 columns 95 and 121, 1024 190 and 125; 8192
   // queries of 16 x 16 rows of 6250 pages 72 and 86.
   const int width = G <= 16 ? 16 : 32;
   p.groups = (G + width - 1) / width;

@@ -258,7 +258,8 @@ extern "C" int gpsr_bank_read(const gpsr_bank* bank, const int32_t* table, int B
 // ---------------------------------------------------------------- images to rows and back
 // WI_X neighbouring windows of an image row a workgroup: their pixels go through LDS once (a window shares all but a column of them
 // with the next), four threads take a window's mean, then a thread makes 8 columns of a window at a time, one store.  Bound by the
-// stores: 8.3 million windows of 7 x 7 pixels as 64 bf16 columns 363 us, 3.1 TB/s (a wave a window, two bytes a store, 1480 us).
+// stores: 8.3 million windows of 7 x 7 pixels as 64 bf16 columns 345 us (384 without their means), 3.1 TB/s (a wave a window, two bytes
+// a store, 1480 us).
 #define WI_X 64
 template <int DT>
 __global__ void __launch_bounds__(256)
@@ -307,7 +308,7 @@ k_bank_windows(const double* __restrict__ img, int W, int side, bool centre, int
 // A workgroup has BL_X x BL_Y pixels and walks the rows of windows that reach them; each row's windows, contiguous in memory, go
 // through LDS.  Thread (x, s) sums for the pixel of column x whose row is s modulo side: side neighbouring rows are being
 // summed at a time, and a window row is the first of one of them and the last of another.  Every pixel's sum so runs over its
-// windows in their order.  The same 8.3 million windows back to pixels 376 us, 3.1 TB/s (a thread a pixel that reads its windows
+// windows in their order.  The same 8.3 million windows back to pixels 329 us, 3.2 TB/s (a thread a pixel that reads its windows
 // itself, side * side cache lines for as many values, 6900 us).
 #define BL_X 32
 #define BL_Y 16

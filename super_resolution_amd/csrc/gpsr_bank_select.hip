@@ -13,7 +13,7 @@
 // at most 3 u^2 |q||c| (one exact term of q: u^2 |q||c|); the 32-bit sum of n products and the offset o adds (n + 2) 2^-23
 // (|q||c| + |o|), n = 3 dim (2 dim); 1e-35 (1 + |q| + |c|) covers subnormal terms.  Norms above 1e18 are not screened: their pages
 // are all candidates.  A page whose centroid is not a number is passed over, as one that does not exist: it is never chosen.
-// 40 000 queries of 64 columns, 1563 pages, 16 of them: prepare 5, screen 104, pick 25 us, one product after the other 127 us
+// 40 000 queries of 64 columns, 1563 pages, 16 of them: prepare 5, screen 104, pick 25 us, one after the other 125 us; one product
 // at its rate in 32 bf16 terms 14; exact scores for all pages took 14 900 us.
 #include "gpsr_bank_tile.hpp"
 

@@ -8,8 +8,8 @@
 // Held values have at most 4 significant bits: bf16 holds them exactly.  Queries are split into Terms<DT>::N bf16 terms
 // (8 bits each: bf16 queries 1, f16 2, f32 3), so that the products lose nothing that the caller's type can hold.  Weights are
 // not the caller's; they enter with at least twice the bits of a bf16 output (16; f32 24) wherever that costs little: few queries and
-// chosen pages wait for memory (a second term took pages_image of 40 000 queries from 125 to 129 us, others not measurably
-// longer).  Many bf16 queries over the whole bank keep one term of 8 bits, which adds up to 2^-8 of the mean |value| to an
+// chosen pages wait for memory (a second term took pages_image of 40 000 queries from 125 to 129 us, 12 to
+// each of 8 long banks from 57 to 60, 30 to each of 4 of 256 columns from 152 to 160, small calls not measurably).  Many bf16 queries over the whole bank keep one term of 8 bits, which adds up to 2^-8 of the mean |value| to an
 // output that is rounded by 2^-8 of itself: two took 65 025 queries of 5000 rows from 127 to 164 us, 40 000 of 100 000 from 1190 to 1700.
 #pragma once
 #include "gpsr_bank.hpp"
@@ -578,8 +578,9 @@ template <int DT, int D, int WJ = 1>
 __global__ void __launch_bounds__(256)
 k_bank_join(const float* __restrict__ sums, const f2v* __restrict__ stats, int T, int G, int H, int64_t C, int n, size_t per_bh,
             size_t per_g, size_t per_t, size_t per_i, typename Row<DT>::T* __restrict__ out, float* __restrict__ lse) {
-  // Weights and sums go from lane to lane through LDS, a wave's own part of it; reading other lanes' registers by
-  // permutes, 28 of them under way at a time, has given other lanes' values now and then in the f32 form of this kernel.
+  // Weights and sums go from lane to lane through LDS, a wave's own part of it.  With permutes (ds_bpermute) the f32 form of 32 columns
+  // added other lanes' values to one column in 3000, never the same ones; why is not known: its assembly reads right, and the other
+  // types' forms, with as many permutes under way, never showed it.  Tests repeat every way over tens of thousands of columns.
   __shared__ float tops[4], ls[4], weight[4][64];
   __shared__ __attribute__((aligned(16))) float part[4][64][4];
   const auto sync = [] { asm volatile("" ::: "memory"); __builtin_amdgcn_wave_barrier(); };

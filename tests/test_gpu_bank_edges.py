@@ -8,7 +8,7 @@ import torch
 
 pytestmark = pytest.mark.gpu
 
-from test_gpu_bank import BF16, F16, F32, Case, _ops, held
+from test_gpu_bank import BF16, F16, F32, Case, _ops, _skips, held
 
 
 def _rewrite(c, kernel="RBF"):
@@ -113,6 +113,24 @@ def test_weights_of_bf16_callers_keep_16_bits_where_few_ask_or_pages_are_chosen(
     sel, seen = _choices(c, T, 4 if T < 40 else 16)
     out, lse = ops.bank_attend_pages(c.bank, c.table, c.length, qd, sel, 0.25, want_lse=True)
     c.check(q, out, lse, 0.25, seen)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("D", [32, 128, 192])
+def test_many_queries_of_the_other_numbers_of_columns(dtype, bits, D):
+    """More than 32 columns of a bank head, so that a tile is shared by the waves of a workgroup."""
+    ops = _ops()
+    c = Case([300, 7], 1, D, 32, bits, "RBF", dtype, seed=D)
+    q, qd = c.queries(70, 2, dtype)
+    s = float(np.float32(1.0 / math.sqrt(D)))
+    skip, sd = _skips(2, 70, c.lengths, c.rng, c.dev)
+    out, lse = ops.bank_attend(c.bank, c.table, c.length, qd, s, skip=sd, want_lse=True)
+
+    def seen(b, t, h):
+        r = np.arange(c.lengths[b])
+        return ~((r >= skip[b, t, 0]) & (r < skip[b, t, 1]))
+    c.check(q, out, lse, s, seen)
 
 
 # ------------------------------------------------------------ the screen of bank_select
